@@ -17,10 +17,10 @@ import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
-SRC = [os.path.join(HERE, "csrc", n) for n in ("rp_spgemm.hip", "rp_libsvm.hip", "rp_dense.hip")]
+SRC = [os.path.join(HERE, "csrc", n) for n in ("rp_spgemm.hip", "rp_libsvm.hip", "rp_dense.hip", "rp_id.hip")]
 # every file the compile reads (relative to the repo root): the id covers all of them
 DEPS = ["randomprojection_amd/csrc/rp_spgemm.hip", "randomprojection_amd/csrc/rp_libsvm.hip",
-        "randomprojection_amd/csrc/rp_dense.hip", "randomprojection_amd/csrc/rp_common.h",
+        "randomprojection_amd/csrc/rp_dense.hip", "randomprojection_amd/csrc/rp_id.hip", "randomprojection_amd/csrc/rp_common.h",
         "randomprojection_amd/csrc/rp_pow5.h", "include/rp.h"]
 OUT = os.path.join(HERE, "librp.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
@@ -28,6 +28,9 @@ FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
     # scipy's csr_matmat rounds the multiply and the add separately: never contract to FMA
     "-ffp-contract=off", "-fno-fast-math", "-Wall",
+    # no packed f32 instructions (v_pk_mul_f32 and the like): some of their forms have given wrong
+    # results on this hardware now and then (hipcc's host pass does not know the feature: a warning)
+    "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
 ]
 MARKER = b"rp-src-sha16:"
 CC_MARKER = b"rp-cc-sha16:"

@@ -3227,21 +3227,6 @@ const char* rp_version(void) { return "rp-mi355x 0.1 (gfx950)"; }
 
 int rp_abi_version(void) { return RP_ABI_VERSION; }
 
-// The sha256 prefix of every source this library was compiled from (build.py passes it as
-// RP_SRC_SHA16 and also finds it in the binary through the marker), so a benched or tested number
-// names the binary that produced it and a stale build is refused (build.py / _native.load).
-#ifndef RP_SRC_SHA16
-#define RP_SRC_SHA16 "unknown"
-#endif
-__attribute__((used)) static const char kBuildMarker[] = "rp-src-sha16:" RP_SRC_SHA16;
-// the compiler identity hash (build.py compiler_hash) the source id above includes: the loader
-// recomputes the id with it instead of running the compiler
-#ifndef RP_CC_SHA16
-#define RP_CC_SHA16 "unknown"
-#endif
-__attribute__((used)) static const char kCcMarker[] = "rp-cc-sha16:" RP_CC_SHA16;
-const char* rp_build_id(void) { return kBuildMarker + 13; }
-
 int rp_device_count(int* count) {
     if (!count) return fail(RP_ERR_INVALID, "NULL count");
     int n = 0;

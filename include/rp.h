@@ -329,6 +329,68 @@ int rp_synth_libsvm_device(int device, int64_t n_rows, const int64_t* indptr, co
 int rp_dense_project_device(int device, const void* X, int32_t dtype, int64_t n, int64_t m, const void* G,
                             int64_t p, void* Y, int64_t ldy, void* stream, int32_t variant);
 
+/* Low-rank adapters of many requests beside the dense projection. Row i of X has the adapter
+ * a = ids[i] (int32, device; a row whose id is outside 0 .. adapters - 1 has none):
+ *   hidden_i = down[a] x_i,   y_i = C x_i + scale[a] up[a]^T hidden_i
+ * dtype RP_BF16 or RP_F32 is the type of X, C, down and up; products are exact and summed in f32, Y
+ * and hidden are f32. With s = 64 (bf16) or 32 (f32), mk and pk are m and p rounded up to a multiple
+ * of s: X is n x mk (row stride ldx), C p x mk, down adapters x rank x mk, up adapters x rank x pk, zeros
+ * in the columns past m or p, all device arrays with 16-byte aligned rows. rank <= 128 (an adapter of
+ * a smaller rank is padded with zero rows), adapters <= 65535. scale: device f32, one for each
+ * adapter, or NULL (1). Y: n x p, row stride ldy. hidden: n x rank (contiguous, zeros for rows without
+ * an adapter) or NULL when the backward pass is not wanted. workspace: rp_adapt_workspace_bytes bytes,
+ * 256-byte aligned, in use until the call's work on `stream` is done. Asynchronous on `stream`; does
+ * not synchronise or allocate, so it can be captured into a graph. No reference counterpart. */
+#define RP_ADAPT_PROJECT 0
+#define RP_ADAPT_GRADIENTS 1
+#define RP_ADAPT_GRADIENTS_DX 2
+/* bytes of workspace of a call: what = RP_ADAPT_PROJECT, _GRADIENTS (without dX) or _GRADIENTS_DX; -1 for
+ * arguments the call would refuse */
+int64_t rp_adapt_workspace_bytes(int32_t dtype, int64_t n, int64_t m, int64_t p, int64_t adapters, int32_t rank,
+                                 int32_t what);
+int rp_adapt_project_device(int device, const void* X, int64_t ldx, int32_t dtype, int64_t n, int64_t m, const void* C,
+                            int64_t p, const void* down, const void* up, int64_t adapters, int32_t rank,
+                            const float* scale, const int32_t* ids, float* Y, int64_t ldy, float* hidden,
+                            void* workspace, int64_t workspace_bytes, void* stream);
+/* Its backward pass: from dY (n x pk, row stride lddy) and the forward pass's hidden,
+ *   t_i = scale[a] up[a] dy_i,   dX = dY C + down[a]^T t_i (in dtype, n x m, row stride lddx)
+ *   d_down[g] = sum of t_i x_i^T,   d_up[g] = scale[g] sum of hidden_i dy_i^T   (over g's rows; f32)
+ * Ct is C transposed (m x pk, zeros past p); with Ct and dX NULL the rows' gradient is left out. d_down
+ * is adapters x rank x m and d_up adapters x rank x p, with their strides between rows and between
+ * adapters; every element is written, zeros for an adapter without rows. Sums run in an order that
+ * depends on the arguments alone: the same call gives the same bits. C is frozen: no gradient. */
+int rp_adapt_gradients_device(int device, const void* dY, int64_t lddy, const void* X, int64_t ldx, int32_t dtype,
+                              int64_t n, int64_t m, int64_t p, const void* Ct, const void* down, const void* up,
+                              int64_t adapters, int32_t rank, const float* scale, const int32_t* ids,
+                              const float* hidden, void* dX, int64_t lddx, float* d_down, int64_t d_down_row,
+                              int64_t d_down_adapter, float* d_up, int64_t d_up_row, int64_t d_up_adapter,
+                              void* workspace, int64_t workspace_bytes, void* stream);
+
+/* An AdamW step over many tensors at once (f32 parameters; gradients all f32 or all bf16):
+ *   m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;
+ *   w = w (1 - lr decay) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+ * with a step count t of each tensor's own. A handle is made over buffers the caller keeps alive and in
+ * place: params, grads (read at every step), copies (NULL, or for each tensor a bf16 array that
+ * receives the rounded new parameters) and the states. Tensor t's states start at 256-element block
+ * b(t) = sum over earlier tensors of ceil(numel / 256). state_bits 32: exp_avg and exp_avg_sq hold f32
+ * m and v. state_bits 8: exp_avg holds e4m3 codes of m, exp_avg_sq unsigned codes of sqrt(v) (5 bits of
+ * exponent, 3 of mantissa), one byte each, exp_avg_scale and root_scale a byte for each block (rp_optim.hip has
+ * the format). steps: int32 for each tensor. A tensor may be empty. All are device arrays. */
+typedef struct rp_adamw rp_adamw;
+int rp_adamw_create(int device, int32_t n_tensors, const int64_t* numels, float* const* params,
+                    const void* const* grads, int32_t grad_type, uint16_t* const* copies, int32_t state_bits,
+                    void* exp_avg, void* exp_avg_sq, uint8_t* exp_avg_scale, uint8_t* root_scale, int32_t* steps,
+                    rp_adamw** out);
+/* One step, asynchronous on `stream` and capturable (step counts live on the device; lr and the other
+ * numbers are those of the call). active: NULL, or a device byte for each tensor: 0 leaves that tensor, its
+ * states and its step count as they are. seed: of the random rounding to 8 bits, hashed with the step count, the
+ * tensor's number and the element's. Calls on one handle must be ordered by the caller. */
+int rp_adamw_step(rp_adamw* h, double lr, double beta1, double beta2, double eps, double weight_decay, uint64_t seed,
+                  const uint8_t* active, void* stream);
+/* state_bits 8: all blocks' m and sqrt(v) as the f32 values the codes stand for (256 per block) */
+int rp_adamw_values(rp_adamw* h, float* exp_avg, float* root, void* stream);
+int rp_adamw_destroy(rp_adamw* h);
+
 #ifdef __cplusplus
 }
 #endif

@@ -14,6 +14,7 @@ RP_OK, RP_ERR_INVALID, RP_ERR_HIP, RP_ERR_CAPACITY, RP_ERR_UNSUPPORTED, RP_ERR_N
 RP_I32, RP_I64, RP_F32, RP_F64, RP_BF16 = 1, 2, 3, 4, 5
 RP_LAYOUT_AUTO, RP_LAYOUT_GENERIC, RP_LAYOUT_PACKED = 0, 1, 2
 RP_ORDER_SCIPY, RP_ORDER_SORTED = 0, 1
+RP_ADAPT_PROJECT, RP_ADAPT_GRADIENTS, RP_ADAPT_GRADIENTS_DX = 0, 1, 2
 RP_OPT_PIPELINE, RP_OPT_DEFER_POLLS, RP_OPT_DEFER_TICKS, RP_OPT_CHUNK_ROWS, RP_OPT_HOST_THREADS = 1, 2, 3, 4, 5
 # include/rp.h RP_ABI_VERSION these bindings are written against (signatures below)
 ABI_VERSION = 6
@@ -28,6 +29,8 @@ EXPORTS = (
     "rp_project_host_begin", "rp_result_fetch", "rp_result_free", "rp_project",
     "rp_synth_rows_device", "rp_libsvm_parse_device", "rp_libsvm_project_stream", "rp_synth_libsvm_device", "rp_project_stream", "rp_project_stream_stats", "rp_host_alloc", "rp_host_free",
     "rp_dense_project_device",
+    "rp_adapt_workspace_bytes", "rp_adapt_project_device", "rp_adapt_gradients_device",
+    "rp_adamw_create", "rp_adamw_step", "rp_adamw_values", "rp_adamw_destroy",
 )
 
 
@@ -169,6 +172,15 @@ def load(path: str = None, verify: bool = None):
         "rp_synth_rows_device": (ctypes.c_int, [ctypes.c_int, i64, i64, dbl, i32, i32, dbl, ctypes.c_uint64,
                                                 vp, i32, vp, vp, vp, P(i64)]),
         "rp_dense_project_device": (ctypes.c_int, [ctypes.c_int, vp, i32, i64, i64, vp, i64, vp, i64, vp, i32]),
+        "rp_adapt_workspace_bytes": (i64, [i32, i64, i64, i64, i64, i32, i32]),
+        "rp_adapt_project_device": (ctypes.c_int, [ctypes.c_int, vp, i64, i32, i64, i64, vp, i64, vp, vp, i64, i32, vp, vp,
+                                                   vp, i64, vp, vp, i64, vp]),
+        "rp_adapt_gradients_device": (ctypes.c_int, [ctypes.c_int, vp, i64, vp, i64, i32, i64, i64, i64, vp, vp, vp, i64,
+                                                     i32, vp, vp, vp, vp, i64, vp, i64, i64, vp, i64, i64, vp, i64, vp]),
+        "rp_adamw_create": (ctypes.c_int, [ctypes.c_int, i32, vp, vp, vp, i32, vp, i32, vp, vp, vp, vp, vp, P(vp)]),
+        "rp_adamw_step": (ctypes.c_int, [vp, dbl, dbl, dbl, dbl, dbl, ctypes.c_uint64, vp, vp]),
+        "rp_adamw_values": (ctypes.c_int, [vp, vp, vp, vp]),
+        "rp_adamw_destroy": (ctypes.c_int, [vp]),
         "rp_libsvm_parse_device": (ctypes.c_int, [ctypes.c_int, vp, i64, i64, vp, vp, i32, vp, vp, i64, i64, vp,
                                                   P(i64), P(i64), P(i64)]),
         "rp_libsvm_project_stream": (ctypes.c_int, [vp, vp, i64, i32, i64, vp, i64, P(CsrOut), P(i64), P(i64),

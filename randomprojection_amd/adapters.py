@@ -1,0 +1,201 @@
+"""Low-rank adapters of many requests beside the dense projection, and their gradients.
+
+``gaussian.dense_project_device`` projects every row by one frozen matrix C (p x m). Here G adapters of rank R
+stand beside it, in two banks with the long axis contiguous: ``down`` (G x R x m) and ``up`` (G x R x p). Row i
+of X belongs to the adapter ``a = ids[i]`` (a row whose id is outside 0 .. G-1 has none):
+
+    hidden_i = down[a] x_i            y_i = C x_i + scale[a] up[a]^T hidden_i
+
+so one call serves rows of many tenants, each with a small learned part of its own, whether a request
+brings one row or many. The backward pass gives the gradients of the banks and, where wanted, of X; C is
+frozen and has none. An adapter of a smaller rank is padded with zero rows, which stay zero in training.
+
+"bf16" takes X, C and the banks in bfloat16, "fp32" in float32; products are exact and summed in float32 in both,
+and Y, hidden and the banks' gradients are float32 (no reference counterpart; csrc/rp_adapt.hip).
+"""
+from __future__ import annotations
+
+import ctypes
+
+from . import _native as nat
+from .gaussian import _STEP
+
+__all__ = ["adapted_project_device", "adapted_project_backward_device", "prepare_bank", "MAX_RANK"]
+
+MAX_RANK = 128
+_CODE = {"bf16": nat.RP_BF16, "fp32": nat.RP_F32}
+
+
+def _dtype(compute):
+    import torch
+
+    if compute not in _CODE:
+        raise ValueError("compute must be 'fp32' or 'bf16'")
+    return torch.bfloat16 if compute == "bf16" else torch.float32
+
+
+def prepare_bank(W, compute: str):
+    """W cast to the compute type, contiguous, its last axis padded with zeros to the kernels' multiple: what
+    ``prepared=True`` expects of C, Ct, down and up. Returned as it is where it is all that already."""
+    import torch
+
+    W = W.to(_dtype(compute))
+    pad = -W.shape[-1] % _STEP[compute]
+    if pad:
+        W = torch.nn.functional.pad(W, (0, pad))
+    W = W.contiguous()
+    return W if W.data_ptr() % 16 == 0 else W.clone()
+
+
+def _rows(X, compute):
+    """X as the kernels read it: itself where rows follow each other, aligned and without need of padding, else a copy."""
+    return prepare_bank(X, compute)
+
+
+def _ld(X):
+    return max(X.stride(0), X.shape[1])
+
+
+def _operand(name, W, shape, compute, prepared):
+    """``shape``: the expected sizes, the last one before padding."""
+    if prepared:
+        want = (*shape[:-1], shape[-1] + -shape[-1] % _STEP[compute])
+        if tuple(W.shape) != want or W.dtype != _dtype(compute) or not W.is_contiguous() or W.data_ptr() % 16:
+            raise ValueError(f"prepared {name} must be a contiguous 16-byte aligned {_dtype(compute)} tensor of shape "
+                             f"{want}, got {W.dtype} {tuple(W.shape)}")
+        return W
+    if tuple(W.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(W.shape)}")
+    return prepare_bank(W, compute)
+
+
+def _check_common(X, down, up, ids, scale, compute):
+    import torch
+
+    _dtype(compute)
+    if X.dim() != 2 or down.dim() != 3 or up.dim() != 3:
+        raise ValueError("X must be 2-D, down and up 3-D (adapters, rank, width)")
+    if down.shape[:2] != up.shape[:2] or 0 in down.shape:
+        raise ValueError(f"down {tuple(down.shape)} and up {tuple(up.shape)} must have the same, positive, number of "
+                         "adapters and rank")
+    if down.shape[1] > MAX_RANK or down.shape[0] > 65535:
+        raise ValueError(f"at most 65535 adapters of rank {MAX_RANK}, got {down.shape[0]} of rank {down.shape[1]}")
+    if ids.dtype != torch.int32 or tuple(ids.shape) != (X.shape[0],) or not ids.is_contiguous():
+        raise ValueError(f"ids must be a contiguous int32 tensor of {X.shape[0]} entries, got {ids.dtype} {tuple(ids.shape)}")
+    if scale is not None and (scale.dtype != torch.float32 or tuple(scale.shape) != (down.shape[0],)
+                              or not scale.is_contiguous()):
+        raise ValueError("scale must be a contiguous float32 tensor with one entry for each adapter")
+
+
+def _check_device(*tensors):
+    import torch
+
+    dev = tensors[0].device
+    if any(t is not None and t.device != dev for t in tensors):
+        raise ValueError("all tensors must be on one device")
+    if dev.type != "cuda":
+        raise RuntimeError("adapted projections need an MI355X (no CPU fallback)")
+    return dev, torch.cuda.current_stream(dev)
+
+
+def _on_stream(stream, cur, tensors):
+    """The stream to launch on. One other than torch's current stream waits for what is queued there (casts and pads
+    of the operands), and the temporaries made here are kept for it."""
+    import torch
+
+    if stream is None or stream == cur.cuda_stream:
+        return cur.cuda_stream
+    ext = torch.cuda.ExternalStream(stream, device=cur.device)
+    ext.wait_stream(cur)
+    for t in tensors:
+        if t is not None:
+            t.record_stream(ext)
+    return stream
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _strided(name, t, shape, dtype):
+    if t.dtype != dtype or tuple(t.shape) != shape or t.stride(-1) != 1 or any(
+            t.stride(d) < t.stride(d + 1) * t.shape[d + 1] for d in range(t.dim() - 1)):
+        raise ValueError(f"{name} must be a {dtype} tensor of shape {shape} with unit column stride and rows that do not overlap")
+    return t
+
+
+def adapted_project_device(X, C, down, up, ids, *, scale=None, out=None, compute: str = "fp32", stream=None,
+                           prepared: bool = False, return_hidden: bool = False):
+    """``X @ C.T`` plus each row's adapter for device tensors X (n x m), C (p x m), down (G x R x m), up (G x R x p) and
+    int32 ids (n); scale: float32 (G), 1 if None. Returns Y (n x p, float32), or (Y, hidden) with the n x R hidden
+    that the backward pass takes. ``prepared``: C, down and up already went through ``prepare_bank`` for this compute
+    mode. ``out``: a float32 n x p tensor with unit column stride to write to. Runs on ``stream`` (a raw handle;
+    default: torch's current stream), without synchronising; it can be captured into a graph."""
+    import torch
+
+    _check_common(X, down, up, ids, scale, compute)
+    n, m = X.shape
+    G, R = down.shape[:2]
+    if C.dim() != 2:
+        raise ValueError("C must be 2-D")
+    p = C.shape[0]
+    Cc = _operand("C", C, (p, m), compute, prepared)
+    Dc = _operand("down", down, (G, R, m), compute, prepared)
+    Uc = _operand("up", up, (G, R, p), compute, prepared)
+    if out is not None:
+        _strided("out", out, (n, p), torch.float32)
+    dev, cur = _check_device(X, C, down, up, ids, scale, out)
+    Xc = _rows(X, compute)
+    y = out if out is not None else torch.empty(n, p, dtype=torch.float32, device=dev)
+    hidden = torch.empty(n, R, dtype=torch.float32, device=dev) if return_hidden else None
+    if n:
+        lib, code = nat.load(), _CODE[compute]
+        need = lib.rp_adapt_workspace_bytes(code, n, m, p, G, R, nat.RP_ADAPT_PROJECT)
+        ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
+        st = _on_stream(stream, cur, (Xc, Cc, Dc, Uc, ids, scale, y, hidden, ws))
+        nat.check(lib.rp_adapt_project_device(
+            dev.index, Xc.data_ptr(), _ld(Xc), code, n, m, Cc.data_ptr(), p, Dc.data_ptr(), Uc.data_ptr(), G, R, _ptr(scale),
+            ids.data_ptr(), y.data_ptr(), max(y.stride(0), p), _ptr(hidden), ws.data_ptr(), need, st))
+    return (y, hidden) if return_hidden else y
+
+
+def adapted_project_backward_device(dY, X, Ct, down, up, ids, hidden, *, scale=None, out=None, compute: str = "fp32",
+                                    stream=None, prepared: bool = False):
+    """The gradients of ``adapted_project_device``: (dX, d_down, d_up) for dY (n x p), the forward pass's X, ids and
+    hidden, and Ct = C.T (m x p). dX has the compute type; with Ct None it is left out (None is returned in its place).
+    d_down (G x R x m) and d_up (G x R x p) are float32, zeros for adapters without rows; ``out``: a pair of such
+    tensors (unit column stride) to write them to. ``prepared``: Ct, down and up went through ``prepare_bank``.
+    The same call gives the same bits. Runs on ``stream`` as the forward pass does."""
+    import torch
+
+    _check_common(X, down, up, ids, scale, compute)
+    n, m = X.shape
+    G, R = down.shape[:2]
+    if dY.dim() != 2 or dY.shape[0] != n or 0 in dY.shape[1:]:
+        raise ValueError(f"dY must be 2-D with {n} rows, got {tuple(dY.shape)}")
+    p = dY.shape[1]
+    if hidden.dtype != torch.float32 or tuple(hidden.shape) != (n, R) or not hidden.is_contiguous():
+        raise ValueError(f"hidden must be the contiguous float32 ({n}, {R}) tensor of the forward pass")
+    Tc = None if Ct is None else _operand("Ct", Ct, (m, p), compute, prepared)
+    Dc = _operand("down", down, (G, R, m), compute, prepared)
+    Uc = _operand("up", up, (G, R, p), compute, prepared)
+    if out is not None:
+        d_down, d_up = _strided("out[0]", out[0], (G, R, m), torch.float32), _strided("out[1]", out[1], (G, R, p), torch.float32)
+    dev, cur = _check_device(X, dY, Ct, down, up, ids, hidden, scale, *(out or ()))
+    Xc, Yc = _rows(X, compute), _rows(dY, compute)
+    if out is None:
+        d_down = torch.empty(G, R, m, dtype=torch.float32, device=dev)
+        d_up = torch.empty(G, R, p, dtype=torch.float32, device=dev)
+    dX = None if Ct is None else torch.empty(n, m, dtype=_dtype(compute), device=dev)
+    lib, code = nat.load(), _CODE[compute]
+    what = nat.RP_ADAPT_GRADIENTS if dX is None else nat.RP_ADAPT_GRADIENTS_DX
+    need = lib.rp_adapt_workspace_bytes(code, n, m, p, G, R, what)
+    ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
+    st = _on_stream(stream, cur, (Xc, Yc, Tc, Dc, Uc, ids, hidden, scale, dX, d_down, d_up, ws))
+    row = lambda t: max(t.stride(1), t.shape[2])  # noqa: E731
+    adapter = lambda t: max(t.stride(0), row(t) * R)  # noqa: E731
+    nat.check(lib.rp_adapt_gradients_device(
+        dev.index, Yc.data_ptr(), _ld(Yc), Xc.data_ptr(), _ld(Xc), code, n, m, p, _ptr(Tc) if n else None, Dc.data_ptr(),
+        Uc.data_ptr(), G, R, _ptr(scale), ids.data_ptr(), hidden.data_ptr(), _ptr(dX) if n else None, m, d_down.data_ptr(),
+        row(d_down), adapter(d_down), d_up.data_ptr(), row(d_up), adapter(d_up), ws.data_ptr(), need, st))
+    return dX, d_down, d_up

@@ -17,10 +17,12 @@ import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
-SRC = [os.path.join(HERE, "csrc", n) for n in ("rp_spgemm.hip", "rp_libsvm.hip", "rp_dense.hip", "rp_id.hip")]
+SRC = [os.path.join(HERE, "csrc", n) for n in ("rp_spgemm.hip", "rp_libsvm.hip", "rp_dense.hip", "rp_adapt.hip",
+                                                     "rp_optim.hip", "rp_id.hip")]
 # every file the compile reads (relative to the repo root): the id covers all of them
 DEPS = ["randomprojection_amd/csrc/rp_spgemm.hip", "randomprojection_amd/csrc/rp_libsvm.hip",
-        "randomprojection_amd/csrc/rp_dense.hip", "randomprojection_amd/csrc/rp_id.hip", "randomprojection_amd/csrc/rp_common.h",
+        "randomprojection_amd/csrc/rp_dense.hip", "randomprojection_amd/csrc/rp_adapt.hip",
+        "randomprojection_amd/csrc/rp_optim.hip", "randomprojection_amd/csrc/rp_id.hip", "randomprojection_amd/csrc/rp_common.h",
         "randomprojection_amd/csrc/rp_pow5.h", "include/rp.h"]
 OUT = os.path.join(HERE, "librp.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")

@@ -37,6 +37,20 @@ inline int fail(int code, const char* fmt, ...) {
                         __FILE__, __LINE__);                                                   \
     } while (0)
 
+// The caller's current device is set back at the end of the call.
+struct DeviceGuard {
+    int before = -1;
+    int enter(int device) {
+        HIP_TRY(hipGetDevice(&before));
+        if (before != device) HIP_TRY(hipSetDevice(device));
+        else before = -1;
+        return RP_OK;
+    }
+    ~DeviceGuard() {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+};
+
 
 struct DevBuf {
     void* p = nullptr;

@@ -1,0 +1,343 @@
+// rp_optim.hip — an AdamW step over many tensors at once, its states in 32 or in 8 bits.
+//
+//   m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2            (t = steps of this tensor so far, this one included)
+//   w = w (1 - lr decay) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// in f32, every product, sum, quotient and root rounded on its own, in this order.
+//
+// States in 8 bits: blocks of 256 consecutive elements of a tensor (a tensor's last block is
+// padded with zeros) share one scale, a power of two held as its biased exponent e, so scaling is exact.
+//   m:       e4m3, |m| 2^(134 - e): e is the exponent of the block's largest |m|, which lands in [128, 256)
+//   sqrt(v): unsigned, 5 bits of exponent (bias 31) and 3 of mantissa, sqrt(v) 2^(126 - e): the largest
+//            lands in [0.5, 1). The root is held, not v: it spans half the binades (2^-33 .. 1 below the
+//            largest), and the update divides by it.
+// Rounding to a code is stochastic: the 20 mantissa bits that are dropped are first added to 16 random
+// bits (a hash of seed, step, tensor and element). With b2 = 0.999 a step changes v by 0.1 % while two
+// codes lie 6 to 12 % apart: rounding to the nearest would keep every v where its largest gradient
+// put it; rounded at random the expected value is the exact one.
+// A block that holds a NaN or an infinity gets e = 255 and stands for NaN from then on.
+#include <new>
+#include <vector>
+
+#include "rp_common.h"
+
+using namespace rpd;
+
+struct rp_adamw {
+    int device = -1;
+    int32_t tensors = 0, bits = 32, grad_type = RP_F32;
+    int64_t items = 0, blocks = 0;
+    // what the caller keeps; a block's states start at 256 elements times its number
+    void *m = nullptr, *v = nullptr;
+    uint8_t *m_scale = nullptr, *v_scale = nullptr;
+    int32_t* steps = nullptr;
+    DevBuf table, list, scalars;
+};
+
+namespace {
+
+constexpr int kBlock = 256;     // elements under one scale: 4 for each lane of a wave
+constexpr int kItemBlocks = 4;  // blocks of one tensor that one wave takes
+
+struct Tensor {
+    float* w;
+    const void* g;
+    uint16_t* copy;
+    int64_t n, first_block;
+    int32_t vec, pad;  // vec: w, g and copy are aligned for four elements at a time
+};
+struct Item {
+    uint32_t tensor, block;  // block: within its tensor
+};
+struct Scalars {
+    float by, rs;  // lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
+    uint32_t key;
+    int32_t active;
+};
+
+__host__ __device__ __forceinline__ uint32_t mix(uint32_t x) {
+    x ^= x >> 16;
+    x *= 0x9E3779B1u;
+    x ^= x >> 15;
+    x *= 0xBB67AE85u;
+    return x ^ (x >> 16);
+}
+
+// one thread a tensor: its step count goes up, and with it what the update scales by
+__global__ void adamw_begin_kernel(Scalars* __restrict__ sc, int32_t* __restrict__ steps, int32_t T, const uint8_t* __restrict__ active,
+                                   double lr, double b1, double b2, uint32_t seed_lo, uint32_t seed_hi) {
+    const int32_t t = (int32_t)(blockIdx.x * blockDim.x + threadIdx.x);
+    if (t >= T) return;
+    Scalars s{0.f, 0.f, 0u, active ? (active[t] != 0) : 1};
+    if (s.active) {
+        const int32_t k = steps[t] + 1;
+        steps[t] = k;
+        s.by = (float)(lr / (1.0 - pow(b1, (double)k)));
+        s.rs = (float)(1.0 / sqrt(1.0 - pow(b2, (double)k)));
+        s.key = mix(mix(mix(mix(seed_lo) ^ seed_hi) ^ (uint32_t)k) ^ (uint32_t)t);
+    }
+    sc[t] = s;
+}
+
+__device__ __forceinline__ float power(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+__device__ __forceinline__ int exponent_of(uint32_t bits) {  // 255: not finite
+    const int e = (int)(bits >> 23);
+    return e == 255 ? 255 : max(e, 30);
+}
+// A code c stands for the float whose top bits it is (sign apart), times a power of two: subnormal
+// codes come out right by the arithmetic of subnormal floats.
+__device__ __forceinline__ float decode_m(uint32_t c, int e) {
+    const float x = __uint_as_float((c & 127u) << 20) * 0x1p120f * power(e - 134);
+    return e == 255 ? __uint_as_float(0x7fc00000u) : (c & 128u) ? -x : x;
+}
+__device__ __forceinline__ float decode_root(uint32_t c, int e) {
+    const float x = __uint_as_float(c << 20) * 0x1p96f * power(e - 126);
+    return e == 255 ? __uint_as_float(0x7fc00000u) : x;
+}
+__device__ __forceinline__ uint32_t encode_m(float m, int e, uint32_t rnd) {
+    if (e == 255) return 0u;
+    const uint32_t t = __float_as_uint(fabsf(m) * power(134 - e) * 0x1p-120f);
+    return ((t + rnd) >> 20) | (__float_as_uint(m) >> 31 << 7);
+}
+__device__ __forceinline__ uint32_t encode_root(float r, int e, uint32_t rnd) {
+    if (e == 255) return 0u;
+    return (__float_as_uint(r * power(126 - e) * 0x1p-96f) + rnd) >> 20;
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) x = max(x, (uint32_t)__shfl_xor((int)x, o));
+    return x;
+}
+
+__device__ __forceinline__ uint16_t to_bf16(float x) {  // to nearest even; a NaN stays one
+    const uint32_t u = __float_as_uint(x);
+    if ((u & 0x7fffffffu) > 0x7f800000u) return (uint16_t)((u >> 16) | 0x40u);
+    return (uint16_t)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
+}
+
+struct StepArgs {
+    const Tensor* tensors;
+    const Item* items;
+    const Scalars* scalars;
+    int64_t n_items;
+    void *m, *v;
+    uint8_t *m_scale, *v_scale;
+    float b1, c1, b2, c2, eps, keep;  // c = 1 - b, keep = 1 - lr decay
+};
+
+// One wave an item: up to kItemBlocks blocks of one tensor, lane l holding elements 4 l .. 4 l + 3 of a block.
+template <int BITS, bool GRAD16>
+__global__ void __launch_bounds__(256) adamw_step_kernel(StepArgs a) {
+    const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (item >= a.n_items) return;
+    const int lane = threadIdx.x & 63;
+    const Item it = a.items[item];
+    const Scalars sc = a.scalars[it.tensor];
+    if (!sc.active) return;
+    const Tensor ts = a.tensors[it.tensor];
+    const int64_t nb = (ts.n + kBlock - 1) / kBlock;
+    for (int64_t b = it.block; b < min(nb, (int64_t)it.block + kItemBlocks); ++b) {
+        const int64_t at = b * kBlock + lane * 4, state = (ts.first_block + b) * kBlock + lane * 4;
+        const int64_t left = ts.n - at;
+        float w[4] = {0.f, 0.f, 0.f, 0.f}, g[4] = {0.f, 0.f, 0.f, 0.f}, m[4], v[4], root[4];
+        if (ts.vec && left >= 4) {
+            const float4 x = *reinterpret_cast<const float4*>(ts.w + at);
+            w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+            if constexpr (GRAD16) {
+                const uint2 y = *reinterpret_cast<const uint2*>((const uint16_t*)ts.g + at);
+                g[0] = __uint_as_float(y.x << 16), g[1] = __uint_as_float(y.x & 0xffff0000u);
+                g[2] = __uint_as_float(y.y << 16), g[3] = __uint_as_float(y.y & 0xffff0000u);
+            } else {
+                const float4 y = *reinterpret_cast<const float4*>((const float*)ts.g + at);
+                g[0] = y.x, g[1] = y.y, g[2] = y.z, g[3] = y.w;
+            }
+        } else {
+            for (int k = 0; k < 4; ++k)
+                if (k < left) {
+                    w[k] = ts.w[at + k];
+                    g[k] = GRAD16 ? __uint_as_float((uint32_t)((const uint16_t*)ts.g)[at + k] << 16) : ((const float*)ts.g)[at + k];
+                }
+        }
+        if constexpr (BITS == 32) {
+            const float4 x = *reinterpret_cast<const float4*>((const float*)a.m + state);
+            const float4 y = *reinterpret_cast<const float4*>((const float*)a.v + state);
+            m[0] = x.x, m[1] = x.y, m[2] = x.z, m[3] = x.w;
+            v[0] = y.x, v[1] = y.y, v[2] = y.z, v[3] = y.w;
+        } else {
+            const uint32_t cm = *reinterpret_cast<const uint32_t*>((const uint8_t*)a.m + state);
+            const uint32_t cv = *reinterpret_cast<const uint32_t*>((const uint8_t*)a.v + state);
+            const int em = a.m_scale[ts.first_block + b], ev = a.v_scale[ts.first_block + b];
+            for (int k = 0; k < 4; ++k) {
+                m[k] = decode_m(cm >> (8 * k) & 255u, em);
+                const float r = decode_root(cv >> (8 * k) & 255u, ev);
+                v[k] = r * r;
+            }
+        }
+        for (int k = 0; k < 4; ++k) {
+            m[k] = m[k] * a.b1 + g[k] * a.c1;
+            v[k] = v[k] * a.b2 + g[k] * g[k] * a.c2;
+            root[k] = sqrtf(v[k]);
+            w[k] = w[k] * a.keep - m[k] / (root[k] * sc.rs + a.eps) * sc.by;
+        }
+        if (ts.vec && left >= 4) {
+            *reinterpret_cast<float4*>(ts.w + at) = make_float4(w[0], w[1], w[2], w[3]);
+            if (ts.copy)
+                *reinterpret_cast<uint2*>(ts.copy + at) = make_uint2(to_bf16(w[0]) | (uint32_t)to_bf16(w[1]) << 16,
+                                                                     to_bf16(w[2]) | (uint32_t)to_bf16(w[3]) << 16);
+        } else {
+            for (int k = 0; k < 4; ++k)
+                if (k < left) {
+                    ts.w[at + k] = w[k];
+                    if (ts.copy) ts.copy[at + k] = to_bf16(w[k]);
+                }
+        }
+        if constexpr (BITS == 32) {
+            *reinterpret_cast<float4*>((float*)a.m + state) = make_float4(m[0], m[1], m[2], m[3]);
+            *reinterpret_cast<float4*>((float*)a.v + state) = make_float4(v[0], v[1], v[2], v[3]);
+        } else {
+            uint32_t mm = 0u, rr = 0u;
+            for (int k = 0; k < 4; ++k) {
+                if (k >= left) m[k] = root[k] = 0.f;
+                mm = max(mm, __float_as_uint(m[k]) & 0x7fffffffu);
+                rr = max(rr, __float_as_uint(root[k]) & 0x7fffffffu);
+            }
+            const int em = exponent_of(wave_max(mm)), ev = exponent_of(wave_max(rr));
+            const uint32_t high = (uint32_t)(at >> 32), key = high ? mix(sc.key + high) : sc.key;
+            uint32_t cm = 0u, cv = 0u;
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t rnd = mix((uint32_t)(at + k) ^ key);
+                cm |= encode_m(m[k], em, (rnd >> 16 << 4) + 8u) << (8 * k);
+                cv |= encode_root(root[k], ev, ((rnd & 0xffffu) << 4) + 8u) << (8 * k);
+            }
+            *reinterpret_cast<uint32_t*>((uint8_t*)a.m + state) = cm;
+            *reinterpret_cast<uint32_t*>((uint8_t*)a.v + state) = cv;
+            if (lane == 0) {
+                a.m_scale[ts.first_block + b] = (uint8_t)em;
+                a.v_scale[ts.first_block + b] = (uint8_t)ev;
+            }
+        }
+    }
+}
+
+// the states in 8 bits as the values they stand for: one wave a block
+__global__ void __launch_bounds__(256)
+adamw_values_kernel(const uint32_t* __restrict__ m, const uint32_t* __restrict__ v, const uint8_t* __restrict__ m_scale,
+                    const uint8_t* __restrict__ v_scale, int64_t blocks, float4* __restrict__ out_m, float4* __restrict__ out_root) {
+    const int64_t b = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (b >= blocks) return;
+    const int64_t i = b * 64 + (threadIdx.x & 63);
+    const uint32_t cm = m[i], cv = v[i];
+    const int em = m_scale[b], ev = v_scale[b];
+    out_m[i] = make_float4(decode_m(cm & 255u, em), decode_m(cm >> 8 & 255u, em), decode_m(cm >> 16 & 255u, em), decode_m(cm >> 24, em));
+    out_root[i] = make_float4(decode_root(cv & 255u, ev), decode_root(cv >> 8 & 255u, ev), decode_root(cv >> 16 & 255u, ev),
+                              decode_root(cv >> 24, ev));
+}
+
+}  // namespace
+
+extern "C" {
+
+int rp_adamw_create(int device, int32_t n_tensors, const int64_t* numels, float* const* params, const void* const* grads,
+                    int32_t grad_type, uint16_t* const* copies, int32_t state_bits, void* exp_avg, void* exp_avg_sq,
+                    uint8_t* exp_avg_scale, uint8_t* root_scale, int32_t* steps, rp_adamw** out) {
+    if (!out) return fail(RP_ERR_INVALID, "NULL out");
+    *out = nullptr;
+    if (n_tensors <= 0 || !numels || !params || !grads) return fail(RP_ERR_INVALID, "no tensors");
+    if (grad_type != RP_F32 && grad_type != RP_BF16) return fail(RP_ERR_INVALID, "grad_type must be RP_F32 or RP_BF16");
+    if (state_bits != 32 && state_bits != 8) return fail(RP_ERR_INVALID, "state_bits must be 32 or 8");
+    if (!exp_avg || !exp_avg_sq || !steps || (state_bits == 8 && (!exp_avg_scale || !root_scale)))
+        return fail(RP_ERR_INVALID, "NULL state");
+    if (((uintptr_t)exp_avg | (uintptr_t)exp_avg_sq) & 15) return fail(RP_ERR_INVALID, "states must be 16-byte aligned");
+    rp_adamw* h = nullptr;
+    try {
+        std::vector<Tensor> ts((size_t)n_tensors);
+        std::vector<Item> items;
+        int64_t first = 0;
+        for (int32_t t = 0; t < n_tensors; ++t) {
+            const int64_t n = numels[t];
+            if (n < 0 || n > ((int64_t)1 << 38)) return fail(RP_ERR_INVALID, "tensor %d: bad size", (int)t);
+            if (n && (!params[t] || !grads[t] || (copies && !copies[t]))) return fail(RP_ERR_INVALID, "tensor %d: NULL", (int)t);
+            const size_t gs = grad_type == RP_BF16 ? 2 : 4;
+            if (((uintptr_t)params[t] & 3) || ((uintptr_t)grads[t] & (gs - 1)) || (copies && ((uintptr_t)copies[t] & 1)))
+                return fail(RP_ERR_INVALID, "tensor %d: not aligned to its elements", (int)t);
+            Tensor& x = ts[(size_t)t];
+            x.w = params[t], x.g = grads[t], x.copy = copies ? copies[t] : nullptr, x.n = n, x.first_block = first, x.pad = 0;
+            x.vec = !((uintptr_t)x.w & 15) && !((uintptr_t)x.g & (4 * gs - 1)) && !((uintptr_t)x.copy & 7);
+            const int64_t nb = (n + kBlock - 1) / kBlock;
+            for (int64_t b = 0; b < nb; b += kItemBlocks) items.push_back({(uint32_t)t, (uint32_t)b});
+            first += nb;
+        }
+        if ((int64_t)items.size() >= ((int64_t)1 << 33)) return fail(RP_ERR_UNSUPPORTED, "too many elements");
+        h = new rp_adamw;
+        h->device = device, h->tensors = n_tensors, h->bits = state_bits, h->grad_type = grad_type;
+        h->items = (int64_t)items.size(), h->blocks = first;
+        h->m = exp_avg, h->v = exp_avg_sq, h->m_scale = exp_avg_scale, h->v_scale = root_scale, h->steps = steps;
+        DeviceGuard guard;
+        int rc = guard.enter(device);
+        if (!rc) rc = h->table.ensure(sizeof(Tensor) * ts.size(), device);
+        if (!rc) rc = h->list.ensure(sizeof(Item) * std::max<size_t>(items.size(), 1), device);
+        if (!rc) rc = h->scalars.ensure(sizeof(Scalars) * ts.size(), device);
+        if (!rc) {
+            hipError_t e = hipMemcpy(h->table.p, ts.data(), sizeof(Tensor) * ts.size(), hipMemcpyHostToDevice);
+            if (e == hipSuccess && !items.empty())
+                e = hipMemcpy(h->list.p, items.data(), sizeof(Item) * items.size(), hipMemcpyHostToDevice);
+            if (e != hipSuccess) rc = fail(RP_ERR_HIP, "hipMemcpy: %s", hipGetErrorString(e));
+        }
+        if (rc) {
+            delete h;
+            return rc;
+        }
+    } catch (const std::bad_alloc&) {
+        delete h;
+        return fail(RP_ERR_NOMEM, "out of host memory");
+    }
+    *out = h;
+    return RP_OK;
+}
+
+int rp_adamw_step(rp_adamw* h, double lr, double beta1, double beta2, double eps, double weight_decay, uint64_t seed,
+                  const uint8_t* active, void* stream) {
+    if (!h) return fail(RP_ERR_INVALID, "NULL handle");
+    if (!(lr >= 0) || !(beta1 >= 0 && beta1 < 1) || !(beta2 >= 0 && beta2 < 1) || !(eps >= 0) || !(weight_decay >= 0))
+        return fail(RP_ERR_INVALID, "lr, eps and weight_decay must not be negative, the betas lie in [0, 1)");
+    DeviceGuard guard;
+    int rc = guard.enter(h->device);
+    if (rc) return rc;
+    hipStream_t st = (hipStream_t)stream;
+    hipLaunchKernelGGL(adamw_begin_kernel, dim3((unsigned)((h->tensors + 63) / 64)), dim3(64), 0, st, (Scalars*)h->scalars.p,
+                       h->steps, h->tensors, active, lr, beta1, beta2, (uint32_t)seed, (uint32_t)(seed >> 32));
+    HIP_TRY(hipGetLastError());
+    if (!h->items) return RP_OK;
+    StepArgs a{(const Tensor*)h->table.p, (const Item*)h->list.p, (const Scalars*)h->scalars.p, h->items, h->m, h->v, h->m_scale,
+               h->v_scale, (float)beta1, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps,
+               (float)(1.0 - lr * weight_decay)};
+    const dim3 grid((unsigned)((h->items + 3) / 4)), block(256);
+    const bool g16 = h->grad_type == RP_BF16;
+    if (h->bits == 32 && g16) hipLaunchKernelGGL((adamw_step_kernel<32, true>), grid, block, 0, st, a);
+    else if (h->bits == 32) hipLaunchKernelGGL((adamw_step_kernel<32, false>), grid, block, 0, st, a);
+    else if (g16) hipLaunchKernelGGL((adamw_step_kernel<8, true>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((adamw_step_kernel<8, false>), grid, block, 0, st, a);
+    HIP_TRY(hipGetLastError());
+    return RP_OK;
+}
+
+int rp_adamw_values(rp_adamw* h, float* exp_avg, float* root, void* stream) {
+    if (!h || !exp_avg || !root) return fail(RP_ERR_INVALID, "NULL handle or output");
+    if (h->bits != 8) return fail(RP_ERR_INVALID, "the states are held in 32 bits");
+    if (((uintptr_t)exp_avg | (uintptr_t)root) & 15) return fail(RP_ERR_INVALID, "outputs must be 16-byte aligned");
+    if (!h->blocks) return RP_OK;
+    DeviceGuard guard;
+    int rc = guard.enter(h->device);
+    if (rc) return rc;
+    hipLaunchKernelGGL(adamw_values_kernel, dim3((unsigned)((h->blocks + 3) / 4)), dim3(256), 0, (hipStream_t)stream,
+                       (const uint32_t*)h->m, (const uint32_t*)h->v, h->m_scale, h->v_scale, h->blocks, (float4*)exp_avg, (float4*)root);
+    HIP_TRY(hipGetLastError());
+    return RP_OK;
+}
+
+int rp_adamw_destroy(rp_adamw* h) {
+    delete h;
+    return RP_OK;
+}
+
+}  // extern "C"

@@ -20,9 +20,9 @@ import ctypes
 from . import _native as nat
 from .gaussian import _STEP
 
-__all__ = ["adapted_project_device", "adapted_project_backward_device", "prepare_bank", "MAX_RANK"]
+__all__ = ["adapted_project_device", "adapted_project_backward_device", "prepare_bank", "MAX_RANK", "MAX_ADAPTERS"]
 
-MAX_RANK = 128
+MAX_RANK, MAX_ADAPTERS = 128, 16383
 _CODE = {"bf16": nat.RP_BF16, "fp32": nat.RP_F32}
 
 
@@ -48,7 +48,10 @@ def prepare_bank(W, compute: str):
 
 
 def _rows(X, compute):
-    """X as the kernels read it: itself where rows follow each other, aligned and without need of padding, else a copy."""
+    """X as the kernels read it: a row stride of its own where rows are aligned and need no padding, else a copy."""
+    if (X.dtype == _dtype(compute) and X.shape[1] % _STEP[compute] == 0 and X.stride(1) == 1 and X.data_ptr() % 16 == 0
+            and X.stride(0) * X.element_size() % 16 == 0 and (X.stride(0) >= X.shape[1] or X.shape[0] <= 1)):
+        return X
     return prepare_bank(X, compute)
 
 
@@ -78,8 +81,8 @@ def _check_common(X, down, up, ids, scale, compute):
     if down.shape[:2] != up.shape[:2] or 0 in down.shape:
         raise ValueError(f"down {tuple(down.shape)} and up {tuple(up.shape)} must have the same, positive, number of "
                          "adapters and rank")
-    if down.shape[1] > MAX_RANK or down.shape[0] > 65535:
-        raise ValueError(f"at most 65535 adapters of rank {MAX_RANK}, got {down.shape[0]} of rank {down.shape[1]}")
+    if down.shape[1] > MAX_RANK or down.shape[0] > MAX_ADAPTERS:
+        raise ValueError(f"at most {MAX_ADAPTERS} adapters of rank {MAX_RANK}, got {down.shape[0]} of rank {down.shape[1]}")
     if ids.dtype != torch.int32 or tuple(ids.shape) != (X.shape[0],) or not ids.is_contiguous():
         raise ValueError(f"ids must be a contiguous int32 tensor of {X.shape[0]} entries, got {ids.dtype} {tuple(ids.shape)}")
     if scale is not None and (scale.dtype != torch.float32 or tuple(scale.shape) != (down.shape[0],)

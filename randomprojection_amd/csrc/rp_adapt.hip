@@ -18,10 +18,8 @@ using namespace rpd;
 
 namespace {
 
-constexpr int kMaxRank = 128;
+constexpr int kMaxRank = 128, kMaxAdapters = 16383;  // a wave's counts of all groups fit 64 KB of LDS
 
-__device__ __forceinline__ float to_f32(float x) { return x; }
-__device__ __forceinline__ float to_f32(uint16_t x) { return __uint_as_float((uint32_t)x << 16); }
 // round to nearest even; a NaN stays one
 __device__ __forceinline__ uint16_t to_bf16(float x) {
     const uint32_t u = __float_as_uint(x);
@@ -31,70 +29,679 @@ __device__ __forceinline__ uint16_t to_bf16(float x) {
 __device__ __forceinline__ void store_as(float* p, float x) { *p = x; }
 __device__ __forceinline__ void store_as(uint16_t* p, float x) { *p = to_bf16(x); }
 
-// H[i][r] = (mul ? mul[a] : 1) sum_q Z[i][q] W[a][r][q]; zeros where row i has no adapter. One wave a row.
-template <typename T>
-__global__ void __launch_bounds__(256)
-shrink_kernel(const T* __restrict__ Z, int64_t ldz, int64_t n, int64_t q, const T* __restrict__ W, int64_t ldw, int64_t G,
-              int R, const float* __restrict__ mul, const int32_t* __restrict__ ids, float* __restrict__ H) {
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+// ------------------------------------------------------------------------------------------
+// Rows grouped by adapter: a stable counting sort of the ids (rows without an adapter come last, as
+// group G), one wave a chunk of rows. Lanes that hold the same id find each other by a ballot for each
+// bit of the id, so a lane's rank is a population count and the order never depends on timing.
+struct Groups {
+    int32_t* perm;    // sorted position -> row
+    int32_t* sid;     // sorted position -> group (0 .. G)
+    int32_t* start;   // group -> first sorted position; G + 2 entries
+    int4* tiles;      // {group, first sorted position, rows, 0}: at most tile_rows rows of one group (G included)
+    int4* chunks;     // {group, first sorted position, rows, its partial sums' number or -1}: at most chunk_rows rows, group < G
+    int32_t* tile0;   // group -> its first tile; G + 1 entries
+    int32_t* chunk0;  // group -> its first chunk; G + 1 entries
+    int32_t* multi0;  // group -> the first of its partial sums, where it has more than one chunk; G + 1 entries
+    int32_t* number;  // {tiles, chunks}
+    int32_t* hist;    // (G + 1) x n_chunks counts, then first positions
+};
+
+__device__ __forceinline__ int group_of(int32_t id, int G) { return id >= 0 && id < G ? id : G; }
+
+// the lanes (of `live` ones) that hold the same g
+__device__ __forceinline__ uint64_t same_lanes(int g, bool live, int bits) {
+    uint64_t m = __ballot(live);
+    for (int b = 0; b < bits; ++b) {
+        const bool on = (g >> b) & 1;
+        const uint64_t v = __ballot(on);
+        m &= on ? v : ~v;
+    }
+    return m;
+}
+
+// LDS that the lanes of one wave share: what was written before is read after
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// counts the ids of rows [r0, r1) by group into cnt (this wave's alone, zero before)
+__device__ __forceinline__ void count_rows(const int32_t* __restrict__ ids, int64_t r0, int64_t r1, int G, int bits, int32_t* cnt) {
     const int lane = threadIdx.x & 63;
-    if (row >= n) return;
-    const int64_t a = ids[row];
-    const bool has = a >= 0 && a < G;
-    for (int r = 0; r < R; ++r) {
-        float s = 0.f;
-        if (has)
-            for (int64_t c = lane; c < q; c += 64) s = fmaf(to_f32(Z[row * ldz + c]), to_f32(W[(a * R + r) * ldw + c]), s);
-        for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
-        if (lane == 0) H[row * R + r] = has ? (mul ? s * mul[a] : s) : 0.f;
+    for (int64_t r = r0; r < r1; r += 64) {
+        const bool live = r + lane < r1;
+        const int g = live ? group_of(ids[r + lane], G) : 0;
+        const uint64_t m = same_lanes(g, live, bits);
+        if (live && __ffsll((unsigned long long)m) - 1 == lane) cnt[g] += __popcll(m);
+        wave_sync();
     }
 }
 
-// O[i][c] = P[i][c] + (mul ? mul[a] : 1) sum_r H[i][r] W[a][r][c]
-template <typename T, typename O>
+// gives every row of [r0, r1) its position, next[g] being the first free one of this wave's rows of group g
+__device__ __forceinline__ void place_rows(const int32_t* __restrict__ ids, int64_t r0, int64_t r1, int G, int bits, int32_t* next,
+                                           const Groups& o) {
+    const int lane = threadIdx.x & 63;
+    for (int64_t r = r0; r < r1; r += 64) {
+        const bool live = r + lane < r1;
+        const int g = live ? group_of(ids[r + lane], G) : 0;
+        const uint64_t m = same_lanes(g, live, bits);
+        if (live) {
+            const int at = next[g] + __popcll(m & ((1ull << lane) - 1));
+            o.perm[at] = (int32_t)(r + lane);
+            o.sid[at] = g;
+        }
+        wave_sync();  // every lane has read next before its leader moves it
+        if (live && __ffsll((unsigned long long)m) - 1 == lane) next[g] += __popcll(m);
+        wave_sync();
+    }
+}
+
+// exclusive prefix sum over the block's threads; total: of all of them
+__device__ __forceinline__ int block_scan(int x, int* sums, int& total) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, nw = blockDim.x >> 6;
+    int s = x;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_up(s, o);
+        if (lane >= o) s += y;
+    }
+    __syncthreads();
+    if (lane == 63) sums[w] = s;
+    __syncthreads();
+    int before = 0;
+    total = 0;
+    for (int k = 0; k < nw; ++k) {
+        if (k < w) before += sums[k];
+        total += sums[k];
+    }
+    return before + s - x;
+}
+
+// one block: from each group's first position (first(g), g <= G + 1) its tiles and chunks
+template <typename F>
+__device__ __forceinline__ void list_groups(const F& first, int G, int tile_rows, int chunk_rows, int* sums, const Groups& o) {
+    int t0 = 0, c0 = 0, p0 = 0;
+    for (int base = 0; base <= G; base += blockDim.x) {
+        const int g = base + threadIdx.x;
+        const int s = g <= G ? first(g) : 0, rows = g <= G ? first(g + 1) - s : 0;
+        const int nt = (rows + tile_rows - 1) / tile_rows, nc = g < G ? (rows + chunk_rows - 1) / chunk_rows : 0;
+        int tt, tc, tp;
+        const int t = t0 + block_scan(nt, sums, tt), c = c0 + block_scan(nc, sums, tc);
+        const int p = p0 + block_scan(nc > 1 ? nc : 0, sums, tp);
+        if (g <= G) {
+            o.start[g] = s;
+            o.tile0[g] = t;
+            o.chunk0[g] = c;
+            o.multi0[g] = p;
+            if (g == G) o.start[G + 1] = s + rows;
+        }
+        t0 += tt, c0 += tc, p0 += tp;
+    }
+    if (threadIdx.x == 0) o.number[0] = t0, o.number[1] = c0;
+    __syncthreads();
+    for (int g = threadIdx.x >> 6; g <= G; g += blockDim.x >> 6) {  // a wave a group
+        const int s = o.start[g], rows = o.start[g + 1] - s, nc = g < G ? (rows + chunk_rows - 1) / chunk_rows : 0;
+        for (int k = threadIdx.x & 63; k * tile_rows < rows; k += 64)
+            o.tiles[o.tile0[g] + k] = make_int4(g, s + k * tile_rows, min(tile_rows, rows - k * tile_rows), 0);
+        for (int k = threadIdx.x & 63; k < nc; k += 64)
+            o.chunks[o.chunk0[g] + k] = make_int4(g, s + k * chunk_rows, min(chunk_rows, rows - k * chunk_rows),
+                                                nc > 1 ? o.multi0[g] + k : -1);
+    }
+}
+
+// few rows: one block does it all, its waves' counts in LDS as cnt[wave][group]
+__global__ void __launch_bounds__(1024)
+group_small_kernel(const int32_t* __restrict__ ids, int n, int G, int bits, int tile_rows, int chunk_rows, Groups o) {
+    extern __shared__ int32_t lds_groups[];
+    __shared__ int sums[16];
+    int32_t* cnt = lds_groups;           // 16 x (G + 1)
+    int32_t* first = cnt + 16 * (G + 1);  // G + 2
+    const int tid = threadIdx.x, w = tid >> 6;
+    for (int i = tid; i < 16 * (G + 1); i += 1024) cnt[i] = 0;
+    __syncthreads();
+    const int each = (n + 1023) / 1024 * 64, r0 = min(n, w * each), r1 = min(n, r0 + each);
+    count_rows(ids, r0, r1, G, bits, cnt + w * (G + 1));
+    __syncthreads();
+    int at = 0;
+    for (int base = 0; base <= G; base += 1024) {
+        const int g = base + tid;
+        int rows = 0, total;
+        if (g <= G)
+            for (int k = 0; k < 16; ++k) rows += cnt[k * (G + 1) + g];
+        int s = at + block_scan(rows, sums, total);
+        if (g <= G) {
+            first[g] = s;
+            if (g == G) first[G + 1] = s + rows;
+            for (int k = 0; k < 16; ++k) {
+                const int c = cnt[k * (G + 1) + g];
+                cnt[k * (G + 1) + g] = s;
+                s += c;
+            }
+        }
+        at += total;
+    }
+    __syncthreads();
+    place_rows(ids, r0, r1, G, bits, cnt + w * (G + 1), o);
+    list_groups([&](int g) { return first[g]; }, G, tile_rows, chunk_rows, sums, o);
+}
+
+// many rows: counts of each wave's rows (4 waves a block) to hist[group][chunk]
 __global__ void __launch_bounds__(256)
-expand_kernel(const float* P, int64_t ldp, O* out, int64_t ldo, int64_t n, int64_t q, const T* __restrict__ W, int64_t ldw,
-              int64_t G, int R, const float* __restrict__ mul, const int32_t* __restrict__ ids, const float* __restrict__ H) {
-    const int64_t row = blockIdx.x;
-    const int64_t a = ids[row];
-    const bool has = a >= 0 && a < G;
-    for (int64_t c = threadIdx.x; c < q; c += 256) {
-        float s = 0.f;
-        if (has)
-            for (int r = 0; r < R; ++r) s = fmaf(H[row * R + r], to_f32(W[(a * R + r) * ldw + c]), s);
-        store_as(out + row * ldo + c, P[row * ldp + c] + (has ? (mul ? s * mul[a] : s) : 0.f));
-    }
+group_count_kernel(const int32_t* __restrict__ ids, int64_t n, int G, int bits, int64_t each, int n_chunks, Groups o) {
+    extern __shared__ int32_t lds_groups[];
+    int32_t* cnt = lds_groups + (threadIdx.x >> 6) * (G + 1);
+    const int lane = threadIdx.x & 63, chunk = blockIdx.x * (blockDim.x >> 6) + (threadIdx.x >> 6);
+    for (int g = lane; g <= G; g += 64) cnt[g] = 0;
+    wave_sync();
+    const int64_t r0 = min(n, chunk * each);
+    count_rows(ids, r0, min(n, r0 + each), G, bits, cnt);
+    if (chunk < n_chunks)
+        for (int g = lane; g <= G; g += 64) o.hist[(int64_t)g * n_chunks + chunk] = cnt[g];
 }
 
-// D[g][r][c] = (mul ? mul[g] : 1) sum over rows of adapter g of H[i][r] Z[i][c]
+// one block: exclusive prefix sums of hist in its order, a run of entries a thread, and the lists
+__global__ void __launch_bounds__(1024) group_scan_kernel(int64_t n, int G, int n_chunks, int tile_rows, int chunk_rows, Groups o) {
+    __shared__ int sums[16];
+    const int64_t all = (int64_t)(G + 1) * n_chunks, each = (all + 1023) / 1024;
+    const int64_t i0 = min(all, threadIdx.x * each), i1 = min(all, i0 + each);
+    int s = 0, total;
+    for (int64_t i = i0; i < i1; ++i) s += o.hist[i];
+    s = block_scan(s, sums, total);
+    for (int64_t i = i0; i < i1; ++i) {
+        const int c = o.hist[i];
+        o.hist[i] = s;
+        s += c;
+    }
+    __syncthreads();
+    list_groups([&](int g) { return g <= G ? o.hist[(int64_t)g * n_chunks] : (int)n; }, G, tile_rows, chunk_rows, sums, o);
+}
+
+__global__ void __launch_bounds__(256)
+group_place_kernel(const int32_t* __restrict__ ids, int64_t n, int G, int bits, int64_t each, int n_chunks, Groups o) {
+    extern __shared__ int32_t lds_groups[];
+    int32_t* next = lds_groups + (threadIdx.x >> 6) * (G + 1);
+    const int lane = threadIdx.x & 63, chunk = blockIdx.x * (blockDim.x >> 6) + (threadIdx.x >> 6);
+    if (chunk >= n_chunks) return;
+    for (int g = lane; g <= G; g += 64) next[g] = o.hist[(int64_t)g * n_chunks + chunk];
+    wave_sync();
+    const int64_t r0 = min(n, chunk * each);
+    place_rows(ids, r0, min(n, r0 + each), G, bits, next, o);
+}
+
+// ------------------------------------------------------------------------------------------
+// Matrix instructions. 16 x 16 tiles; a lane's operand is 16 bytes of a row of each side (row = lane &
+// 15, 16-byte chunk = lane >> 4), so 64 bytes of a row are one step of the contraction: 32 bf16 in one
+// instruction, 16 f32 in four (element e of every lane's chunk in instruction e: a permutation of the
+// step, the same on both sides). D[i][j], i a row of `a`, j a row of `b`: lane l holds j = l & 15, i = 4 (l >> 4) + e.
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+
+// four neighbouring values, of which the first `left` are inside
+__device__ __forceinline__ void put4(float* p, f32x4 x, int vec, int left) {
+    if (vec && left >= 4) *reinterpret_cast<f32x4*>(p) = x;
+    else
+        for (int e = 0; e < 4; ++e)
+            if (e < left) p[e] = x[e];
+}
+__device__ __forceinline__ void put4(uint16_t* p, f32x4 x, int vec, int left) {
+    if (vec && left >= 4)
+        *reinterpret_cast<uint2*>(p) = make_uint2(to_bf16(x[0]) | (uint32_t)to_bf16(x[1]) << 16, to_bf16(x[2]) | (uint32_t)to_bf16(x[3]) << 16);
+    else
+        for (int e = 0; e < 4; ++e)
+            if (e < left) p[e] = to_bf16(x[e]);
+}
+
 template <typename T>
-__global__ void __launch_bounds__(256)
-outer_kernel(const T* __restrict__ Z, int64_t ldz, int64_t n, int64_t q, int64_t G, int R, const float* __restrict__ mul,
-             const int32_t* __restrict__ ids, const float* __restrict__ H, float* __restrict__ D, int64_t ldd, int64_t sdd) {
-    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (c >= q) return;
-    for (int64_t k = blockIdx.y; k < G * R; k += gridDim.y) {
-        const int64_t g = k / R, r = k % R;
-        float s = 0.f;
-        for (int64_t i = 0; i < n; ++i)
-            if (ids[i] == g) s = fmaf(H[i * R + r], to_f32(Z[i * ldz + c]), s);
-        D[g * sdd + r * ldd + c] = mul ? s * mul[g] : s;
+__device__ __forceinline__ f32x4 mma(uint4 a, uint4 b, f32x4 c) {
+    if constexpr (sizeof(T) == 2) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(s16x8, a), __builtin_bit_cast(s16x8, b), c, 0, 0, 0);
+    } else {
+        c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.x), __uint_as_float(b.x), c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.y), __uint_as_float(b.y), c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.z), __uint_as_float(b.z), c, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.w), __uint_as_float(b.w), c, 0, 0, 0);
     }
 }
 
+// x = hi + mid + low exactly, each a bf16 (8 bits of the 24 at a time, cut off): an f32 factor against
+// bf16 ones in three matrix instructions without a rounding. An infinity is hi alone.
+__device__ __forceinline__ void split3(float x, uint32_t& hi, uint32_t& mid, uint32_t& low) {
+    hi = __float_as_uint(x) & 0xffff0000u;
+    const float h = __uint_as_float(hi), y = h == x ? 0.f : x - h;
+    mid = __float_as_uint(y) & 0xffff0000u;
+    low = __float_as_uint(y - __uint_as_float(mid)) & 0xffff0000u;
+}
+// the upper halves of a (low half of the result) and b
+__device__ __forceinline__ uint32_t pack_high(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
+__device__ __forceinline__ uint32_t pack_low(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
+
+// H[i][r] = (mul ? mul[a] : 1) sum_q Z[i][q] W[a][r][q]; zeros for rows without an adapter. A block takes a tile
+// of 16 RT rows of one group; its NW waves split the contraction and add up in LDS in their order. Bound by
+// reading Z once: the wave holds 16 RT x 16 KT of H, so W (from L2) is read once for 16 RT rows, and there is
+// nothing between the loads and the matrix instructions.
+template <typename T, int RT, int KT, int NW>
+__global__ void __launch_bounds__(64 * NW)
+shrink_kernel(const T* __restrict__ Z, int64_t ldz, int64_t kp, const T* __restrict__ W, int G, int R, const float* __restrict__ mul,
+              Groups o, float* __restrict__ H) {
+    __shared__ f32x4 red[NW][RT * KT][64];
+    if ((int)blockIdx.x >= o.number[0]) return;
+    const int4 tile = o.tiles[blockIdx.x];
+    const int g = tile.x, pos = tile.y, rows = tile.z;
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, c = lane & 15, q = lane >> 4;
+    if (g == G) {
+        for (int i = tid; i < rows * R; i += 64 * NW) H[(int64_t)o.perm[pos + i / R] * R + i % R] = 0.f;
+        return;
+    }
+    const char* z[RT];
+    const char* b[KT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+        z[t] = reinterpret_cast<const char*>(Z + o.perm[pos + min(t * 16 + c, rows - 1)] * ldz) + q * 16;
+#pragma unroll
+    for (int j = 0; j < KT; ++j)
+        b[j] = reinterpret_cast<const char*>(W + ((int64_t)g * R + min(j * 16 + c, R - 1)) * kp) + q * 16;
+    f32x4 acc[RT][KT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int j = 0; j < KT; ++j) acc[t][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int64_t lines = kp * (int64_t)sizeof(T) / 128, each = (lines + NW - 1) / NW;  // 128 bytes of a row: two steps
+    const int64_t l1 = min(lines, (w + 1) * each);
+    for (int64_t l = w * each; l < l1; ++l) {
+        uint4 zf[2][RT], bf[2][KT];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int t = 0; t < RT; ++t) zf[h][t] = *reinterpret_cast<const uint4*>(z[t] + l * 128 + h * 64);
+#pragma unroll
+            for (int j = 0; j < KT; ++j) bf[h][j] = *reinterpret_cast<const uint4*>(b[j] + l * 128 + h * 64);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int t = 0; t < RT; ++t)
+#pragma unroll
+                for (int j = 0; j < KT; ++j) acc[t][j] = mma<T>(bf[h][j], zf[h][t], acc[t][j]);
+    }
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int j = 0; j < KT; ++j) red[w][t * KT + j][lane] = acc[t][j];
+    __syncthreads();
+    const float s = mul ? mul[g] : 1.f;
+    for (int i = tid; i < RT * KT * 64; i += 64 * NW) {
+        const f32x4* p = &red[0][0][0] + i;
+        f32x4 x = p[0];
+#pragma unroll
+        for (int k = 1; k < NW; ++k) x += p[k * RT * KT * 64];
+        const int l = i & 63, row = i / (64 * KT) * 16 + (l & 15), r = (i >> 6) % KT * 16 + 4 * (l >> 4);
+        if (row >= rows) continue;
+        float* h = H + (int64_t)o.perm[pos + row] * R + r;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (r + e < R) h[e] = x[e] * s;
+    }
+}
+
+// D[g][r][c] (+ partial sums) = (mul ? mul[g] : 1) sum over rows i of adapter g of H[i][r] Z[i][c]. A wave takes 16 KT
+// ranks by 128 (bf16) or 64 (f32) columns over a chunk of one group's rows, its lanes reading 16 bytes of
+// neighbouring columns of each row: no LDS for Z, which is read once (per 16 KT ranks) and bounds the kernel.
+//   bf16: 32 rows a step, lane (c, q) rows 8 q .. 8 q + 7, columns 8 c .. 8 c + 7: 8 x 8 values turned round in
+//         registers (a byte permutation for two values), so column j of every lane is one matrix operand. H is split exactly
+//         into three bf16.
+//   f32:  4 rows a matrix instruction, lane (c, q) row q, columns 4 c .. 4 c + 3.
+struct OuterArgs {
+    const void* Z;
+    int64_t ldz, qp, q;  // qp: readable columns
+    int R;
+    const float *mul, *H;
+    float* D;
+    int64_t ldd, sdd;
+    float* part;
+    int vec;  // rows of D and of the partial sums are 16-byte aligned
+};
+
+constexpr int kMaxChunk = 2048;
+
+template <typename T, int KT>
+__global__ void __launch_bounds__(256) outer_kernel(OuterArgs a, Groups o) {
+    constexpr int NC = sizeof(T) == 2 ? 8 : 4;  // columns of a lane
+    __shared__ int32_t list[kMaxChunk];
+    if ((int)blockIdx.x >= o.number[1]) return;
+    const int4 chunk = o.chunks[blockIdx.x];
+    const int g = chunk.x, rows = chunk.z;
+    for (int i = threadIdx.x; i < rows; i += 256) list[i] = o.perm[chunk.y + i];
+    __syncthreads();
+    const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
+    const int64_t col = ((int64_t)blockIdx.y * 4 + (threadIdx.x >> 6)) * (16 * NC) + c * NC;
+    if (col - c * NC >= a.q) return;
+    const T* __restrict__ Z = (const T*)a.Z + min(col, a.qp - NC);
+    const int r0 = blockIdx.z * 16 * KT;
+    f32x4 acc[KT][NC];
+#pragma unroll
+    for (int k = 0; k < KT; ++k)
+#pragma unroll
+        for (int j = 0; j < NC; ++j) acc[k][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    constexpr int RS = sizeof(T) == 2 ? 8 : 4;  // rows of a lane in a step of 4 RS rows
+    for (int i0 = 0; i0 < rows; i0 += 4 * RS) {
+        uint4 z[RS];
+        float h[KT][RS];
+#pragma unroll
+        for (int j = 0; j < RS; ++j) {
+            const int i = i0 + (sizeof(T) == 2 ? q * RS + j : j * 4 + q);
+            const bool in = i < rows;
+            const int64_t row = list[in ? i : rows - 1];
+            z[j] = *reinterpret_cast<const uint4*>(Z + row * a.ldz);
+#pragma unroll
+            for (int k = 0; k < KT; ++k) {
+                const int r = r0 + k * 16 + c;
+                h[k][j] = a.H[row * a.R + min(r, a.R - 1)];
+                if (!in) h[k][j] = 0.f;
+            }
+            if (!in) z[j] = make_uint4(0, 0, 0, 0);
+        }
+        if constexpr (sizeof(T) == 2) {
+            uint4 hp[KT][3];
+#pragma unroll
+            for (int k = 0; k < KT; ++k) {
+                uint32_t p[3][8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) split3(h[k][j], p[0][j], p[1][j], p[2][j]);
+#pragma unroll
+                for (int s = 0; s < 3; ++s)
+                    hp[k][s] = make_uint4(pack_high(p[s][0], p[s][1]), pack_high(p[s][2], p[s][3]), pack_high(p[s][4], p[s][5]),
+                                          pack_high(p[s][6], p[s][7]));
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const auto word = [&](int i) { return j / 2 == 0 ? z[i].x : j / 2 == 1 ? z[i].y : j / 2 == 2 ? z[i].z : z[i].w; };
+                const auto pair = [&](int i) { return j & 1 ? pack_high(word(i), word(i + 1)) : pack_low(word(i), word(i + 1)); };
+                const uint4 zc = make_uint4(pair(0), pair(2), pair(4), pair(6));
+#pragma unroll
+                for (int k = 0; k < KT; ++k)
+#pragma unroll
+                    for (int s = 0; s < 3; ++s) acc[k][j] = mma<T>(hp[k][s], zc, acc[k][j]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float v = __uint_as_float(j == 0 ? z[i].x : j == 1 ? z[i].y : j == 2 ? z[i].z : z[i].w);
+#pragma unroll
+                    for (int k = 0; k < KT; ++k) acc[k][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(h[k][i], v, acc[k][j], 0, 0, 0);
+                }
+        }
+    }
+    const float s = a.mul ? a.mul[g] : 1.f;
+    float* out = chunk.w >= 0 ? a.part + (int64_t)chunk.w * a.R * a.qp : a.D + g * a.sdd;
+    const int64_t ld = chunk.w >= 0 ? a.qp : a.ldd;
+#pragma unroll
+    for (int k = 0; k < KT; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int r = r0 + k * 16 + 4 * q + e;
+            if (r >= a.R) continue;
+            float* d = out + r * ld + col;
+            if (a.vec && col + NC <= a.q) {
+#pragma unroll
+                for (int j = 0; j < NC; j += 4)
+                    *reinterpret_cast<f32x4*>(d + j) = f32x4{acc[k][j][e], acc[k][j + 1][e], acc[k][j + 2][e], acc[k][j + 3][e]} * s;
+            } else {
+#pragma unroll
+                for (int j = 0; j < NC; ++j)
+                    if (col + j < a.q) d[j] = acc[k][j][e] * s;
+            }
+        }
+}
+
+// Adapters whose rows were cut into chunks: the partial sums in order; adapters without rows: zeros.
+__global__ void __launch_bounds__(256) outer_join_kernel(OuterArgs a, Groups o, int chunk_rows) {
+    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int g = blockIdx.z, r = blockIdx.y;
+    const int rows = o.start[g + 1] - o.start[g], nc = (rows + chunk_rows - 1) / chunk_rows;
+    if (nc == 1 || c >= a.q) return;
+    float s = 0.f;
+    const float* p = a.part + ((int64_t)o.multi0[g] * a.R + r) * a.qp + c;
+    for (int k = 0; k < nc; ++k) s += p[(int64_t)k * a.R * a.qp];
+    a.D[g * a.sdd + r * a.ldd + c] = s;
+}
+
+// ------------------------------------------------------------------------------------------
+// The shared product with the adapters' expand: O[i][c] = sum_k A[i][k] B[c][k] + (mul ? mul[a] : 1) sum_r H[i][r] W[a][r][c].
+//
+// BM x BN tiles, WM x WN waves; rows are taken in the order of the adapters (gathered by the loads, scattered by the
+// stores, at no cost), so few tiles hold more than one or two. The main loop stages 64 bytes of every row of A
+// and B at a time into a ring of NS LDS buffers by loads that go to LDS directly, NS - 1 steps ahead; the step's operands
+// are read from LDS into registers one step ahead, during the matrix instructions of the step before. After it the
+// rows' H (split exactly into three bf16) and the adapter's W take the ring's place, 64 bytes of ranks at a time,
+// and are multiplied into registers of their own, from where only the adapter's rows are added: a value that is not finite in one
+// adapter reaches no other's rows.
+struct GemmArgs {
+    const char *A, *B;
+    int64_t lda, ldb;  // bytes
+    int64_t M;
+    int N, steps;  // steps of 64 bytes
+    void* out;
+    int64_t ldo;
+    int vec;  // rows of out are aligned for four elements at a time
+    const float *H, *mul;
+    const char* W;
+    int64_t ldw;  // bytes between ranks
+    int G, R;
+    unsigned m_tiles, n_tiles, splits, per_xcd;
+    float* part;  // splits > 1: partial sums, splits x M x N
+};
+
+template <typename T, typename O, int BM, int BN, int WM, int WN, int NS>
+__global__ void __launch_bounds__(64 * WM * WN, 2)
+gemm_kernel(GemmArgs a, Groups o) {
+    constexpr int NT = 64 * WM * WN, MT = BM / WM / 16, NN = BN / WN / 16, SZ = (BM + BN) * 4;
+    constexpr int PA = BM * 4 / NT, PB = BN * 4 / NT;  // loads of a thread in a step
+    constexpr int PARTS = sizeof(T) == 2 ? 3 : 1, KR = 64 / (int)sizeof(T);
+    static_assert(PA + PB == 4, "the waits below count four loads a step");
+    static_assert(PARTS * BM * 4 + BN * 4 <= NS * SZ, "adapters take the ring's place");
+    __shared__ uint4 lds[NS * SZ + BM / 4];
+    int32_t* sid = reinterpret_cast<int32_t*>(lds + NS * SZ);
+    // XCD x (block i runs on XCD i % 8) takes a run of tiles; tiles go down 8 row tiles, then along the columns, so the
+    // tiles that run at the same time on an XCD share their rows of A and of B in its L2
+    const unsigned tiles = a.m_tiles * a.n_tiles, id = (blockIdx.x & 7u) * a.per_xcd + (blockIdx.x >> 3);
+    if (id >= tiles * a.splits) return;
+    const unsigned split = id / tiles, t = id % tiles, band = t / (8u * a.n_tiles), in = t % (8u * a.n_tiles);
+    const unsigned high = min(8u, a.m_tiles - band * 8u), mt = band * 8u + in % high, nt = in / high;
+    const int64_t m0 = (int64_t)mt * BM;
+    const int n0 = (int)nt * BN, live = (int)min((int64_t)BM, a.M - m0);
+    const int k0 = (int)((int64_t)a.steps * split / a.splits), steps = (int)((int64_t)a.steps * (split + 1) / a.splits) - k0;
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, wm = w / WN, wn = w % WN, fr = lane & 15, fq = lane >> 4;
+    const int32_t* __restrict__ perm = o.perm + m0;
+    // 16-byte chunk c of row r of a buffer lies at r * 4 + (c ^ F(r)): the 16 lanes that read one chunk of 16 rows hit all banks
+    auto F = [](int r) { return (4 - ((r >> 2) & 3)) & 3; };
+    const int srow = tid >> 2, sxc = (tid & 3) ^ F(srow);
+    const char* ga[PA];
+    const char* gb[PB];
+#pragma unroll
+    for (int i = 0; i < PA; ++i) ga[i] = a.A + perm[min(i * (NT / 4) + srow, live - 1)] * a.lda + sxc * 16 + (int64_t)k0 * 64;
+#pragma unroll
+    for (int i = 0; i < PB; ++i) gb[i] = a.B + min(n0 + i * (NT / 4) + srow, a.N - 1) * a.ldb + sxc * 16 + (int64_t)k0 * 64;
+    const uint32_t lds0 = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)reinterpret_cast<uintptr_t>(lds + 64 * w));
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // m0 is reserved: the clobber keeps the compiler's own uses safe
+    auto dma = [&](const char* g, uint32_t l) {
+        asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(l) : "memory", "m0");
+    };
+#pragma clang diagnostic pop
+    auto stage = [&](int kt) {
+        const uint32_t base = lds0 + (uint32_t)((kt % NS) * SZ) * 16u;
+#pragma unroll
+        for (int i = 0; i < PA; ++i) dma(ga[i] + (int64_t)kt * 64, base + i * NT * 16);
+#pragma unroll
+        for (int i = 0; i < PB; ++i) dma(gb[i] + (int64_t)kt * 64, base + (BM * 4 + i * NT) * 16);
+    };
+    // the wave's loads but the `younger` last steps' have landed, its LDS reads are in registers; then everyone's
+    auto wait = [&](int younger) {
+        if (younger >= 3) asm volatile("s_waitcnt vmcnt(12) lgkmcnt(0)" ::: "memory");
+        else if (younger == 2) asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)" ::: "memory");
+        else if (younger == 1) asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)" ::: "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    static_assert(NS == 4, "the waits count up to three younger steps");
+    const int ra = wm * MT * 16 + fr, rb = wn * NN * 16 + fr;
+    uint4 fa[2][MT], fb[2][NN];
+    auto read = [&](int kt, uint4 (&xa)[MT], uint4 (&xb)[NN]) {
+        const uint4* sa = lds + (kt % NS) * SZ;
+        const uint4* sb = sa + BM * 4;
+#pragma unroll
+        for (int ni = 0; ni < NN; ++ni) xb[ni] = sb[(rb + ni * 16) * 4 + (fq ^ F(rb + ni * 16))];
+#pragma unroll
+        for (int mi = 0; mi < MT; ++mi) xa[mi] = sa[(ra + mi * 16) * 4 + (fq ^ F(ra + mi * 16))];
+    };
+    f32x4 acc[MT][NN];
+#pragma unroll
+    for (int mi = 0; mi < MT; ++mi)
+#pragma unroll
+        for (int ni = 0; ni < NN; ++ni) acc[mi][ni] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto multiply = [&](const uint4 (&xa)[MT], const uint4 (&xb)[NN]) {
+#pragma unroll
+        for (int mi = 0; mi < MT; ++mi)
+#pragma unroll
+            for (int ni = 0; ni < NN; ++ni) acc[mi][ni] = mma<T>(xb[ni], xa[mi], acc[mi][ni]);
+    };
+    for (int i = tid; i < BM; i += NT) sid[i] = i < live ? o.sid[m0 + i] : a.G;
+    for (int kt = 0; kt < NS && kt < steps; ++kt) stage(kt);
+    // step kt: its operands are in registers; step kt + 1 has landed, step kt + 4 takes the buffer of step kt
+    wait(steps - 1);
+    read(0, fa[0], fb[0]);
+    auto step = [&](int kt, uint4 (&xa)[MT], uint4 (&xb)[NN], uint4 (&ya)[MT], uint4 (&yb)[NN]) {
+        if (kt + 1 < steps) {
+            wait(min(2, steps - 2 - kt));
+            if (kt + NS < steps) stage(kt + NS);
+            read(kt + 1, ya, yb);
+        }
+        multiply(xa, xb);
+    };
+    for (int kt = 0; kt < steps; kt += 2) {
+        step(kt, fa[0], fb[0], fa[1], fb[1]);
+        if (kt + 1 < steps) step(kt + 1, fa[1], fb[1], fa[0], fb[0]);
+    }
+    // the adapters of the tile's rows, one after the other (rows without one come last)
+    if (split == 0) {
+        uint4* st = lds;                      // PARTS x BM rows of 64 bytes of ranks
+        uint4* sw = lds + PARTS * BM * 4;      // BN columns of 64 bytes of ranks
+        for (int p0 = 0, p1; p0 < live; p0 = p1) {
+            const int g = __builtin_amdgcn_readfirstlane(sid[p0]);
+            if (g == a.G) break;
+            p1 = (int)min((int64_t)live, o.start[g + 1] - m0);
+            const float s = a.mul ? a.mul[g] : 1.f;
+            for (int r0 = 0; r0 < a.R; r0 += KR) {
+                __syncthreads();  // the ring, or the ranks before, have been read
+                constexpr int EH = BM * KR / NT, EW = BN * KR / NT;  // a thread's values of H and of W
+                static_assert(EH * (int)sizeof(T) == 32 && EW == EH, "two chunks of each");
+                {
+                    const int i = tid / (KR / EH), e0 = tid % (KR / EH) * EH;
+                    const bool has = i >= p0 && i < p1;
+                    const float* h = a.H + (int64_t)perm[has ? i : p0] * a.R + r0 + e0;
+                    float x[EH];
+#pragma unroll
+                    for (int e = 0; e < EH; ++e) x[e] = has && r0 + e0 + e < a.R ? h[e] * s : 0.f;
+                    const int at = i * 4, ch = e0 * (int)sizeof(T) / 16;
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const int to = at + ((ch + k) ^ F(i));
+                        if constexpr (sizeof(T) == 2) {
+                            uint32_t p[3][8];
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) split3(x[k * 8 + e], p[0][e], p[1][e], p[2][e]);
+#pragma unroll
+                            for (int u = 0; u < 3; ++u)
+                                st[u * BM * 4 + to] = make_uint4(pack_high(p[u][0], p[u][1]), pack_high(p[u][2], p[u][3]),
+                                                                 pack_high(p[u][4], p[u][5]), pack_high(p[u][6], p[u][7]));
+                        } else {
+                            st[to] = make_uint4(__float_as_uint(x[k * 4]), __float_as_uint(x[k * 4 + 1]),
+                                                __float_as_uint(x[k * 4 + 2]), __float_as_uint(x[k * 4 + 3]));
+                        }
+                    }
+                }
+                {
+                    const int i = tid % BN, e0 = tid / BN * EW, col = min(n0 + i, a.N - 1);
+                    const char* base = a.W + ((int64_t)g * a.R + r0 + e0) * a.ldw + (int64_t)col * sizeof(T);
+                    T x[EW];
+#pragma unroll
+                    for (int e = 0; e < EW; ++e) x[e] = r0 + e0 + e < a.R ? *reinterpret_cast<const T*>(base + e * a.ldw) : T(0);
+                    const int ch = e0 * (int)sizeof(T) / 16;
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        uint4 y;
+                        __builtin_memcpy(&y, x + k * (16 / sizeof(T)), 16);
+                        sw[i * 4 + ((ch + k) ^ F(i))] = y;
+                    }
+                }
+                __syncthreads();
+#pragma unroll
+                for (int ni = 0; ni < NN; ++ni) fb[0][ni] = sw[(rb + ni * 16) * 4 + (fq ^ F(rb + ni * 16))];
+#pragma unroll
+                for (int mi = 0; mi < MT; ++mi) {
+                    const int r = ra + mi * 16;
+                    if (r - fr + 16 <= p0 || r - fr >= p1) continue;  // none of the 16 rows
+                    f32x4 x[NN];
+#pragma unroll
+                    for (int ni = 0; ni < NN; ++ni) x[ni] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int u = 0; u < PARTS; ++u) {
+                        const uint4 h = st[(u * BM + r) * 4 + (fq ^ F(r))];
+#pragma unroll
+                        for (int ni = 0; ni < NN; ++ni) x[ni] = mma<T>(fb[0][ni], h, x[ni]);
+                    }
+                    if (r >= p0 && r < p1)
+#pragma unroll
+                        for (int ni = 0; ni < NN; ++ni) acc[mi][ni] += x[ni];
+                }
+            }
+        }
+    }
+    // lane: row ra + 16 mi, columns rb - fr + 16 ni + 4 fq + e
+    const bool partial = a.splits > 1;
+#pragma unroll
+    for (int mi = 0; mi < MT; ++mi) {
+        const int i = ra + mi * 16;
+        if (i >= live) continue;
+        const int64_t row = perm[i];
+#pragma unroll
+        for (int ni = 0; ni < NN; ++ni) {
+            const int c = n0 + rb - fr + ni * 16 + 4 * fq;
+            if (c >= a.N) continue;
+            if (partial) {
+                put4(a.part + ((int64_t)split * a.M + row) * a.N + c, acc[mi][ni], !(a.N & 3), a.N - c);
+            } else {
+                put4((O*)a.out + row * a.ldo + c, acc[mi][ni], a.vec, a.N - c);
+            }
+        }
+    }
+}
+
+// the sum of a product's splits, in order
+template <typename O>
+__global__ void __launch_bounds__(256) gemm_join_kernel(GemmArgs a) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, all = a.M * a.N;
+    if (i >= all) return;
+    float s = 0.f;
+    for (unsigned k = 0; k < a.splits; ++k) s += a.part[k * all + i];
+    store_as((O*)a.out + i / a.N * a.ldo + i % a.N, s);
+}
 int64_t padded(int64_t w, int32_t dtype) {
     const int64_t step = dtype == RP_BF16 ? 64 : 32;
     return (w + step - 1) / step * step;
 }
-
-size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
 
 // the arguments both directions share
 int check_shared(int32_t dtype, int64_t n, int64_t m, int64_t p, int64_t G, int32_t R) {
     if (dtype != RP_F32 && dtype != RP_BF16) return fail(RP_ERR_INVALID, "dtype must be RP_F32 or RP_BF16");
     if (n < 0 || m <= 0 || p <= 0 || G <= 0 || R <= 0) return fail(RP_ERR_INVALID, "bad shape");
     if (R > kMaxRank) return fail(RP_ERR_UNSUPPORTED, "rank %d is over %d", (int)R, kMaxRank);
-    if (n > INT32_MAX || m > INT32_MAX - 64 || p > INT32_MAX - 64 || G > 65535)
+    if (n > INT32_MAX || m > INT32_MAX - 64 || p > INT32_MAX - 64 || G > kMaxAdapters)
         return fail(RP_ERR_UNSUPPORTED, "n, m, p or the number of adapters too large");
     return RP_OK;
 }
@@ -108,52 +715,218 @@ int check_operand(const char* name, const void* p, int64_t ld, int64_t width, in
     return RP_OK;
 }
 
-template <typename T>
-int project(int device, const T* X, int64_t ldx, int64_t n, int64_t m, const T* C, int64_t p, const T* down, const T* up,
-            int64_t G, int R, const float* scale, const int32_t* ids, float* Y, int64_t ldy, float* hidden, hipStream_t st) {
-    constexpr int32_t dt = sizeof(T) == 2 ? RP_BF16 : RP_F32;
-    const int64_t mk = padded(m, dt), pk = padded(p, dt);
-    if (ldx != mk) return fail(RP_ERR_UNSUPPORTED, "rows of X must be contiguous");
-    int rc = rp_dense_project_device(device, X, dt, n, mk, C, p, Y, ldy, st, -1);
-    if (rc) return rc;
-    hipLaunchKernelGGL(shrink_kernel<T>, dim3((unsigned)((n + 3) / 4)), dim3(256), 0, st, X, ldx, n, mk, down, mk, G, R,
-                       (const float*)nullptr, ids, hidden);
+// Everything a call lays out in its workspace and launches, from its sizes alone.
+struct Plan {
+    int bits, tile_rows, chunk_rows, kt, waves;  // kt: shrink's rank tiles (1, 2, 4 or 8)
+    bool small;                                  // one block groups the rows
+    int64_t each;                                // else rows of a wave that counts
+    int n_chunks;
+    int64_t max_tiles, max_chunks, max_parts;
+    size_t perm, sid, start, tiles, chunks, tile0, chunk0, multi0, number, hist, hidden, t, part, bytes;
+};
+
+// split of a product over the contraction: enough blocks for 256 CUs with two each, where there are few tiles, as long as a split has
+// 16 steps (1 KB of a row)
+struct Tiling {
+    bool big;
+    unsigned m_tiles, n_tiles, splits;
+};
+Tiling tiling(int64_t M, int64_t N, int64_t steps) {
+    Tiling t;
+    t.big = ((M + 255) / 256) * ((N + 255) / 256) >= 192;
+    const int64_t b = t.big ? 256 : 128;
+    t.m_tiles = (unsigned)((M + b - 1) / b), t.n_tiles = (unsigned)((N + b - 1) / b);
+    const int64_t tiles = std::max<int64_t>(1, (int64_t)t.m_tiles * t.n_tiles);
+    t.splits = t.big || tiles >= 256 ? 1 : (unsigned)std::max<int64_t>(1, std::min<int64_t>({512 / tiles, steps / 16, 32}));
+    return t;
+}
+
+Plan plan_for(int32_t dtype, int64_t n, int64_t m, int64_t p, int64_t G, int R, int what) {
+    Plan l;
+    const int es = dtype == RP_BF16 ? 2 : 4;
+    const int64_t mk = padded(m, dtype), pk = padded(p, dtype);
+    l.bits = 1;
+    while ((G >> l.bits) != 0) ++l.bits;
+    l.kt = R <= 16 ? 1 : R <= 32 ? 2 : R <= 64 ? 4 : 8;
+    const int rt = l.kt <= 2 ? 4 : l.kt == 4 ? 2 : 1;
+    // many rows: as many of them as registers hold under one read of the adapter; few: 16, for more blocks
+    const bool many = n >= 512 * 16 * rt;
+    l.tile_rows = many ? 16 * rt : 16;
+    l.waves = many ? 4 : 8;
+    // chunks of rows for the banks' gradients: long, unless that leaves under 1024 blocks
+    l.chunk_rows = (int)std::max<int64_t>(64, std::min<int64_t>(kMaxChunk, n * ((m + 511) / 512) / 1024 / 64 * 64));
+    l.small = n <= 4096 && G <= 800;
+    l.each = 256;
+    while ((n + l.each - 1) / l.each * (G + 1) > (1 << 22)) l.each *= 2;
+    l.n_chunks = l.small ? 0 : (int)((n + l.each - 1) / l.each);
+    l.max_tiles = n / l.tile_rows + std::min(n, G + 1);
+    l.max_chunks = n / l.chunk_rows + std::min(n, G);
+    l.max_parts = 2 * (n / l.chunk_rows);
+    size_t at = 0;
+    const auto take = [&](size_t b) {
+        const size_t r = at;
+        at = (at + b + 255) & ~(size_t)255;
+        return r;
+    };
+    l.perm = take(4 * n), l.sid = take(4 * n), l.start = take(4 * (G + 2));
+    l.tiles = take(16 * l.max_tiles), l.chunks = take(16 * l.max_chunks);
+    l.tile0 = take(4 * (G + 1)), l.chunk0 = take(4 * (G + 1)), l.multi0 = take(4 * (G + 1)), l.number = take(8);
+    l.hist = take((size_t)4 * l.n_chunks * (G + 1));
+    l.hidden = l.t = l.part = at;
+    if (what == RP_ADAPT_PROJECT) {
+        l.hidden = take((size_t)4 * n * R);
+        const Tiling g = tiling(n, p, mk * es / 64);
+        l.part = take(g.splits > 1 ? (size_t)4 * g.splits * n * p : 0);
+    } else {
+        l.t = take((size_t)4 * n * R);
+        size_t part = (size_t)4 * l.max_parts * R * std::max(mk, pk);
+        if (what == RP_ADAPT_GRADIENTS_DX) {
+            const Tiling g = tiling(n, m, pk * es / 64);
+            if (g.splits > 1) part = std::max(part, (size_t)4 * g.splits * n * m);
+        }
+        l.part = take(part);
+    }
+    l.bytes = at;
+    return l;
+}
+
+Groups groups_of(const Plan& l, char* ws) {
+    Groups o;
+    o.perm = (int32_t*)(ws + l.perm), o.sid = (int32_t*)(ws + l.sid), o.start = (int32_t*)(ws + l.start);
+    o.tiles = (int4*)(ws + l.tiles), o.chunks = (int4*)(ws + l.chunks);
+    o.tile0 = (int32_t*)(ws + l.tile0), o.chunk0 = (int32_t*)(ws + l.chunk0), o.multi0 = (int32_t*)(ws + l.multi0);
+    o.number = (int32_t*)(ws + l.number), o.hist = (int32_t*)(ws + l.hist);
+    return o;
+}
+
+int launch_groups(const Plan& l, const Groups& o, const int32_t* ids, int64_t n, int G, hipStream_t st) {
+    if (l.small) {
+        hipLaunchKernelGGL(group_small_kernel, dim3(1), dim3(1024), 4 * (17 * (G + 1) + 1), st, ids, (int)n, G, l.bits, l.tile_rows,
+                           l.chunk_rows, o);
+    } else {
+        const int waves = G < 4000 ? 4 : 1;
+        const dim3 grid((unsigned)((l.n_chunks + waves - 1) / waves)), block(64 * waves);
+        const size_t lds = (size_t)4 * waves * (G + 1);
+        hipLaunchKernelGGL(group_count_kernel, grid, block, lds, st, ids, n, G, l.bits, l.each, l.n_chunks, o);
+        HIP_TRY(hipGetLastError());
+        hipLaunchKernelGGL(group_scan_kernel, dim3(1), dim3(1024), 0, st, n, G, l.n_chunks, l.tile_rows, l.chunk_rows, o);
+        HIP_TRY(hipGetLastError());
+        hipLaunchKernelGGL(group_place_kernel, grid, block, lds, st, ids, n, G, l.bits, l.each, l.n_chunks, o);
+    }
     HIP_TRY(hipGetLastError());
-    hipLaunchKernelGGL((expand_kernel<T, float>), dim3((unsigned)n), dim3(256), 0, st, Y, ldy, Y, ldy, n, p, up, pk, G, R,
-                       scale, ids, hidden);
+    return RP_OK;
+}
+
+template <typename T, int RT, int KT, int NW>
+int launch_shrink_as(const Plan& l, const T* Z, int64_t ldz, int64_t kp, const T* W, int G, int R, const float* mul, const Groups& o,
+                     float* H, hipStream_t st) {
+    hipLaunchKernelGGL((shrink_kernel<T, RT, KT, NW>), dim3((unsigned)l.max_tiles), dim3(64 * NW), 0, st, Z, ldz, kp, W, G, R, mul, o, H);
     HIP_TRY(hipGetLastError());
     return RP_OK;
 }
 
 template <typename T>
-int gradients(int device, const T* dY, int64_t lddy, const T* X, int64_t ldx, int64_t n, int64_t m, int64_t p, const T* Ct,
-              const T* down, const T* up, int64_t G, int R, const float* scale, const int32_t* ids, const float* hidden, T* dX,
-              int64_t lddx, float* d_down, int64_t ldd, int64_t sdd, float* d_up, int64_t ldu, int64_t sdu, char* ws,
-              hipStream_t st) {
-    constexpr int32_t dt = sizeof(T) == 2 ? RP_BF16 : RP_F32;
-    const int64_t mk = padded(m, dt), pk = padded(p, dt);
-    float* t = (float*)ws;
-    if (n) {
-        hipLaunchKernelGGL(shrink_kernel<T>, dim3((unsigned)((n + 3) / 4)), dim3(256), 0, st, dY, lddy, n, pk, up, pk, G, R, scale,
-                           ids, t);
+int launch_shrink(const Plan& l, const T* Z, int64_t ldz, int64_t kp, const T* W, int G, int R, const float* mul, const Groups& o,
+                  float* H, hipStream_t st) {
+    if (l.waves == 4) switch (l.kt) {
+            case 1: return launch_shrink_as<T, 4, 1, 4>(l, Z, ldz, kp, W, G, R, mul, o, H, st);
+            case 2: return launch_shrink_as<T, 4, 2, 4>(l, Z, ldz, kp, W, G, R, mul, o, H, st);
+            case 4: return launch_shrink_as<T, 2, 4, 4>(l, Z, ldz, kp, W, G, R, mul, o, H, st);
+            default: return launch_shrink_as<T, 1, 8, 4>(l, Z, ldz, kp, W, G, R, mul, o, H, st);
+        }
+    switch (l.kt) {
+        case 1: return launch_shrink_as<T, 1, 1, 8>(l, Z, ldz, kp, W, G, R, mul, o, H, st);
+        case 2: return launch_shrink_as<T, 1, 2, 8>(l, Z, ldz, kp, W, G, R, mul, o, H, st);
+        case 4: return launch_shrink_as<T, 1, 4, 8>(l, Z, ldz, kp, W, G, R, mul, o, H, st);
+        default: return launch_shrink_as<T, 1, 8, 8>(l, Z, ldz, kp, W, G, R, mul, o, H, st);
+    }
+}
+
+template <typename T>
+int launch_outer(const Plan& l, const OuterArgs& a, const Groups& o, int G, hipStream_t st) {
+    if (l.max_chunks) {
+        const int64_t wide = 4 * 16 * (sizeof(T) == 2 ? 8 : 4);
+        const unsigned qb = (unsigned)((a.q + wide - 1) / wide);
+        if (qb > 65535) return fail(RP_ERR_UNSUPPORTED, "m or p too large");
+        const int kt = a.R <= 16 ? 1 : a.R <= 32 ? 2 : 4;
+        const dim3 grid((unsigned)l.max_chunks, qb, (unsigned)((a.R + 16 * kt - 1) / (16 * kt))), block(256);
+        if (kt == 1) hipLaunchKernelGGL((outer_kernel<T, 1>), grid, block, 0, st, a, o);
+        else if (kt == 2) hipLaunchKernelGGL((outer_kernel<T, 2>), grid, block, 0, st, a, o);
+        else hipLaunchKernelGGL((outer_kernel<T, 4>), grid, block, 0, st, a, o);
         HIP_TRY(hipGetLastError());
     }
-    hipLaunchKernelGGL(outer_kernel<T>, dim3((unsigned)((m + 255) / 256), (unsigned)std::min<int64_t>(G * R, 65535)), dim3(256), 0, st, X, ldx, n, m, G, R,
-                       (const float*)nullptr, ids, t, d_down, ldd, sdd);
+    hipLaunchKernelGGL(outer_join_kernel, dim3((unsigned)((a.q + 255) / 256), (unsigned)a.R, (unsigned)G), dim3(256), 0, st, a, o,
+                       l.chunk_rows);
     HIP_TRY(hipGetLastError());
-    hipLaunchKernelGGL(outer_kernel<T>, dim3((unsigned)((p + 255) / 256), (unsigned)std::min<int64_t>(G * R, 65535)), dim3(256), 0, st, dY, lddy, n, p, G,
-                       R, scale, ids, hidden, d_up, ldu, sdu);
+    return RP_OK;
+}
+
+template <typename T, typename O>
+int launch_gemm(GemmArgs a, const Groups& o, hipStream_t st) {
+    const Tiling t = tiling(a.M, a.N, a.steps);
+    a.m_tiles = t.m_tiles, a.n_tiles = t.n_tiles, a.splits = t.splits;
+    const uint64_t per = ((uint64_t)t.m_tiles * t.n_tiles * t.splits + 7) / 8;
+    if (per * 8 >= (1ull << 31)) return fail(RP_ERR_UNSUPPORTED, "too many rows for one launch");
+    a.per_xcd = (unsigned)per;
+    if (t.big) hipLaunchKernelGGL((gemm_kernel<T, O, 256, 256, 2, 4, 4>), dim3(a.per_xcd * 8), dim3(512), 0, st, a, o);
+    else hipLaunchKernelGGL((gemm_kernel<T, O, 128, 128, 2, 2, 4>), dim3(a.per_xcd * 8), dim3(256), 0, st, a, o);
     HIP_TRY(hipGetLastError());
-    if (dX && n) {
-        if (lddy != pk) return fail(RP_ERR_UNSUPPORTED, "rows of dY must be contiguous");
-        float* tmp = (float*)(ws + align256((size_t)n * R * 4));
-        int rc = rp_dense_project_device(device, dY, dt, n, pk, Ct, m, tmp, m, st, -1);
-        if (rc) return rc;
-        hipLaunchKernelGGL((expand_kernel<T, T>), dim3((unsigned)n), dim3(256), 0, st, tmp, m, dX, lddx, n, m, down, mk, G, R,
-                           (const float*)nullptr, ids, t);
+    if (t.splits > 1) {
+        hipLaunchKernelGGL(gemm_join_kernel<O>, dim3((unsigned)((a.M * a.N + 255) / 256)), dim3(256), 0, st, a);
         HIP_TRY(hipGetLastError());
     }
     return RP_OK;
+}
+
+template <typename T, typename O>
+GemmArgs gemm_args(const T* A, int64_t lda, const T* B, int64_t kp, int64_t M, int64_t N, O* out, int64_t ldo, const float* H,
+                   const float* mul, const T* W, int64_t wp, int G, int R, void* part) {
+    GemmArgs a{};
+    a.A = (const char*)A, a.B = (const char*)B, a.lda = lda * (int64_t)sizeof(T), a.ldb = kp * (int64_t)sizeof(T);
+    a.M = M, a.N = (int)N, a.steps = (int)(kp * (int64_t)sizeof(T) / 64), a.out = out, a.ldo = ldo;
+    a.vec = !((uintptr_t)out & (4 * sizeof(O) - 1)) && ldo % 4 == 0;
+    a.H = H, a.mul = mul, a.W = (const char*)W, a.ldw = wp * (int64_t)sizeof(T), a.G = G, a.R = R, a.part = (float*)part;
+    return a;
+}
+
+template <typename T>
+int project(const T* X, int64_t ldx, int64_t n, int64_t m, const T* C, int64_t p, const T* down, const T* up, int G, int R,
+            const float* scale, const int32_t* ids, float* Y, int64_t ldy, float* hidden, char* ws, hipStream_t st) {
+    constexpr int32_t dt = sizeof(T) == 2 ? RP_BF16 : RP_F32;
+    const int64_t mk = padded(m, dt), pk = padded(p, dt);
+    const Plan l = plan_for(dt, n, m, p, G, R, RP_ADAPT_PROJECT);
+    const Groups o = groups_of(l, ws);
+    if (!hidden) hidden = (float*)(ws + l.hidden);
+    int rc = launch_groups(l, o, ids, n, G, st);
+    if (!rc) rc = launch_shrink<T>(l, X, ldx, mk, down, G, R, nullptr, o, hidden, st);
+    if (!rc) rc = launch_gemm<T, float>(gemm_args<T, float>(X, ldx, C, mk, n, p, Y, ldy, hidden, scale, up, pk, G, R, ws + l.part), o, st);
+    return rc;
+}
+
+template <typename T>
+OuterArgs outer_args(const T* Z, int64_t ldz, int64_t qp, int64_t q, int R, const float* mul, const float* H, float* D, int64_t ldd,
+                     int64_t sdd, char* part) {
+    OuterArgs a{Z, ldz, qp, q, R, mul, H, D, ldd, sdd, (float*)part, 0};
+    a.vec = !((uintptr_t)D & 15) && ldd % 4 == 0 && sdd % 4 == 0;
+    return a;
+}
+
+template <typename T>
+int gradients(const T* dY, int64_t lddy, const T* X, int64_t ldx, int64_t n, int64_t m, int64_t p, const T* Ct, const T* down,
+              const T* up, int G, int R, const float* scale, const int32_t* ids, const float* hidden, T* dX, int64_t lddx,
+              float* d_down, int64_t ldd, int64_t sdd, float* d_up, int64_t ldu, int64_t sdu, char* ws, hipStream_t st) {
+    constexpr int32_t dt = sizeof(T) == 2 ? RP_BF16 : RP_F32;
+    const int64_t mk = padded(m, dt), pk = padded(p, dt);
+    const Plan l = plan_for(dt, n, m, p, G, R, dX ? RP_ADAPT_GRADIENTS_DX : RP_ADAPT_GRADIENTS);
+    const Groups o = groups_of(l, ws);
+    float* t = (float*)(ws + l.t);
+    int rc = launch_groups(l, o, ids, n, G, st);
+    if (!rc && n) rc = launch_shrink<T>(l, dY, lddy, pk, up, G, R, scale, o, t, st);
+    if (!rc) rc = launch_outer<T>(l, outer_args<T>(X, ldx, mk, m, R, nullptr, t, d_down, ldd, sdd, ws + l.part), o, G, st);
+    if (!rc) rc = launch_outer<T>(l, outer_args<T>(dY, lddy, pk, p, R, scale, hidden, d_up, ldu, sdu, ws + l.part), o, G, st);
+    if (!rc && dX && n)
+        rc = launch_gemm<T, T>(gemm_args<T, T>(dY, lddy, Ct, pk, n, m, dX, lddx, t, nullptr, down, mk, G, R, ws + l.part), o, st);
+    return rc;
 }
 
 }  // namespace
@@ -163,9 +936,7 @@ extern "C" {
 int64_t rp_adapt_workspace_bytes(int32_t dtype, int64_t n, int64_t m, int64_t p, int64_t adapters, int32_t rank,
                                  int32_t what) {
     if (check_shared(dtype, n, m, p, adapters, rank)) return -1;
-    size_t b = align256((size_t)n * rank * 4);
-    if (what == RP_ADAPT_GRADIENTS_DX) b += (size_t)n * m * 4;
-    return (int64_t)b;
+    return (int64_t)plan_for(dtype, n, m, p, adapters, rank, what).bytes;
 }
 
 int rp_adapt_project_device(int device, const void* X, int64_t ldx, int32_t dtype, int64_t n, int64_t m, const void* C,
@@ -186,13 +957,14 @@ int rp_adapt_project_device(int device, const void* X, int64_t ldx, int32_t dtyp
         return fail(RP_ERR_INVALID, "workspace must be 256-byte aligned and hold %lld bytes", (long long)need);
     DeviceGuard guard;
     if ((rc = guard.enter(device))) return rc;
-    if (!hidden) hidden = (float*)workspace;
     hipStream_t st = (hipStream_t)stream;
     if (dtype == RP_BF16)
-        return project<uint16_t>(device, (const uint16_t*)X, ldx, n, m, (const uint16_t*)C, p, (const uint16_t*)down,
-                                 (const uint16_t*)up, adapters, rank, scale, ids, Y, ldy, hidden, st);
-    return project<float>(device, (const float*)X, ldx, n, m, (const float*)C, p, (const float*)down, (const float*)up, adapters,
-                          rank, scale, ids, Y, ldy, hidden, st);
+        return project<uint16_t>((const uint16_t*)X, ldx, n, m, (const uint16_t*)C, p, (const uint16_t*)down,
+                                 (const uint16_t*)up, (int)adapters, rank, scale, ids, Y, ldy, hidden,
+                                 (char*)workspace, st);
+    return project<float>((const float*)X, ldx, n, m, (const float*)C, p, (const float*)down, (const float*)up, adapters,
+                          rank, scale, ids, Y, ldy, hidden,
+                                 (char*)workspace, st);
 }
 
 int rp_adapt_gradients_device(int device, const void* dY, int64_t lddy, const void* X, int64_t ldx, int32_t dtype, int64_t n,
@@ -220,10 +992,10 @@ int rp_adapt_gradients_device(int device, const void* dY, int64_t lddy, const vo
     if ((rc = guard.enter(device))) return rc;
     hipStream_t st = (hipStream_t)stream;
     if (dtype == RP_BF16)
-        return gradients<uint16_t>(device, (const uint16_t*)dY, lddy, (const uint16_t*)X, ldx, n, m, p, (const uint16_t*)Ct,
-                                   (const uint16_t*)down, (const uint16_t*)up, adapters, rank, scale, ids, hidden, (uint16_t*)dX,
+        return gradients<uint16_t>((const uint16_t*)dY, lddy, (const uint16_t*)X, ldx, n, m, p, (const uint16_t*)Ct,
+                                   (const uint16_t*)down, (const uint16_t*)up, (int)adapters, rank, scale, ids, hidden, (uint16_t*)dX,
                                    lddx, d_down, d_down_row, d_down_adapter, d_up, d_up_row, d_up_adapter, (char*)workspace, st);
-    return gradients<float>(device, (const float*)dY, lddy, (const float*)X, ldx, n, m, p, (const float*)Ct, (const float*)down,
+    return gradients<float>((const float*)dY, lddy, (const float*)X, ldx, n, m, p, (const float*)Ct, (const float*)down,
                             (const float*)up, adapters, rank, scale, ids, hidden, (float*)dX, lddx, d_down, d_down_row,
                             d_down_adapter, d_up, d_up_row, d_up_adapter, (char*)workspace, st);
 }

@@ -147,3 +147,14 @@ def test_abi_refuses_before_the_device_is_used():
     assert lib.rp_adamw_step(None, 1e-3, 0.9, 0.999, 1e-8, 0.0, 0, None, None) == nat.RP_ERR_INVALID
     assert lib.rp_adamw_values(None, None, None, None) == nat.RP_ERR_INVALID
     assert lib.rp_adamw_destroy(None) == nat.RP_OK
+
+
+def test_workspace_of_every_size():
+    lib = nat.load()
+    for dtype in (nat.RP_F32, nat.RP_BF16):
+        for n in (0, 1, 64, 65, 5000, 10 ** 7):
+            for m, p in ((1, 1), (16384, 1024), (100, 70000)):
+                for G, R in ((1, 1), (16383, 128)):
+                    project, gradients, dx = (lib.rp_adapt_workspace_bytes(dtype, n, m, p, G, R, k) for k in (
+                        nat.RP_ADAPT_PROJECT, nat.RP_ADAPT_GRADIENTS, nat.RP_ADAPT_GRADIENTS_DX))
+                    assert project >= 0 and dx >= gradients >= 4 * n * R

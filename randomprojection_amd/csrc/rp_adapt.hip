@@ -12,6 +12,8 @@
 //   shrink  H = Z W^T      (n x q, R x q -> n x R)
 //   expand  O += H W       (n x R, R x q -> n x q)
 //   outer   dW = H^T Z     (per adapter, over its rows)
+#include <type_traits>
+
 #include "rp_common.h"
 
 using namespace rpd;
@@ -20,14 +22,14 @@ namespace {
 
 constexpr int kMaxRank = 128, kMaxAdapters = 16383;  // a wave's counts of all groups fit 64 KB of LDS
 
-// round to nearest even; a NaN stays one
-__device__ __forceinline__ uint16_t to_bf16(float x) {
-    const uint32_t u = __float_as_uint(x);
-    if ((u & 0x7fffffffu) > 0x7f800000u) return (uint16_t)((u >> 16) | 0x40u);
-    return (uint16_t)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
+// rounded to nearest even, two at a time (one instruction); a NaN stays one
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t to_bf16(float a, float b) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
 }
 __device__ __forceinline__ void store_as(float* p, float x) { *p = x; }
-__device__ __forceinline__ void store_as(uint16_t* p, float x) { *p = to_bf16(x); }
+__device__ __forceinline__ void store_as(uint16_t* p, float x) { *p = (uint16_t)to_bf16(x, 0.f); }
 
 // ------------------------------------------------------------------------------------------
 // Rows grouped by adapter: a stable counting sort of the ids (rows without an adapter come last, as
@@ -238,19 +240,9 @@ typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 
-// four neighbouring values, of which the first `left` are inside
-__device__ __forceinline__ void put4(float* p, f32x4 x, int vec, int left) {
-    if (vec && left >= 4) *reinterpret_cast<f32x4*>(p) = x;
-    else
-        for (int e = 0; e < 4; ++e)
-            if (e < left) p[e] = x[e];
-}
-__device__ __forceinline__ void put4(uint16_t* p, f32x4 x, int vec, int left) {
-    if (vec && left >= 4)
-        *reinterpret_cast<uint2*>(p) = make_uint2(to_bf16(x[0]) | (uint32_t)to_bf16(x[1]) << 16, to_bf16(x[2]) | (uint32_t)to_bf16(x[3]) << 16);
-    else
-        for (int e = 0; e < 4; ++e)
-            if (e < left) p[e] = to_bf16(x[e]);
+__device__ __forceinline__ void put4(float* p, f32x4 x) { *reinterpret_cast<f32x4*>(p) = x; }
+__device__ __forceinline__ void put4(uint16_t* p, f32x4 x) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(to_bf16(x[0], x[1]), to_bf16(x[2], x[3]));
 }
 
 template <typename T>
@@ -277,28 +269,48 @@ __device__ __forceinline__ void split3(float x, uint32_t& hi, uint32_t& mid, uin
 __device__ __forceinline__ uint32_t pack_high(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
 __device__ __forceinline__ uint32_t pack_low(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
 
-// H[i][r] = (mul ? mul[a] : 1) sum_q Z[i][q] W[a][r][q]; zeros for rows without an adapter. A block takes a tile
+// The factor that the expand reads: `parts` pieces of scale[a] H[i][r] for every row, each of its ranks padded with zeros to 64
+// bytes. bf16: the pieces of split3; f32: the value itself.
+__host__ __device__ __forceinline__ int padded_rank(int R, int size) { return size == 2 ? (R + 31) / 32 * 32 : (R + 15) / 16 * 16; }
+template <typename T>
+__host__ __device__ constexpr int pieces() { return sizeof(T) == 2 ? 3 : 1; }
+
+struct ShrinkArgs {
+    const void* Z;
+    int64_t ldz, kp;
+    const void* W;
+    int G, R;
+    const float* scale;  // or NULL: 1
+    float* H;            // or NULL; n x R
+    int scaled;          // H takes the scale too
+    void* S;             // or NULL; n x pieces x padded rank
+};
+
+// H[i][r] = (scaled ? scale[a] : 1) sum_q Z[i][q] W[a][r][q], zeros for rows without an adapter, and its pieces. A block takes a tile
 // of 16 RT rows of one group; its NW waves split the contraction and add up in LDS in their order. Bound by
 // reading Z once: the wave holds 16 RT x 16 KT of H, so W (from L2) is read once for 16 RT rows, and there is
 // nothing between the loads and the matrix instructions.
 template <typename T, int RT, int KT, int NW>
 __global__ void __launch_bounds__(64 * NW)
-shrink_kernel(const T* __restrict__ Z, int64_t ldz, int64_t kp, const T* __restrict__ W, int G, int R, const float* __restrict__ mul,
-              Groups o, float* __restrict__ H) {
+shrink_kernel(ShrinkArgs a, Groups o) {
     __shared__ f32x4 red[NW][RT * KT][64];
     if ((int)blockIdx.x >= o.number[0]) return;
     const int4 tile = o.tiles[blockIdx.x];
-    const int g = tile.x, pos = tile.y, rows = tile.z;
+    const int g = tile.x, pos = tile.y, rows = tile.z, R = a.R;
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, c = lane & 15, q = lane >> 4;
-    if (g == G) {
-        for (int i = tid; i < rows * R; i += 64 * NW) H[(int64_t)o.perm[pos + i / R] * R + i % R] = 0.f;
+    if (g == a.G) {
+        if (a.H)
+            for (int i = tid; i < rows * R; i += 64 * NW) a.H[(int64_t)o.perm[pos + i / R] * R + i % R] = 0.f;
         return;
     }
+    const T* __restrict__ Z = (const T*)a.Z;
+    const T* __restrict__ W = (const T*)a.W;
+    const int64_t kp = a.kp;
     const char* z[RT];
     const char* b[KT];
 #pragma unroll
     for (int t = 0; t < RT; ++t)
-        z[t] = reinterpret_cast<const char*>(Z + o.perm[pos + min(t * 16 + c, rows - 1)] * ldz) + q * 16;
+        z[t] = reinterpret_cast<const char*>(Z + o.perm[pos + min(t * 16 + c, rows - 1)] * a.ldz) + q * 16;
 #pragma unroll
     for (int j = 0; j < KT; ++j)
         b[j] = reinterpret_cast<const char*>(W + ((int64_t)g * R + min(j * 16 + c, R - 1)) * kp) + q * 16;
@@ -330,7 +342,8 @@ shrink_kernel(const T* __restrict__ Z, int64_t ldz, int64_t kp, const T* __restr
 #pragma unroll
         for (int j = 0; j < KT; ++j) red[w][t * KT + j][lane] = acc[t][j];
     __syncthreads();
-    const float s = mul ? mul[g] : 1.f;
+    const float s = a.scale ? a.scale[g] : 1.f;
+    const int rp = padded_rank(R, sizeof(T));
     for (int i = tid; i < RT * KT * 64; i += 64 * NW) {
         const f32x4* p = &red[0][0][0] + i;
         f32x4 x = p[0];
@@ -338,10 +351,31 @@ shrink_kernel(const T* __restrict__ Z, int64_t ldz, int64_t kp, const T* __restr
         for (int k = 1; k < NW; ++k) x += p[k * RT * KT * 64];
         const int l = i & 63, row = i / (64 * KT) * 16 + (l & 15), r = (i >> 6) % KT * 16 + 4 * (l >> 4);
         if (row >= rows) continue;
-        float* h = H + (int64_t)o.perm[pos + row] * R + r;
+        const int64_t at = o.perm[pos + row];
+        f32x4 y = x * s;
+        if (a.H) {
+            float* h = a.H + at * R + r;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (r + e < R) h[e] = a.scaled ? y[e] : x[e];
+        }
+        if (!a.S || r >= rp) continue;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            if (r + e < R) h[e] = x[e] * s;
+            if (r + e >= R) y[e] = 0.f;
+        if constexpr (sizeof(T) == 2) {
+            uint32_t v[3][4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) split3(y[e], v[0][e], v[1][e], v[2][e]);
+            uint16_t* d = (uint16_t*)a.S + at * 3 * rp + r;
+#pragma unroll
+            for (int u = 0; u < 3; ++u) {
+                *reinterpret_cast<uint2*>(d + u * rp) = make_uint2(pack_high(v[u][0], v[u][1]), pack_high(v[u][2], v[u][3]));
+                if (KT == 1) *reinterpret_cast<uint2*>(d + u * rp + 16) = make_uint2(0, 0);  // ranks 16 .. 31
+            }
+        } else {
+            *reinterpret_cast<f32x4*>((float*)a.S + at * rp + r) = y;
+        }
     }
 }
 
@@ -470,41 +504,49 @@ __global__ void __launch_bounds__(256) outer_join_kernel(OuterArgs a, Groups o, 
 }
 
 // ------------------------------------------------------------------------------------------
-// The shared product with the adapters' expand: O[i][c] = sum_k A[i][k] B[c][k] + (mul ? mul[a] : 1) sum_r H[i][r] W[a][r][c].
+// The shared product with the adapters' expand: O[i][c] = sum_k A[i][k] B[c][k] + sum_r (scale[a] H[i][r]) W[a][r][c].
 //
 // BM x BN tiles, WM x WN waves; rows are taken in the order of the adapters (gathered by the loads, scattered by the
-// stores, at no cost), so few tiles hold more than one or two. The main loop stages 64 bytes of every row of A
-// and B at a time into a ring of NS LDS buffers by loads that go to LDS directly, NS - 1 steps ahead; the step's operands
-// are read from LDS into registers one step ahead, during the matrix instructions of the step before. After it the
-// rows' H (split exactly into three bf16) and the adapter's W take the ring's place, 64 bytes of ranks at a time,
-// and are multiplied into registers of their own, from where only the adapter's rows are added: a value that is not finite in one
-// adapter reaches no other's rows.
+// stores, at no cost), so few tiles hold more than one or two. The main loop stages 128 bytes of every row of A and B
+// at a time into two LDS buffers by loads that go to LDS directly. Whole lines: with 64 bytes a stage every line crossed
+// from L2 twice (its other half had left the L1 by the next stage): 1.10 against 1.25 to 1.31 PFLOP/s at 65536 x 16384 ->
+// 1024. A stage is multiplied in two halves, each half's operands read into registers during the half before; in the middle all
+// waves meet once, the other buffer having landed, and the stage after the next starts into this one.
+// After it the pieces of the rows' H (exact in three bf16) and the adapter's W take the buffers' place, 64 bytes of ranks
+// at a time, and are multiplied into registers of their own, from where only the adapter's rows are added: a value that is
+// not finite in one adapter reaches no other's rows. The result goes through LDS so that rows are stored 128 bytes at a
+// time (16 rows a store otherwise: 0.58 against 0.53 ms at 16384 x 1024 -> 16384 with bf16 out).
 struct GemmArgs {
     const char *A, *B;
     int64_t lda, ldb;  // bytes
     int64_t M;
-    int N, steps;  // steps of 64 bytes
+    int N, steps;  // stages of 128 bytes of a row
     void* out;
     int64_t ldo;
-    int vec;  // rows of out are aligned for four elements at a time
-    const float *H, *mul;
+    int vec;  // rows of out are 16-byte aligned
+    const char* S;  // the rows' factors (ShrinkArgs)
     const char* W;
-    int64_t ldw;  // bytes between ranks
+    int64_t ldw;    // bytes between ranks
     int G, R;
     unsigned m_tiles, n_tiles, splits, per_xcd;
     float* part;  // splits > 1: partial sums, splits x M x N
 };
 
-template <typename T, typename O, int BM, int BN, int WM, int WN, int NS>
+template <typename T, typename O, int BM, int BN, int WM, int WN>
 __global__ void __launch_bounds__(64 * WM * WN, 2)
 gemm_kernel(GemmArgs a, Groups o) {
-    constexpr int NT = 64 * WM * WN, MT = BM / WM / 16, NN = BN / WN / 16, SZ = (BM + BN) * 4;
-    constexpr int PA = BM * 4 / NT, PB = BN * 4 / NT;  // loads of a thread in a step
-    constexpr int PARTS = sizeof(T) == 2 ? 3 : 1, KR = 64 / (int)sizeof(T);
-    static_assert(PA + PB == 4, "the waits below count four loads a step");
-    static_assert(PARTS * BM * 4 + BN * 4 <= NS * SZ, "adapters take the ring's place");
-    __shared__ uint4 lds[NS * SZ + BM / 4];
-    int32_t* sid = reinterpret_cast<int32_t*>(lds + NS * SZ);
+    constexpr int NT = 64 * WM * WN, MT = BM / WM / 16, NN = BN / WN / 16, SZ = (BM + BN) * 8;
+    constexpr int PA = BM * 8 / NT, PB = BN * 8 / NT, P = PA + PB;  // loads of a thread in a stage
+    // hi, mid and low of H; a result in bf16 does without low (2^-17 of H, against a rounding of 2^-9)
+    constexpr int PARTS = sizeof(T) == 4 ? 1 : sizeof(O) == 4 ? 3 : 2, KR = 64 / (int)sizeof(T);
+    static_assert(NT >= BM, "a row a thread");
+    static_assert(P == 8, "the first wait below counts eight loads a stage");
+    static_assert(2 * (PARTS * BM * 4 + BN * 4) <= 2 * SZ, "adapters take the buffers' place");
+    static_assert(WM * WN * MT * 16 * 8 <= 2 * SZ && NN == 4, "so do the stores, 64 columns a wave");
+    __shared__ uint4 lds[2 * SZ + BM * 3 / 4];
+    int32_t* sid = reinterpret_cast<int32_t*>(lds + 2 * SZ);  // the tile's rows' groups
+    int32_t* rows = sid + BM;                                 // where they are
+    int32_t* ends = rows + BM;                                // where in the tile their group ends
     // XCD x (block i runs on XCD i % 8) takes a run of tiles; tiles go down 8 row tiles, then along the columns, so the
     // tiles that run at the same time on an XCD share their rows of A and of B in its L2
     const unsigned tiles = a.m_tiles * a.n_tiles, id = (blockIdx.x & 7u) * a.per_xcd + (blockIdx.x >> 3);
@@ -515,171 +557,204 @@ gemm_kernel(GemmArgs a, Groups o) {
     const int n0 = (int)nt * BN, live = (int)min((int64_t)BM, a.M - m0);
     const int k0 = (int)((int64_t)a.steps * split / a.splits), steps = (int)((int64_t)a.steps * (split + 1) / a.splits) - k0;
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, wm = w / WN, wn = w % WN, fr = lane & 15, fq = lane >> 4;
-    const int32_t* __restrict__ perm = o.perm + m0;
-    // 16-byte chunk c of row r of a buffer lies at r * 4 + (c ^ F(r)): the 16 lanes that read one chunk of 16 rows hit all banks
-    auto F = [](int r) { return (4 - ((r >> 2) & 3)) & 3; };
-    const int srow = tid >> 2, sxc = (tid & 3) ^ F(srow);
+    int end = 0;
+    if (tid < BM) {
+        const int i = min(tid, live - 1), g = o.sid[m0 + i], row = o.perm[m0 + i];
+        end = o.start[g + 1];
+        sid[tid] = tid < live ? g : a.G;
+        rows[tid] = row;
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the LDS writes alone: `end` is on its way
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    // 16-byte chunk c of row r of a buffer lies at r * 8 + (c ^ (r & 7)): lanes that read one chunk of 16 rows hit all banks
+    const int srow = tid >> 3, sxc = (tid & 7) ^ (srow & 7);
     const char* ga[PA];
     const char* gb[PB];
 #pragma unroll
-    for (int i = 0; i < PA; ++i) ga[i] = a.A + perm[min(i * (NT / 4) + srow, live - 1)] * a.lda + sxc * 16 + (int64_t)k0 * 64;
+    for (int i = 0; i < PA; ++i) ga[i] = a.A + rows[i * (NT / 8) + srow] * a.lda + sxc * 16 + (int64_t)k0 * 128;
 #pragma unroll
-    for (int i = 0; i < PB; ++i) gb[i] = a.B + min(n0 + i * (NT / 4) + srow, a.N - 1) * a.ldb + sxc * 16 + (int64_t)k0 * 64;
+    for (int i = 0; i < PB; ++i) gb[i] = a.B + min(n0 + i * (NT / 8) + srow, a.N - 1) * a.ldb + sxc * 16 + (int64_t)k0 * 128;
     const uint32_t lds0 = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)reinterpret_cast<uintptr_t>(lds + 64 * w));
+    // Loads to LDS as inline asm: the compiler does not see what they write, so it puts no wait for all of them before an LDS
+    // read; the waits are below. No output register is involved; M0 holds the wave's destination.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"  // m0 is reserved: the clobber keeps the compiler's own uses safe
-    auto dma = [&](const char* g, uint32_t l) {
-        asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(l) : "memory", "m0");
+    auto to_lds = [&](const char* from, int chunk) {
+        asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(lds0 + (uint32_t)chunk * 16u) : "m0");
     };
 #pragma clang diagnostic pop
-    auto stage = [&](int kt) {
-        const uint32_t base = lds0 + (uint32_t)((kt % NS) * SZ) * 16u;
-#pragma unroll
-        for (int i = 0; i < PA; ++i) dma(ga[i] + (int64_t)kt * 64, base + i * NT * 16);
-#pragma unroll
-        for (int i = 0; i < PB; ++i) dma(gb[i] + (int64_t)kt * 64, base + (BM * 4 + i * NT) * 16);
+    auto load = [&](int kt, int i) {
+        const char* g = (i < PA ? ga[i < PA ? i : 0] : gb[i >= PA ? i - PA : 0]) + (int64_t)kt * 128;
+        to_lds(g, (kt & 1) * SZ + (i < PA ? i * NT : BM * 8 + (i - PA) * NT));
     };
-    // the wave's loads but the `younger` last steps' have landed, its LDS reads are in registers; then everyone's
-    auto wait = [&](int younger) {
-        if (younger >= 3) asm volatile("s_waitcnt vmcnt(12) lgkmcnt(0)" ::: "memory");
-        else if (younger == 2) asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)" ::: "memory");
-        else if (younger == 1) asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)" ::: "memory");
-        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-    };
-    static_assert(NS == 4, "the waits count up to three younger steps");
     const int ra = wm * MT * 16 + fr, rb = wn * NN * 16 + fr;
+    const int a0 = ra * 8 + (fq ^ (ra & 7)), a1 = ra * 8 + ((4 + fq) ^ (ra & 7));  // a lane's chunk of the two halves
+    const int b0 = BM * 8 + rb * 8 + (fq ^ (rb & 7)), b1 = BM * 8 + rb * 8 + ((4 + fq) ^ (rb & 7));
     uint4 fa[2][MT], fb[2][NN];
-    auto read = [&](int kt, uint4 (&xa)[MT], uint4 (&xb)[NN]) {
-        const uint4* sa = lds + (kt % NS) * SZ;
-        const uint4* sb = sa + BM * 4;
-#pragma unroll
-        for (int ni = 0; ni < NN; ++ni) xb[ni] = sb[(rb + ni * 16) * 4 + (fq ^ F(rb + ni * 16))];
-#pragma unroll
-        for (int mi = 0; mi < MT; ++mi) xa[mi] = sa[(ra + mi * 16) * 4 + (fq ^ F(ra + mi * 16))];
-    };
     f32x4 acc[MT][NN];
 #pragma unroll
     for (int mi = 0; mi < MT; ++mi)
 #pragma unroll
         for (int ni = 0; ni < NN; ++ni) acc[mi][ni] = f32x4{0.f, 0.f, 0.f, 0.f};
-    auto multiply = [&](const uint4 (&xa)[MT], const uint4 (&xb)[NN]) {
+    // x is multiplied while y is read (rd) from s and stage next (>= 0) starts to load; a row of tiles at a time, in this order
+    auto half = [&](uint4 (&xa)[MT], uint4 (&xb)[NN], uint4 (&ya)[MT], uint4 (&yb)[NN], const uint4* s, int oa, int ob, bool rd,
+                    int next) {
+        constexpr int RD = (MT + NN + MT - 1) / MT, LD = P / MT > 2 ? P / MT : 2;
 #pragma unroll
-        for (int mi = 0; mi < MT; ++mi)
+        for (int mi = 0; mi < MT; ++mi) {
+            if (rd)
+#pragma unroll
+                for (int r = mi * RD; r < (mi + 1) * RD; ++r) {
+                    if (r < NN) yb[r < NN ? r : 0] = s[ob + r * 128];
+                    else if (r < NN + MT) ya[r >= NN && r < NN + MT ? r - NN : 0] = s[oa + (r - NN) * 128];
+                }
+            if (next >= 0)
+#pragma unroll
+                for (int d = mi * LD; d < (mi + 1) * LD; ++d)
+                    if (d < P) load(next, d);
 #pragma unroll
             for (int ni = 0; ni < NN; ++ni) acc[mi][ni] = mma<T>(xb[ni], xa[mi], acc[mi][ni]);
-    };
-    for (int i = tid; i < BM; i += NT) sid[i] = i < live ? o.sid[m0 + i] : a.G;
-    for (int kt = 0; kt < NS && kt < steps; ++kt) stage(kt);
-    // step kt: its operands are in registers; step kt + 1 has landed, step kt + 4 takes the buffer of step kt
-    wait(steps - 1);
-    read(0, fa[0], fb[0]);
-    auto step = [&](int kt, uint4 (&xa)[MT], uint4 (&xb)[NN], uint4 (&ya)[MT], uint4 (&yb)[NN]) {
-        if (kt + 1 < steps) {
-            wait(min(2, steps - 2 - kt));
-            if (kt + NS < steps) stage(kt + NS);
-            read(kt + 1, ya, yb);
+            __builtin_amdgcn_sched_barrier(0);
         }
-        multiply(xa, xb);
     };
-    for (int kt = 0; kt < steps; kt += 2) {
-        step(kt, fa[0], fb[0], fa[1], fb[1]);
-        if (kt + 1 < steps) step(kt + 1, fa[1], fb[1], fa[0], fb[0]);
+    // KR ranks of an adapter, 64 bytes of each row's pieces and of each column of W: `fetch` starts the pieces to LDS (those of
+    // other adapters' rows come along and are not used) and W into registers, `place` turns it round into LDS. Two blocks lie in LDS,
+    // so the next is fetched while one is multiplied, and the first during the last half stage of the main loop.
+    constexpr int EW = BN * KR / NT, BLOCK = PARTS * BM * 4 + BN * 4, FP = PARTS * BM * 4 / NT;
+    static_assert(EW * (int)sizeof(T) == 32, "two chunks of W a thread");
+    const int wi = tid % BN, we = __builtin_amdgcn_readfirstlane(tid / BN * EW);
+    T wx[EW];
+    auto F = [](int r) { return (4 - ((r >> 2) & 3)) & 3; };  // chunk c of a row r of 64 bytes lies at r * 4 + (c ^ F(r)): all banks
+    const int rp = padded_rank(a.R, sizeof(T));
+    auto fetch = [&](int g, int r0, int buf) {
+#pragma unroll
+        for (int i = 0; i < FP; ++i) {
+            const int k = i * NT + tid, u = k / (BM * 4), r = (k >> 2) % BM, ch = (k & 3) ^ F(r);
+            to_lds(a.S + (((int64_t)rows[r] * pieces<T>() + u) * rp + r0) * (int)sizeof(T) + ch * 16, buf * BLOCK + i * NT);
+        }
+        const char* base = a.W + (int64_t)g * a.R * a.ldw + (int64_t)min(n0 + wi, a.N - 1) * (int)sizeof(T);
+#pragma unroll
+        for (int e = 0; e < EW; ++e) wx[e] = *reinterpret_cast<const T*>(base + min(r0 + we + e, a.R - 1) * a.ldw);
+    };
+    auto place = [&](int r0, int buf) {
+        uint4* sw = lds + buf * BLOCK + PARTS * BM * 4;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            constexpr int E = 16 / (int)sizeof(T);
+            T y[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) y[e] = r0 + we + k * E + e < a.R ? wx[k * E + e] : T(0);
+            uint4 z;
+            __builtin_memcpy(&z, y, 16);
+            sw[wi * 4 + ((we / E + k) ^ F(wi))] = z;
+        }
+    };
+    for (int kt = 0; kt < 2 && kt < steps; ++kt)
+#pragma unroll
+        for (int i = 0; i < P; ++i) load(kt, i);
+    if (tid < BM) ends[tid] = (int)min((int64_t)live, end - m0);
+    if (steps > 1) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");  // the first of the two stages
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int ni = 0; ni < NN; ++ni) fb[0][ni] = lds[b0 + ni * 128];
+#pragma unroll
+    for (int mi = 0; mi < MT; ++mi) fa[0][mi] = lds[a0 + mi * 128];
+    // in the middle of a stage: this wave's reads of it are in registers, the next one has landed; then so it is for every wave
+    auto meet = [&] {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    int kt = 0;
+    for (; kt + 1 < steps; ++kt) {
+        half(fa[0], fb[0], fa[1], fb[1], lds + (kt & 1) * SZ, a1, b1, true, -1);
+        meet();
+        half(fa[1], fb[1], fa[0], fb[0], lds + ((kt + 1) & 1) * SZ, a0, b0, true, kt + 2 < steps ? kt + 2 : -1);
     }
-    // the adapters of the tile's rows, one after the other (rows without one come last)
-    if (split == 0) {
-        uint4* st = lds;                      // PARTS x BM rows of 64 bytes of ranks
-        uint4* sw = lds + PARTS * BM * 4;      // BN columns of 64 bytes of ranks
-        for (int p0 = 0, p1; p0 < live; p0 = p1) {
-            const int g = __builtin_amdgcn_readfirstlane(sid[p0]);
-            if (g == a.G) break;
-            p1 = (int)min((int64_t)live, o.start[g + 1] - m0);
-            const float s = a.mul ? a.mul[g] : 1.f;
-            for (int r0 = 0; r0 < a.R; r0 += KR) {
-                __syncthreads();  // the ring, or the ranks before, have been read
-                constexpr int EH = BM * KR / NT, EW = BN * KR / NT;  // a thread's values of H and of W
-                static_assert(EH * (int)sizeof(T) == 32 && EW == EH, "two chunks of each");
-                {
-                    const int i = tid / (KR / EH), e0 = tid % (KR / EH) * EH;
-                    const bool has = i >= p0 && i < p1;
-                    const float* h = a.H + (int64_t)perm[has ? i : p0] * a.R + r0 + e0;
-                    float x[EH];
+    half(fa[0], fb[0], fa[1], fb[1], lds + (kt & 1) * SZ, a1, b1, true, -1);
+    meet();
+    const int first = __builtin_amdgcn_readfirstlane(sid[0]);
+    if (split == 0 && first < a.G) fetch(first, 0, 0);
+    half(fa[1], fb[1], fa[0], fb[0], lds, a0, b0, false, -1);
+    // 128 bytes of columns of the wave's rows at a time: written to LDS as the lanes hold them, read as rows
+    auto store = [&](auto* out, int64_t ldo, bool vec) {
+        using V = std::remove_pointer_t<decltype(out)>;
+        constexpr int E = 16 / (int)sizeof(V), NP = 128 / (int)sizeof(V) / 16;  // values of a chunk; tiles in 128 bytes
+        char* mine = reinterpret_cast<char*>(lds + w * MT * 16 * 8);
 #pragma unroll
-                    for (int e = 0; e < EH; ++e) x[e] = has && r0 + e0 + e < a.R ? h[e] * s : 0.f;
-                    const int at = i * 4, ch = e0 * (int)sizeof(T) / 16;
+        for (int n = 0; n < NN; n += NP) {
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const int to = at + ((ch + k) ^ F(i));
-                        if constexpr (sizeof(T) == 2) {
-                            uint32_t p[3][8];
+            for (int mi = 0; mi < MT; ++mi)
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) split3(x[k * 8 + e], p[0][e], p[1][e], p[2][e]);
-#pragma unroll
-                            for (int u = 0; u < 3; ++u)
-                                st[u * BM * 4 + to] = make_uint4(pack_high(p[u][0], p[u][1]), pack_high(p[u][2], p[u][3]),
-                                                                 pack_high(p[u][4], p[u][5]), pack_high(p[u][6], p[u][7]));
-                        } else {
-                            st[to] = make_uint4(__float_as_uint(x[k * 4]), __float_as_uint(x[k * 4 + 1]),
-                                                __float_as_uint(x[k * 4 + 2]), __float_as_uint(x[k * 4 + 3]));
-                        }
-                    }
+                for (int j = 0; j < NP; ++j) {
+                    const int r = mi * 16 + fr, at = j * 16 + 4 * fq;  // its first column
+                    put4(reinterpret_cast<V*>(mine + r * 128 + ((at / E) ^ (r & 7)) * 16) + at % E, acc[mi][n + j]);
                 }
-                {
-                    const int i = tid % BN, e0 = tid / BN * EW, col = min(n0 + i, a.N - 1);
-                    const char* base = a.W + ((int64_t)g * a.R + r0 + e0) * a.ldw + (int64_t)col * sizeof(T);
-                    T x[EW];
+            wave_sync();
+            const int c = n0 + wn * NN * 16 + n * 16 + (lane & 7) * E;
 #pragma unroll
-                    for (int e = 0; e < EW; ++e) x[e] = r0 + e0 + e < a.R ? *reinterpret_cast<const T*>(base + e * a.ldw) : T(0);
-                    const int ch = e0 * (int)sizeof(T) / 16;
+            for (int i = 0; i < MT * 2; ++i) {
+                const int r = i * 8 + (lane >> 3), row = wm * MT * 16 + r;
+                const uint4 x = *reinterpret_cast<const uint4*>(mine + r * 128 + ((lane & 7) ^ (r & 7)) * 16);
+                if (row >= live || c >= a.N) continue;
+                V* d = out + rows[row] * ldo + c;
+                if (vec && c + E <= a.N) {
+                    *reinterpret_cast<uint4*>(d) = x;
+                } else {
+                    V v[E];
+                    __builtin_memcpy(v, &x, 16);
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        uint4 y;
-                        __builtin_memcpy(&y, x + k * (16 / sizeof(T)), 16);
-                        sw[i * 4 + ((ch + k) ^ F(i))] = y;
-                    }
-                }
-                __syncthreads();
-#pragma unroll
-                for (int ni = 0; ni < NN; ++ni) fb[0][ni] = sw[(rb + ni * 16) * 4 + (fq ^ F(rb + ni * 16))];
-#pragma unroll
-                for (int mi = 0; mi < MT; ++mi) {
-                    const int r = ra + mi * 16;
-                    if (r - fr + 16 <= p0 || r - fr >= p1) continue;  // none of the 16 rows
-                    f32x4 x[NN];
-#pragma unroll
-                    for (int ni = 0; ni < NN; ++ni) x[ni] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int u = 0; u < PARTS; ++u) {
-                        const uint4 h = st[(u * BM + r) * 4 + (fq ^ F(r))];
-#pragma unroll
-                        for (int ni = 0; ni < NN; ++ni) x[ni] = mma<T>(fb[0][ni], h, x[ni]);
-                    }
-                    if (r >= p0 && r < p1)
-#pragma unroll
-                        for (int ni = 0; ni < NN; ++ni) acc[mi][ni] += x[ni];
+                    for (int e = 0; e < E; ++e)
+                        if (c + e < a.N) d[e] = v[e];
                 }
             }
+            wave_sync();
+        }
+    };
+    // the adapters of the tile's rows, one after the other (rows without one come last), KR ranks at a time
+    if (split == 0) {
+        int g = first, p0 = 0, p1 = __builtin_amdgcn_readfirstlane(ends[0]), r0 = 0, buf = 0;
+        while (g < a.G) {
+            place(r0, buf);
+            meet();  // this block has landed for every wave, and the one before has been read
+            int g1 = g, q0 = p0, q1 = p1, r1 = r0 + KR;
+            if (r1 >= a.R) {
+                r1 = 0, q0 = p1;
+                g1 = q0 < live ? __builtin_amdgcn_readfirstlane(sid[q0]) : a.G;
+                if (g1 < a.G) q1 = __builtin_amdgcn_readfirstlane(ends[q0]);
+            }
+            if (g1 < a.G) fetch(g1, r1, buf ^ 1);
+            const uint4* st = lds + buf * BLOCK;
+            const uint4* sw = st + PARTS * BM * 4;
+#pragma unroll
+            for (int ni = 0; ni < NN; ++ni) fb[0][ni] = sw[(rb + ni * 16) * 4 + (fq ^ F(rb + ni * 16))];
+#pragma unroll
+            for (int mi = 0; mi < MT; ++mi) {
+                const int r = ra + mi * 16;
+                if (r - fr + 16 <= p0 || r - fr >= p1) continue;  // none of the 16 rows
+                f32x4 x[NN];
+#pragma unroll
+                for (int ni = 0; ni < NN; ++ni) x[ni] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int u = 0; u < PARTS; ++u) {
+                    const uint4 h = st[(u * BM + r) * 4 + (fq ^ F(r))];
+#pragma unroll
+                    for (int ni = 0; ni < NN; ++ni) x[ni] = mma<T>(fb[0][ni], h, x[ni]);
+                }
+                if (r >= p0 && r < p1)
+#pragma unroll
+                    for (int ni = 0; ni < NN; ++ni) acc[mi][ni] += x[ni];
+            }
+            g = g1, p0 = q0, p1 = q1, r0 = r1, buf ^= 1;
         }
     }
     // lane: row ra + 16 mi, columns rb - fr + 16 ni + 4 fq + e
-    const bool partial = a.splits > 1;
-#pragma unroll
-    for (int mi = 0; mi < MT; ++mi) {
-        const int i = ra + mi * 16;
-        if (i >= live) continue;
-        const int64_t row = perm[i];
-#pragma unroll
-        for (int ni = 0; ni < NN; ++ni) {
-            const int c = n0 + rb - fr + ni * 16 + 4 * fq;
-            if (c >= a.N) continue;
-            if (partial) {
-                put4(a.part + ((int64_t)split * a.M + row) * a.N + c, acc[mi][ni], !(a.N & 3), a.N - c);
-            } else {
-                put4((O*)a.out + row * a.ldo + c, acc[mi][ni], a.vec, a.N - c);
-            }
-        }
-    }
+    __syncthreads();  // the buffers have been read by all
+    if (a.splits > 1) store(a.part + (int64_t)split * a.M * a.N, a.N, !(a.N & 3));
+    else store((O*)a.out, a.ldo, a.vec);
 }
 
 // the sum of a product's splits, in order
@@ -722,11 +797,11 @@ struct Plan {
     int64_t each;                                // else rows of a wave that counts
     int n_chunks;
     int64_t max_tiles, max_chunks, max_parts;
-    size_t perm, sid, start, tiles, chunks, tile0, chunk0, multi0, number, hist, hidden, t, part, bytes;
+    size_t perm, sid, start, tiles, chunks, tile0, chunk0, multi0, number, hist, pieces, t, part, bytes;
 };
 
 // split of a product over the contraction: enough blocks for 256 CUs with two each, where there are few tiles, as long as a split has
-// 16 steps (1 KB of a row)
+// 8 stages (1 KB of a row)
 struct Tiling {
     bool big;
     unsigned m_tiles, n_tiles, splits;
@@ -737,7 +812,7 @@ Tiling tiling(int64_t M, int64_t N, int64_t steps) {
     const int64_t b = t.big ? 256 : 128;
     t.m_tiles = (unsigned)((M + b - 1) / b), t.n_tiles = (unsigned)((N + b - 1) / b);
     const int64_t tiles = std::max<int64_t>(1, (int64_t)t.m_tiles * t.n_tiles);
-    t.splits = t.big || tiles >= 256 ? 1 : (unsigned)std::max<int64_t>(1, std::min<int64_t>({512 / tiles, steps / 16, 32}));
+    t.splits = t.big || tiles >= 256 ? 1 : (unsigned)std::max<int64_t>(1, std::min<int64_t>({512 / tiles, steps / 8, 32}));
     return t;
 }
 
@@ -772,16 +847,18 @@ Plan plan_for(int32_t dtype, int64_t n, int64_t m, int64_t p, int64_t G, int R, 
     l.tiles = take(16 * l.max_tiles), l.chunks = take(16 * l.max_chunks);
     l.tile0 = take(4 * (G + 1)), l.chunk0 = take(4 * (G + 1)), l.multi0 = take(4 * (G + 1)), l.number = take(8);
     l.hist = take((size_t)4 * l.n_chunks * (G + 1));
-    l.hidden = l.t = l.part = at;
+    l.t = l.part = at;
+    // the rows' factors, for the products that have an expand
+    const size_t factors = (size_t)n * (dtype == RP_BF16 ? 3 : 1) * padded_rank(R, es) * es;
+    l.pieces = take(what == RP_ADAPT_GRADIENTS ? 0 : factors);
     if (what == RP_ADAPT_PROJECT) {
-        l.hidden = take((size_t)4 * n * R);
-        const Tiling g = tiling(n, p, mk * es / 64);
+        const Tiling g = tiling(n, p, mk * es / 128);
         l.part = take(g.splits > 1 ? (size_t)4 * g.splits * n * p : 0);
     } else {
         l.t = take((size_t)4 * n * R);
         size_t part = (size_t)4 * l.max_parts * R * std::max(mk, pk);
         if (what == RP_ADAPT_GRADIENTS_DX) {
-            const Tiling g = tiling(n, m, pk * es / 64);
+            const Tiling g = tiling(n, m, pk * es / 128);
             if (g.splits > 1) part = std::max(part, (size_t)4 * g.splits * n * m);
         }
         l.part = take(part);
@@ -817,29 +894,22 @@ int launch_groups(const Plan& l, const Groups& o, const int32_t* ids, int64_t n,
     return RP_OK;
 }
 
-template <typename T, int RT, int KT, int NW>
-int launch_shrink_as(const Plan& l, const T* Z, int64_t ldz, int64_t kp, const T* W, int G, int R, const float* mul, const Groups& o,
-                     float* H, hipStream_t st) {
-    hipLaunchKernelGGL((shrink_kernel<T, RT, KT, NW>), dim3((unsigned)l.max_tiles), dim3(64 * NW), 0, st, Z, ldz, kp, W, G, R, mul, o, H);
+template <typename T>
+int launch_shrink(const Plan& l, const ShrinkArgs& a, const Groups& o, hipStream_t st) {
+    const dim3 grid((unsigned)l.max_tiles);
+    if (l.waves == 4) {
+        if (l.kt == 1) hipLaunchKernelGGL((shrink_kernel<T, 4, 1, 4>), grid, dim3(256), 0, st, a, o);
+        else if (l.kt == 2) hipLaunchKernelGGL((shrink_kernel<T, 4, 2, 4>), grid, dim3(256), 0, st, a, o);
+        else if (l.kt == 4) hipLaunchKernelGGL((shrink_kernel<T, 2, 4, 4>), grid, dim3(256), 0, st, a, o);
+        else hipLaunchKernelGGL((shrink_kernel<T, 1, 8, 4>), grid, dim3(256), 0, st, a, o);
+    } else {
+        if (l.kt == 1) hipLaunchKernelGGL((shrink_kernel<T, 1, 1, 8>), grid, dim3(512), 0, st, a, o);
+        else if (l.kt == 2) hipLaunchKernelGGL((shrink_kernel<T, 1, 2, 8>), grid, dim3(512), 0, st, a, o);
+        else if (l.kt == 4) hipLaunchKernelGGL((shrink_kernel<T, 1, 4, 8>), grid, dim3(512), 0, st, a, o);
+        else hipLaunchKernelGGL((shrink_kernel<T, 1, 8, 8>), grid, dim3(512), 0, st, a, o);
+    }
     HIP_TRY(hipGetLastError());
     return RP_OK;
-}
-
-template <typename T>
-int launch_shrink(const Plan& l, const T* Z, int64_t ldz, int64_t kp, const T* W, int G, int R, const float* mul, const Groups& o,
-                  float* H, hipStream_t st) {
-    if (l.waves == 4) switch (l.kt) {
-            case 1: return launch_shrink_as<T, 4, 1, 4>(l, Z, ldz, kp, W, G, R, mul, o, H, st);
-            case 2: return launch_shrink_as<T, 4, 2, 4>(l, Z, ldz, kp, W, G, R, mul, o, H, st);
-            case 4: return launch_shrink_as<T, 2, 4, 4>(l, Z, ldz, kp, W, G, R, mul, o, H, st);
-            default: return launch_shrink_as<T, 1, 8, 4>(l, Z, ldz, kp, W, G, R, mul, o, H, st);
-        }
-    switch (l.kt) {
-        case 1: return launch_shrink_as<T, 1, 1, 8>(l, Z, ldz, kp, W, G, R, mul, o, H, st);
-        case 2: return launch_shrink_as<T, 1, 2, 8>(l, Z, ldz, kp, W, G, R, mul, o, H, st);
-        case 4: return launch_shrink_as<T, 1, 4, 8>(l, Z, ldz, kp, W, G, R, mul, o, H, st);
-        default: return launch_shrink_as<T, 1, 8, 8>(l, Z, ldz, kp, W, G, R, mul, o, H, st);
-    }
 }
 
 template <typename T>
@@ -868,8 +938,8 @@ int launch_gemm(GemmArgs a, const Groups& o, hipStream_t st) {
     const uint64_t per = ((uint64_t)t.m_tiles * t.n_tiles * t.splits + 7) / 8;
     if (per * 8 >= (1ull << 31)) return fail(RP_ERR_UNSUPPORTED, "too many rows for one launch");
     a.per_xcd = (unsigned)per;
-    if (t.big) hipLaunchKernelGGL((gemm_kernel<T, O, 256, 256, 2, 4, 4>), dim3(a.per_xcd * 8), dim3(512), 0, st, a, o);
-    else hipLaunchKernelGGL((gemm_kernel<T, O, 128, 128, 2, 2, 4>), dim3(a.per_xcd * 8), dim3(256), 0, st, a, o);
+    if (t.big) hipLaunchKernelGGL((gemm_kernel<T, O, 256, 256, 2, 4>), dim3(a.per_xcd * 8), dim3(512), 0, st, a, o);
+    else hipLaunchKernelGGL((gemm_kernel<T, O, 128, 128, 2, 2>), dim3(a.per_xcd * 8), dim3(256), 0, st, a, o);
     HIP_TRY(hipGetLastError());
     if (t.splits > 1) {
         hipLaunchKernelGGL(gemm_join_kernel<O>, dim3((unsigned)((a.M * a.N + 255) / 256)), dim3(256), 0, st, a);
@@ -879,13 +949,13 @@ int launch_gemm(GemmArgs a, const Groups& o, hipStream_t st) {
 }
 
 template <typename T, typename O>
-GemmArgs gemm_args(const T* A, int64_t lda, const T* B, int64_t kp, int64_t M, int64_t N, O* out, int64_t ldo, const float* H,
-                   const float* mul, const T* W, int64_t wp, int G, int R, void* part) {
+GemmArgs gemm_args(const T* A, int64_t lda, const T* B, int64_t kp, int64_t M, int64_t N, O* out, int64_t ldo, const char* S,
+                   const T* W, int64_t wp, int G, int R, void* part) {
     GemmArgs a{};
     a.A = (const char*)A, a.B = (const char*)B, a.lda = lda * (int64_t)sizeof(T), a.ldb = kp * (int64_t)sizeof(T);
-    a.M = M, a.N = (int)N, a.steps = (int)(kp * (int64_t)sizeof(T) / 64), a.out = out, a.ldo = ldo;
-    a.vec = !((uintptr_t)out & (4 * sizeof(O) - 1)) && ldo % 4 == 0;
-    a.H = H, a.mul = mul, a.W = (const char*)W, a.ldw = wp * (int64_t)sizeof(T), a.G = G, a.R = R, a.part = (float*)part;
+    a.M = M, a.N = (int)N, a.steps = (int)(kp * (int64_t)sizeof(T) / 128), a.out = out, a.ldo = ldo;
+    a.vec = !((uintptr_t)out & 15) && ldo * sizeof(O) % 16 == 0;
+    a.S = S, a.W = (const char*)W, a.ldw = wp * (int64_t)sizeof(T), a.G = G, a.R = R, a.part = (float*)part;
     return a;
 }
 
@@ -896,10 +966,9 @@ int project(const T* X, int64_t ldx, int64_t n, int64_t m, const T* C, int64_t p
     const int64_t mk = padded(m, dt), pk = padded(p, dt);
     const Plan l = plan_for(dt, n, m, p, G, R, RP_ADAPT_PROJECT);
     const Groups o = groups_of(l, ws);
-    if (!hidden) hidden = (float*)(ws + l.hidden);
     int rc = launch_groups(l, o, ids, n, G, st);
-    if (!rc) rc = launch_shrink<T>(l, X, ldx, mk, down, G, R, nullptr, o, hidden, st);
-    if (!rc) rc = launch_gemm<T, float>(gemm_args<T, float>(X, ldx, C, mk, n, p, Y, ldy, hidden, scale, up, pk, G, R, ws + l.part), o, st);
+    if (!rc) rc = launch_shrink<T>(l, ShrinkArgs{X, ldx, mk, down, G, R, scale, hidden, 0, ws + l.pieces}, o, st);
+    if (!rc) rc = launch_gemm<T, float>(gemm_args<T, float>(X, ldx, C, mk, n, p, Y, ldy, ws + l.pieces, up, pk, G, R, ws + l.part), o, st);
     return rc;
 }
 
@@ -921,11 +990,11 @@ int gradients(const T* dY, int64_t lddy, const T* X, int64_t ldx, int64_t n, int
     const Groups o = groups_of(l, ws);
     float* t = (float*)(ws + l.t);
     int rc = launch_groups(l, o, ids, n, G, st);
-    if (!rc && n) rc = launch_shrink<T>(l, dY, lddy, pk, up, G, R, scale, o, t, st);
+    if (!rc && n) rc = launch_shrink<T>(l, ShrinkArgs{dY, lddy, pk, up, G, R, scale, t, 1, dX ? ws + l.pieces : nullptr}, o, st);
     if (!rc) rc = launch_outer<T>(l, outer_args<T>(X, ldx, mk, m, R, nullptr, t, d_down, ldd, sdd, ws + l.part), o, G, st);
     if (!rc) rc = launch_outer<T>(l, outer_args<T>(dY, lddy, pk, p, R, scale, hidden, d_up, ldu, sdu, ws + l.part), o, G, st);
     if (!rc && dX && n)
-        rc = launch_gemm<T, T>(gemm_args<T, T>(dY, lddy, Ct, pk, n, m, dX, lddx, t, nullptr, down, mk, G, R, ws + l.part), o, st);
+        rc = launch_gemm<T, T>(gemm_args<T, T>(dY, lddy, Ct, pk, n, m, dX, lddx, ws + l.pieces, down, mk, G, R, ws + l.part), o, st);
     return rc;
 }
 

@@ -109,10 +109,11 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t x) {
     return x;
 }
 
-__device__ __forceinline__ uint16_t to_bf16(float x) {  // to nearest even; a NaN stays one
-    const uint32_t u = __float_as_uint(x);
-    if ((u & 0x7fffffffu) > 0x7f800000u) return (uint16_t)((u >> 16) | 0x40u);
-    return (uint16_t)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
+// rounded to nearest even, two at a time (one instruction); a NaN stays one
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t to_bf16(float a, float b) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
 }
 
 struct StepArgs {
@@ -182,13 +183,12 @@ __global__ void __launch_bounds__(256) adamw_step_kernel(StepArgs a) {
         if (ts.vec && left >= 4) {
             *reinterpret_cast<float4*>(ts.w + at) = make_float4(w[0], w[1], w[2], w[3]);
             if (ts.copy)
-                *reinterpret_cast<uint2*>(ts.copy + at) = make_uint2(to_bf16(w[0]) | (uint32_t)to_bf16(w[1]) << 16,
-                                                                     to_bf16(w[2]) | (uint32_t)to_bf16(w[3]) << 16);
+                *reinterpret_cast<uint2*>(ts.copy + at) = make_uint2(to_bf16(w[0], w[1]), to_bf16(w[2], w[3]));
         } else {
             for (int k = 0; k < 4; ++k)
                 if (k < left) {
                     ts.w[at + k] = w[k];
-                    if (ts.copy) ts.copy[at + k] = to_bf16(w[k]);
+                    if (ts.copy) ts.copy[at + k] = (uint16_t)to_bf16(w[k], 0.f);
                 }
         }
         if constexpr (BITS == 32) {

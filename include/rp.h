@@ -334,8 +334,9 @@ int rp_dense_project_device(int device, const void* X, int32_t dtype, int64_t n,
  *   hidden_i = down[a] x_i,   y_i = C x_i + scale[a] up[a]^T hidden_i
  * dtype RP_BF16 or RP_F32 is the type of X, C, down and up; products are exact and summed in f32, Y
  * and hidden are f32. With s = 64 (bf16) or 32 (f32), mk and pk are m and p rounded up to a multiple
- * of s: X is n x mk (row stride ldx), C p x mk, down adapters x rank x mk, up adapters x rank x pk, zeros
- * in the columns past m or p, all device arrays with 16-byte aligned rows. rank <= 128 (an adapter of
+ * of s: C is p x mk, down adapters x rank x mk, up adapters x rank x pk, zeros in the columns past m or p,
+ * 16-byte aligned. X is n x m with row stride ldx; its rows are 16-byte aligned where m is a multiple of s, and
+ * are copied to padded ones in the workspace where it is not. rank <= 128 (an adapter of
  * a smaller rank is padded with zero rows), adapters <= 16383. scale: device f32, one for each
  * adapter, or NULL (1). Y: n x p, row stride ldy. hidden: n x rank (contiguous, zeros for rows without
  * an adapter) or NULL when the backward pass is not wanted. workspace: rp_adapt_workspace_bytes bytes,
@@ -352,7 +353,7 @@ int rp_adapt_project_device(int device, const void* X, int64_t ldx, int32_t dtyp
                             int64_t p, const void* down, const void* up, int64_t adapters, int32_t rank,
                             const float* scale, const int32_t* ids, float* Y, int64_t ldy, float* hidden,
                             void* workspace, int64_t workspace_bytes, void* stream);
-/* Its backward pass: from dY (n x pk, row stride lddy) and the forward pass's hidden,
+/* Its backward pass: from dY (n x p, row stride lddy, aligned as X is) and the forward pass's hidden,
  *   t_i = scale[a] up[a] dy_i,   dX = dY C + down[a]^T t_i (in dtype, n x m, row stride lddx)
  *   d_down[g] = sum of t_i x_i^T,   d_up[g] = scale[g] sum of hidden_i dy_i^T   (over g's rows; f32)
  * Ct is C transposed (m x pk, zeros past p); with Ct and dX NULL the rows' gradient is left out. d_down

@@ -15,7 +15,9 @@ and Y, hidden and the banks' gradients are float32 (no reference counterpart; cs
 """
 from __future__ import annotations
 
-import ctypes
+import functools
+
+import torch
 
 from . import _native as nat
 from .gaussian import _STEP
@@ -24,21 +26,24 @@ __all__ = ["adapted_project_device", "adapted_project_backward_device", "prepare
 
 MAX_RANK, MAX_ADAPTERS = 128, 16383
 _CODE = {"bf16": nat.RP_BF16, "fp32": nat.RP_F32}
+_TYPE = {"bf16": torch.bfloat16, "fp32": torch.float32}
 
 
 def _dtype(compute):
-    import torch
+    try:
+        return _TYPE[compute]
+    except KeyError:
+        raise ValueError("compute must be 'fp32' or 'bf16'") from None
 
-    if compute not in _CODE:
-        raise ValueError("compute must be 'fp32' or 'bf16'")
-    return torch.bfloat16 if compute == "bf16" else torch.float32
+
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(code, n, m, p, G, R, what):
+    return nat.load().rp_adapt_workspace_bytes(code, n, m, p, G, R, what)
 
 
 def prepare_bank(W, compute: str):
     """W cast to the compute type, contiguous, its last axis padded with zeros to the kernels' multiple: what
     ``prepared=True`` expects of C, Ct, down and up. Returned as it is where it is all that already."""
-    import torch
-
     W = W.to(_dtype(compute))
     pad = -W.shape[-1] % _STEP[compute]
     if pad:
@@ -48,11 +53,15 @@ def prepare_bank(W, compute: str):
 
 
 def _rows(X, compute):
-    """X as the kernels read it: a row stride of its own where rows are aligned and need no padding, else a copy."""
-    if (X.dtype == _dtype(compute) and X.shape[1] % _STEP[compute] == 0 and X.stride(1) == 1 and X.data_ptr() % 16 == 0
-            and X.stride(0) * X.element_size() % 16 == 0 and (X.stride(0) >= X.shape[1] or X.shape[0] <= 1)):
-        return X
-    return prepare_bank(X, compute)
+    """X as the library takes it: of the compute type, with a row stride of its own, rows aligned unless their width needs
+    padding (the library copies them then); else a copy."""
+    if X.dtype is _TYPE[compute]:
+        row, one = X.stride()
+        if one == 1 and (row >= X.shape[1] or X.shape[0] <= 1) and (
+                X.shape[1] % _STEP[compute] or (X.data_ptr() % 16 == 0 and row * X.element_size() % 16 == 0)):
+            return X
+    X = X.to(_TYPE[compute]).contiguous()
+    return X if X.data_ptr() % 16 == 0 else X.clone()
 
 
 def _ld(X):
@@ -63,39 +72,37 @@ def _operand(name, W, shape, compute, prepared):
     """``shape``: the expected sizes, the last one before padding."""
     if prepared:
         want = (*shape[:-1], shape[-1] + -shape[-1] % _STEP[compute])
-        if tuple(W.shape) != want or W.dtype != _dtype(compute) or not W.is_contiguous() or W.data_ptr() % 16:
+        if W.shape != want or W.dtype is not _TYPE[compute] or not W.is_contiguous() or W.data_ptr() % 16:
             raise ValueError(f"prepared {name} must be a contiguous 16-byte aligned {_dtype(compute)} tensor of shape "
                              f"{want}, got {W.dtype} {tuple(W.shape)}")
         return W
-    if tuple(W.shape) != tuple(shape):
-        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(W.shape)}")
+    if W.shape != shape:
+        raise ValueError(f"{name} must have shape {shape}, got {tuple(W.shape)}")
     return prepare_bank(W, compute)
 
 
 def _check_common(X, down, up, ids, scale, compute):
-    import torch
-
     _dtype(compute)
     if X.dim() != 2 or down.dim() != 3 or up.dim() != 3:
         raise ValueError("X must be 2-D, down and up 3-D (adapters, rank, width)")
-    if down.shape[:2] != up.shape[:2] or 0 in down.shape:
+    (n, m), (G, R, _), (G2, R2, _) = X.shape, down.shape, up.shape
+    if G != G2 or R != R2 or not G or not R or not m:
         raise ValueError(f"down {tuple(down.shape)} and up {tuple(up.shape)} must have the same, positive, number of "
                          "adapters and rank")
-    if down.shape[1] > MAX_RANK or down.shape[0] > MAX_ADAPTERS:
-        raise ValueError(f"at most {MAX_ADAPTERS} adapters of rank {MAX_RANK}, got {down.shape[0]} of rank {down.shape[1]}")
-    if ids.dtype != torch.int32 or tuple(ids.shape) != (X.shape[0],) or not ids.is_contiguous():
-        raise ValueError(f"ids must be a contiguous int32 tensor of {X.shape[0]} entries, got {ids.dtype} {tuple(ids.shape)}")
-    if scale is not None and (scale.dtype != torch.float32 or tuple(scale.shape) != (down.shape[0],)
-                              or not scale.is_contiguous()):
+    if R > MAX_RANK or G > MAX_ADAPTERS:
+        raise ValueError(f"at most {MAX_ADAPTERS} adapters of rank {MAX_RANK}, got {G} of rank {R}")
+    if ids.dtype is not torch.int32 or ids.shape != (n,) or not ids.is_contiguous():
+        raise ValueError(f"ids must be a contiguous int32 tensor of {n} entries, got {ids.dtype} {tuple(ids.shape)}")
+    if scale is not None and (scale.dtype is not torch.float32 or scale.shape != (G,) or not scale.is_contiguous()):
         raise ValueError("scale must be a contiguous float32 tensor with one entry for each adapter")
+    return n, m, G, R
 
 
 def _check_device(*tensors):
-    import torch
-
     dev = tensors[0].device
-    if any(t is not None and t.device != dev for t in tensors):
-        raise ValueError("all tensors must be on one device")
+    for t in tensors:
+        if t is not None and t.device != dev:
+            raise ValueError("all tensors must be on one device")
     if dev.type != "cuda":
         raise RuntimeError("adapted projections need an MI355X (no CPU fallback)")
     return dev, torch.cuda.current_stream(dev)
@@ -104,8 +111,6 @@ def _check_device(*tensors):
 def _on_stream(stream, cur, tensors):
     """The stream to launch on. One other than torch's current stream waits for what is queued there (casts and pads
     of the operands), and the temporaries made here are kept for it."""
-    import torch
-
     if stream is None or stream == cur.cuda_stream:
         return cur.cuda_stream
     ext = torch.cuda.ExternalStream(stream, device=cur.device)
@@ -121,7 +126,7 @@ def _ptr(t):
 
 
 def _strided(name, t, shape, dtype):
-    if t.dtype != dtype or tuple(t.shape) != shape or t.stride(-1) != 1 or any(
+    if t.dtype is not dtype or t.shape != shape or t.stride(-1) != 1 or any(
             t.stride(d) < t.stride(d + 1) * t.shape[d + 1] for d in range(t.dim() - 1)):
         raise ValueError(f"{name} must be a {dtype} tensor of shape {shape} with unit column stride and rows that do not overlap")
     return t
@@ -134,11 +139,7 @@ def adapted_project_device(X, C, down, up, ids, *, scale=None, out=None, compute
     that the backward pass takes. ``prepared``: C, down and up already went through ``prepare_bank`` for this compute
     mode. ``out``: a float32 n x p tensor with unit column stride to write to. Runs on ``stream`` (a raw handle;
     default: torch's current stream), without synchronising; it can be captured into a graph."""
-    import torch
-
-    _check_common(X, down, up, ids, scale, compute)
-    n, m = X.shape
-    G, R = down.shape[:2]
+    n, m, G, R = _check_common(X, down, up, ids, scale, compute)
     if C.dim() != 2:
         raise ValueError("C must be 2-D")
     p = C.shape[0]
@@ -153,7 +154,7 @@ def adapted_project_device(X, C, down, up, ids, *, scale=None, out=None, compute
     hidden = torch.empty(n, R, dtype=torch.float32, device=dev) if return_hidden else None
     if n:
         lib, code = nat.load(), _CODE[compute]
-        need = lib.rp_adapt_workspace_bytes(code, n, m, p, G, R, nat.RP_ADAPT_PROJECT)
+        need = _workspace_bytes(code, n, m, p, G, R, nat.RP_ADAPT_PROJECT)
         ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
         st = _on_stream(stream, cur, (Xc, Cc, Dc, Uc, ids, scale, y, hidden, ws))
         nat.check(lib.rp_adapt_project_device(
@@ -169,15 +170,11 @@ def adapted_project_backward_device(dY, X, Ct, down, up, ids, hidden, *, scale=N
     d_down (G x R x m) and d_up (G x R x p) are float32, zeros for adapters without rows; ``out``: a pair of such
     tensors (unit column stride) to write them to. ``prepared``: Ct, down and up went through ``prepare_bank``.
     The same call gives the same bits. Runs on ``stream`` as the forward pass does."""
-    import torch
-
-    _check_common(X, down, up, ids, scale, compute)
-    n, m = X.shape
-    G, R = down.shape[:2]
+    n, m, G, R = _check_common(X, down, up, ids, scale, compute)
     if dY.dim() != 2 or dY.shape[0] != n or 0 in dY.shape[1:]:
         raise ValueError(f"dY must be 2-D with {n} rows, got {tuple(dY.shape)}")
     p = dY.shape[1]
-    if hidden.dtype != torch.float32 or tuple(hidden.shape) != (n, R) or not hidden.is_contiguous():
+    if hidden.dtype is not torch.float32 or hidden.shape != (n, R) or not hidden.is_contiguous():
         raise ValueError(f"hidden must be the contiguous float32 ({n}, {R}) tensor of the forward pass")
     Tc = None if Ct is None else _operand("Ct", Ct, (m, p), compute, prepared)
     Dc = _operand("down", down, (G, R, m), compute, prepared)
@@ -192,7 +189,7 @@ def adapted_project_backward_device(dY, X, Ct, down, up, ids, hidden, *, scale=N
     dX = None if Ct is None else torch.empty(n, m, dtype=_dtype(compute), device=dev)
     lib, code = nat.load(), _CODE[compute]
     what = nat.RP_ADAPT_GRADIENTS if dX is None else nat.RP_ADAPT_GRADIENTS_DX
-    need = lib.rp_adapt_workspace_bytes(code, n, m, p, G, R, what)
+    need = _workspace_bytes(code, n, m, p, G, R, what)
     ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
     st = _on_stream(stream, cur, (Xc, Yc, Tc, Dc, Uc, ids, hidden, scale, dX, d_down, d_up, ws))
     row = lambda t: max(t.stride(1), t.shape[2])  # noqa: E731

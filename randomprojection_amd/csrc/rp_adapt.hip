@@ -20,6 +20,7 @@ using namespace rpd;
 
 namespace {
 
+constexpr int kSmallRows = 4096;  // rows that one block groups
 constexpr int kMaxRank = 128, kMaxAdapters = 16383;  // a wave's counts of all groups fit 64 KB of LDS
 
 // rounded to nearest even, two at a time (one instruction); a NaN stays one
@@ -40,7 +41,7 @@ struct Groups {
     int32_t* sid;     // sorted position -> group (0 .. G)
     int32_t* start;   // group -> first sorted position; G + 2 entries
     int4* tiles;      // {group, first sorted position, rows, 0}: at most tile_rows rows of one group (G included)
-    int4* chunks;     // {group, first sorted position, rows, its partial sums' number or -1}: at most chunk_rows rows, group < G
+    int4* chunks;     // {group, first sorted position, rows, its partial sums' number or -1}: at most chunk_rows rows (none where the group has none), group < G
     int32_t* tile0;   // group -> its first tile; G + 1 entries
     int32_t* chunk0;  // group -> its first chunk; G + 1 entries
     int32_t* multi0;  // group -> the first of its partial sums, where it has more than one chunk; G + 1 entries
@@ -100,34 +101,36 @@ __device__ __forceinline__ void place_rows(const int32_t* __restrict__ ids, int6
 }
 
 // exclusive prefix sum over the block's threads; total: of all of them
-__device__ __forceinline__ int block_scan(int x, int* sums, int& total) {
+template <typename I>
+__device__ __forceinline__ I block_scan(I x, uint64_t* sums, I& total) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, nw = blockDim.x >> 6;
-    int s = x;
+    I s = x;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(s, o);
+        const I y = __shfl_up(s, o);
         if (lane >= o) s += y;
     }
     __syncthreads();
-    if (lane == 63) sums[w] = s;
+    if (lane == 63) sums[w] = (uint64_t)s;
     __syncthreads();
-    int before = 0;
+    I before = 0;
     total = 0;
     for (int k = 0; k < nw; ++k) {
-        if (k < w) before += sums[k];
-        total += sums[k];
+        const I y = (I)sums[k];
+        if (k < w) before += y;
+        total += y;
     }
     return before + s - x;
 }
 
 // one block: from each group's first position (first(g), g <= G + 1) its tiles and chunks
 template <typename F>
-__device__ __forceinline__ void list_groups(const F& first, int G, int tile_rows, int chunk_rows, int* sums, const Groups& o) {
+__device__ __forceinline__ void list_groups(const F& first, int G, int tile_rows, int chunk_rows, uint64_t* sums, const Groups& o) {
     int t0 = 0, c0 = 0, p0 = 0;
     for (int base = 0; base <= G; base += blockDim.x) {
         const int g = base + threadIdx.x;
         const int s = g <= G ? first(g) : 0, rows = g <= G ? first(g + 1) - s : 0;
-        const int nt = (rows + tile_rows - 1) / tile_rows, nc = g < G ? (rows + chunk_rows - 1) / chunk_rows : 0;
+        const int nt = (rows + tile_rows - 1) / tile_rows, nc = g < G ? max(1, (rows + chunk_rows - 1) / chunk_rows) : 0;
         int tt, tc, tp;
         const int t = t0 + block_scan(nt, sums, tt), c = c0 + block_scan(nc, sums, tc);
         const int p = p0 + block_scan(nc > 1 ? nc : 0, sums, tp);
@@ -143,7 +146,7 @@ __device__ __forceinline__ void list_groups(const F& first, int G, int tile_rows
     if (threadIdx.x == 0) o.number[0] = t0, o.number[1] = c0;
     __syncthreads();
     for (int g = threadIdx.x >> 6; g <= G; g += blockDim.x >> 6) {  // a wave a group
-        const int s = o.start[g], rows = o.start[g + 1] - s, nc = g < G ? (rows + chunk_rows - 1) / chunk_rows : 0;
+        const int s = o.start[g], rows = o.start[g + 1] - s, nc = g < G ? max(1, (rows + chunk_rows - 1) / chunk_rows) : 0;
         for (int k = threadIdx.x & 63; k * tile_rows < rows; k += 64)
             o.tiles[o.tile0[g] + k] = make_int4(g, s + k * tile_rows, min(tile_rows, rows - k * tile_rows), 0);
         for (int k = threadIdx.x & 63; k < nc; k += 64)
@@ -152,40 +155,107 @@ __device__ __forceinline__ void list_groups(const F& first, int G, int tile_rows
     }
 }
 
-// few rows: one block does it all, its waves' counts in LDS as cnt[wave][group]
+// Rows whose width is no multiple of the kernels' step, copied to rows that are, zeros behind: block `block` of `blocks`
+struct Pad {
+    const void* from;
+    void* to;  // or NULL: nothing to do
+    int64_t ld, rows;
+    int width, padded, size;  // size: bytes of an element
+};
+__device__ __forceinline__ void pad_rows(const Pad& p, int64_t block, int64_t blocks) {
+    if (!p.to) return;
+    const int each = p.padded <= 256 ? 64 : p.padded <= 1024 ? 256 : blockDim.x;  // threads of a row
+    const int per = blockDim.x / each, lane = threadIdx.x % each;
+    for (int64_t r = block * per + threadIdx.x / each; r < p.rows; r += blocks * per) {
+        if (p.size == 2) {
+            const uint16_t* from = (const uint16_t*)p.from + r * p.ld;
+            uint16_t* to = (uint16_t*)p.to + r * p.padded;
+#pragma unroll 4
+            for (int c = lane; c < p.padded; c += each) to[c] = c < p.width ? from[c] : (uint16_t)0;
+        } else {
+            const float* from = (const float*)p.from + r * p.ld;
+            float* to = (float*)p.to + r * p.padded;
+#pragma unroll 4
+            for (int c = lane; c < p.padded; c += each) to[c] = c < p.width ? from[c] : 0.f;
+        }
+    }
+}
+__global__ void __launch_bounds__(256) pad_kernel(Pad p, Pad q) {
+    pad_rows(p, blockIdx.x, gridDim.x);
+    pad_rows(q, blockIdx.x, gridDim.x);
+}
+
+// few rows: one block does it all, its waves' counts in LDS as cnt[wave][group]; other blocks pad rows meanwhile
 __global__ void __launch_bounds__(1024)
-group_small_kernel(const int32_t* __restrict__ ids, int n, int G, int bits, int tile_rows, int chunk_rows, Groups o) {
+group_small_kernel(const int32_t* __restrict__ ids, int n, int G, int bits, int tile_rows, int chunk_rows, Groups o, Pad p, Pad q) {
     extern __shared__ int32_t lds_groups[];
-    __shared__ int sums[16];
-    int32_t* cnt = lds_groups;           // 16 x (G + 1)
-    int32_t* first = cnt + 16 * (G + 1);  // G + 2
-    const int tid = threadIdx.x, w = tid >> 6;
-    for (int i = tid; i < 16 * (G + 1); i += 1024) cnt[i] = 0;
+    __shared__ uint64_t sums[16];
+    if (blockIdx.x) {
+        pad_rows(p, blockIdx.x - 1, gridDim.x - 1);
+        pad_rows(q, blockIdx.x - 1, gridDim.x - 1);
+        return;
+    }
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, nt = blockDim.x, nw = nt >> 6;
+    int32_t* cnt = lds_groups;             // nw x (G + 1): the wave's rows of a group, then the first of them
+    int32_t* first = cnt + nw * (G + 1);   // G + 2, and G + 1 each of the lists' first entries
+    int32_t *tile0 = first + G + 2, *chunk0 = tile0 + G + 1, *multi0 = chunk0 + G + 1;
+    for (int i = tid; i < nw * (G + 1); i += nt) cnt[i] = 0;
+    const int each = (n + nt - 1) / nt * 64, r0 = w * each;
+    int g[kSmallRows / 1024], at[kSmallRows / 1024];  // the lane's rows' groups, and their places among the wave's rows of these
+#pragma unroll
+    for (int k = 0; k < kSmallRows / 1024; ++k) g[k] = k * 64 < each && r0 + k * 64 + lane < n ? group_of(ids[r0 + k * 64 + lane], G) : -1;
     __syncthreads();
-    const int each = (n + 1023) / 1024 * 64, r0 = min(n, w * each), r1 = min(n, r0 + each);
-    count_rows(ids, r0, r1, G, bits, cnt + w * (G + 1));
+#pragma unroll
+    for (int k = 0; k < kSmallRows / 1024; ++k) {
+        if (k * 64 >= each) break;
+        const uint64_t m = same_lanes(max(g[k], 0), g[k] >= 0, bits);
+        const int before = g[k] >= 0 ? cnt[w * (G + 1) + g[k]] : 0;
+        at[k] = before + __popcll(m & ((1ull << lane) - 1));
+        wave_sync();  // every lane has read the count before its first lane moves it
+        if (g[k] >= 0 && __ffsll((unsigned long long)m) - 1 == lane) cnt[w * (G + 1) + g[k]] = before + __popcll(m);
+        wave_sync();
+    }
     __syncthreads();
-    int at = 0;
-    for (int base = 0; base <= G; base += 1024) {
-        const int g = base + tid;
+    int row0 = 0;
+    uint64_t list0 = 0;  // tiles, chunks and partial sums so far, 21 bits each
+    for (int base = 0; base <= G; base += nt) {
+        const int h = base + tid;
         int rows = 0, total;
-        if (g <= G)
-            for (int k = 0; k < 16; ++k) rows += cnt[k * (G + 1) + g];
-        int s = at + block_scan(rows, sums, total);
-        if (g <= G) {
-            first[g] = s;
-            if (g == G) first[G + 1] = s + rows;
-            for (int k = 0; k < 16; ++k) {
-                const int c = cnt[k * (G + 1) + g];
-                cnt[k * (G + 1) + g] = s;
+        if (h <= G)
+            for (int k = 0; k < nw; ++k) rows += cnt[k * (G + 1) + h];
+        int s = row0 + block_scan(rows, sums, total);
+        const int nt_ = (rows + tile_rows - 1) / tile_rows, nc = h < G ? max(1, (rows + chunk_rows - 1) / chunk_rows) : 0;
+        const uint64_t lists = h <= G ? (uint64_t)nt_ | (uint64_t)nc << 21 | (uint64_t)(nc > 1 ? nc : 0) << 42 : 0;
+        uint64_t all;
+        const uint64_t l = list0 + block_scan(lists, sums, all);
+        if (h <= G) {
+            first[h] = o.start[h] = s;
+            tile0[h] = (int)(l & 0x1fffff), chunk0[h] = (int)(l >> 21 & 0x1fffff), multi0[h] = o.multi0[h] = (int)(l >> 42);
+            if (h == G) first[G + 1] = o.start[G + 1] = n;
+            for (int k = 0; k < nw; ++k) {
+                const int c = cnt[k * (G + 1) + h];
+                cnt[k * (G + 1) + h] = s;
                 s += c;
             }
         }
-        at += total;
+        row0 += total, list0 += all;
     }
+    if (tid == 0) o.number[0] = (int)(list0 & 0x1fffff), o.number[1] = (int)(list0 >> 21 & 0x1fffff);
     __syncthreads();
-    place_rows(ids, r0, r1, G, bits, cnt + w * (G + 1), o);
-    list_groups([&](int g) { return first[g]; }, G, tile_rows, chunk_rows, sums, o);
+#pragma unroll
+    for (int k = 0; k < kSmallRows / 1024; ++k)
+        if (k * 64 < each && g[k] >= 0) {
+            const int to = cnt[w * (G + 1) + g[k]] + at[k];
+            o.perm[to] = r0 + k * 64 + lane;
+            o.sid[to] = g[k];
+        }
+    for (int h = w; h <= G; h += nw) {  // a wave a group
+        const int s = first[h], rows = first[h + 1] - s, nc = h < G ? max(1, (rows + chunk_rows - 1) / chunk_rows) : 0;
+        for (int k = lane; k * tile_rows < rows; k += 64)
+            o.tiles[tile0[h] + k] = make_int4(h, s + k * tile_rows, min(tile_rows, rows - k * tile_rows), 0);
+        for (int k = lane; k < nc; k += 64)
+            o.chunks[chunk0[h] + k] = make_int4(h, s + k * chunk_rows, min(chunk_rows, rows - k * chunk_rows), nc > 1 ? multi0[h] + k : -1);
+    }
 }
 
 // many rows: counts of each wave's rows (4 waves a block) to hist[group][chunk]
@@ -204,7 +274,7 @@ group_count_kernel(const int32_t* __restrict__ ids, int64_t n, int G, int bits, 
 
 // one block: exclusive prefix sums of hist in its order, a run of entries a thread, and the lists
 __global__ void __launch_bounds__(1024) group_scan_kernel(int64_t n, int G, int n_chunks, int tile_rows, int chunk_rows, Groups o) {
-    __shared__ int sums[16];
+    __shared__ uint64_t sums[16];
     const int64_t all = (int64_t)(G + 1) * n_chunks, each = (all + 1023) / 1024;
     const int64_t i0 = min(all, threadIdx.x * each), i1 = min(all, i0 + each);
     int s = 0, total;
@@ -284,22 +354,58 @@ struct ShrinkArgs {
     float* H;            // or NULL; n x R
     int scaled;          // H takes the scale too
     void* S;             // or NULL; n x pieces x padded rank
+    f32x4* part;
 };
 
+// a lane's four ranks of one row of a tile (place i of the tile's 16 x 16 sums, KT of them along the ranks) to H and to the pieces
+template <typename T, int KT>
+__device__ __forceinline__ void shrink_finish(const ShrinkArgs& a, const Groups& o, int4 tile, int i, f32x4 x) {
+    const int R = a.R, rp = padded_rank(R, sizeof(T));
+    const int l = i & 63, row = i / (64 * KT) * 16 + (l & 15), r = (i >> 6) % KT * 16 + 4 * (l >> 4);
+    if (row >= tile.z) return;
+    const int64_t to = o.perm[tile.y + row];
+    f32x4 y = x * (a.scale ? a.scale[tile.x] : 1.f);
+    if (a.H) {
+        float* h = a.H + to * R + r;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (r + e < R) h[e] = a.scaled ? y[e] : x[e];
+    }
+    if (!a.S || r >= rp) return;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (r + e >= R) y[e] = 0.f;
+    if constexpr (sizeof(T) == 2) {
+        uint32_t v[3][4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) split3(y[e], v[0][e], v[1][e], v[2][e]);
+        uint16_t* d = (uint16_t*)a.S + to * 3 * rp + r;
+#pragma unroll
+        for (int u = 0; u < 3; ++u) {
+            *reinterpret_cast<uint2*>(d + u * rp) = make_uint2(pack_high(v[u][0], v[u][1]), pack_high(v[u][2], v[u][3]));
+            if (KT == 1) *reinterpret_cast<uint2*>(d + u * rp + 16) = make_uint2(0, 0);  // ranks 16 .. 31
+        }
+    } else {
+        *reinterpret_cast<f32x4*>((float*)a.S + to * rp + r) = y;
+    }
+}
+
 // H[i][r] = (scaled ? scale[a] : 1) sum_q Z[i][q] W[a][r][q], zeros for rows without an adapter, and its pieces. A block takes a tile
-// of 16 RT rows of one group; its NW waves split the contraction and add up in LDS in their order. Bound by
-// reading Z once: the wave holds 16 RT x 16 KT of H, so W (from L2) is read once for 16 RT rows, and there is
-// nothing between the loads and the matrix instructions.
-template <typename T, int RT, int KT, int NW>
-__global__ void __launch_bounds__(64 * NW)
+// of 16 RT rows of one group; its four waves split the contraction and add up in LDS in their order. Bound by reading Z once where
+// there are many rows: the wave holds 16 RT x 16 KT of H, so W (from L2) is read once for 16 RT rows, and there is nothing between
+// the loads and the matrix instructions (65536 x 16384 by rank 16 in bf16: 0.39 ms, 5.5 TB/s). Where there are few, by how much of
+// its row a compute unit can take in: the contraction is then split over the grid too, and shrink_join_kernel adds up.
+template <typename T, int RT, int KT>
+__global__ void __launch_bounds__(256)
 shrink_kernel(ShrinkArgs a, Groups o) {
+    constexpr int NW = 4;
     __shared__ f32x4 red[NW][RT * KT][64];
     if ((int)blockIdx.x >= o.number[0]) return;
     const int4 tile = o.tiles[blockIdx.x];
     const int g = tile.x, pos = tile.y, rows = tile.z, R = a.R;
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, c = lane & 15, q = lane >> 4;
     if (g == a.G) {
-        if (a.H)
+        if (a.H && blockIdx.y == 0)
             for (int i = tid; i < rows * R; i += 64 * NW) a.H[(int64_t)o.perm[pos + i / R] * R + i % R] = 0.f;
         return;
     }
@@ -319,9 +425,10 @@ shrink_kernel(ShrinkArgs a, Groups o) {
     for (int t = 0; t < RT; ++t)
 #pragma unroll
         for (int j = 0; j < KT; ++j) acc[t][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const int64_t lines = kp * (int64_t)sizeof(T) / 128, each = (lines + NW - 1) / NW;  // 128 bytes of a row: two steps
-    const int64_t l1 = min(lines, (w + 1) * each);
-    for (int64_t l = w * each; l < l1; ++l) {
+    const int64_t lines = kp * (int64_t)sizeof(T) / 128;  // 128 bytes of a row: two steps
+    const int64_t s0 = lines * blockIdx.y / gridDim.y, s1 = lines * (blockIdx.y + 1) / gridDim.y, each = (s1 - s0 + NW - 1) / NW;
+    const int64_t l1 = min(s1, s0 + (w + 1) * each);
+    for (int64_t l = s0 + w * each; l < l1; ++l) {
         uint4 zf[2][RT], bf[2][KT];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -342,46 +449,32 @@ shrink_kernel(ShrinkArgs a, Groups o) {
 #pragma unroll
         for (int j = 0; j < KT; ++j) red[w][t * KT + j][lane] = acc[t][j];
     __syncthreads();
-    const float s = a.scale ? a.scale[g] : 1.f;
-    const int rp = padded_rank(R, sizeof(T));
     for (int i = tid; i < RT * KT * 64; i += 64 * NW) {
         const f32x4* p = &red[0][0][0] + i;
         f32x4 x = p[0];
 #pragma unroll
         for (int k = 1; k < NW; ++k) x += p[k * RT * KT * 64];
-        const int l = i & 63, row = i / (64 * KT) * 16 + (l & 15), r = (i >> 6) % KT * 16 + 4 * (l >> 4);
-        if (row >= rows) continue;
-        const int64_t at = o.perm[pos + row];
-        f32x4 y = x * s;
-        if (a.H) {
-            float* h = a.H + at * R + r;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (r + e < R) h[e] = a.scaled ? y[e] : x[e];
-        }
-        if (!a.S || r >= rp) continue;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (r + e >= R) y[e] = 0.f;
-        if constexpr (sizeof(T) == 2) {
-            uint32_t v[3][4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) split3(y[e], v[0][e], v[1][e], v[2][e]);
-            uint16_t* d = (uint16_t*)a.S + at * 3 * rp + r;
-#pragma unroll
-            for (int u = 0; u < 3; ++u) {
-                *reinterpret_cast<uint2*>(d + u * rp) = make_uint2(pack_high(v[u][0], v[u][1]), pack_high(v[u][2], v[u][3]));
-                if (KT == 1) *reinterpret_cast<uint2*>(d + u * rp + 16) = make_uint2(0, 0);  // ranks 16 .. 31
-            }
-        } else {
-            *reinterpret_cast<f32x4*>((float*)a.S + at * rp + r) = y;
-        }
+        if (gridDim.y == 1) shrink_finish<T, KT>(a, o, tile, i, x);
+        else a.part[((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * (RT * KT * 64) + i] = x;
     }
 }
 
-// D[g][r][c] (+ partial sums) = (mul ? mul[g] : 1) sum over rows i of adapter g of H[i][r] Z[i][c]. A wave takes 16 KT
-// ranks by 128 (bf16) or 64 (f32) columns over a chunk of one group's rows, its lanes reading 16 bytes of
-// neighbouring columns of each row: no LDS for Z, which is read once (per 16 KT ranks) and bounds the kernel.
+// the splits' sums of tiles of 16 rows, in order
+template <typename T, int KT>
+__global__ void __launch_bounds__(64 * KT) shrink_join_kernel(ShrinkArgs a, Groups o, int splits) {
+    if ((int)blockIdx.x >= o.number[0]) return;
+    const int4 tile = o.tiles[blockIdx.x];
+    if (tile.x == a.G) return;
+    const int i = threadIdx.x;
+    f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+    for (int k = 0; k < splits; ++k) x += a.part[((int64_t)k * gridDim.x + blockIdx.x) * (KT * 64) + i];
+    shrink_finish<T, KT>(a, o, tile, i, x);
+}
+
+// D[g][r][c] (+ partial sums) = (mul ? mul[g] : 1) sum over rows i of adapter g of H[i][r] Z[i][c]. A block takes 16
+// KT ranks by 128 (bf16) or 64 (f32) columns over a chunk of one group's rows, a wave every fourth step of them, its lanes
+// reading 16 bytes of neighbouring columns of each row: no LDS for Z, which is read once (per 16 KT ranks) and bounds the kernel.
 //   bf16: 32 rows a step, lane (c, q) rows 8 q .. 8 q + 7, columns 8 c .. 8 c + 7: 8 x 8 values turned round in
 //         registers (a byte permutation for two values), so column j of every lane is one matrix operand. H is split exactly
 //         into three bf16.
@@ -400,41 +493,49 @@ struct OuterArgs {
 constexpr int kMaxChunk = 2048;
 
 template <typename T, int KT>
-__global__ void __launch_bounds__(256) outer_kernel(OuterArgs a, Groups o) {
+__global__ void __launch_bounds__(256, KT == 1 ? 4 : 2) outer_kernel(OuterArgs a0, OuterArgs a1, int blocks0, int blocks, Groups o) {
     constexpr int NC = sizeof(T) == 2 ? 8 : 4;  // columns of a lane
+    constexpr int RS = sizeof(T) == 2 ? 8 : 4;  // rows of a lane in a step of 4 RS rows
     __shared__ int32_t list[kMaxChunk];
-    if ((int)blockIdx.x >= o.number[1]) return;
-    const int4 chunk = o.chunks[blockIdx.x];
+    __shared__ float red[4][NC][64][4];
+    const int which = blockIdx.x / blocks, block = blockIdx.x % blocks;
+    if (which >= o.number[1]) return;
+    const bool second = block >= blocks0;  // both banks' gradients in one launch
+    const OuterArgs& a = second ? a1 : a0;
+    const int4 chunk = o.chunks[which];
     const int g = chunk.x, rows = chunk.z;
     for (int i = threadIdx.x; i < rows; i += 256) list[i] = o.perm[chunk.y + i];
     __syncthreads();
-    const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
-    const int64_t col = ((int64_t)blockIdx.y * 4 + (threadIdx.x >> 6)) * (16 * NC) + c * NC;
-    if (col - c * NC >= a.q) return;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = lane & 15, q = lane >> 4;
+    const int64_t col0 = (int64_t)(block - (second ? blocks0 : 0)) * (16 * NC), col = col0 + c * NC;
     const T* __restrict__ Z = (const T*)a.Z + min(col, a.qp - NC);
-    const int r0 = blockIdx.z * 16 * KT;
+    const float* __restrict__ H = a.H;
+    const int64_t ldz = a.ldz;
+    const int r0 = blockIdx.z * 16 * KT, R = a.R;
     f32x4 acc[KT][NC];
 #pragma unroll
     for (int k = 0; k < KT; ++k)
 #pragma unroll
         for (int j = 0; j < NC; ++j) acc[k][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    constexpr int RS = sizeof(T) == 2 ? 8 : 4;  // rows of a lane in a step of 4 RS rows
-    for (int i0 = 0; i0 < rows; i0 += 4 * RS) {
-        uint4 z[RS];
-        float h[KT][RS];
+    auto load = [&](int i0, uint4 (&z)[RS], float (&h)[KT][RS]) {
 #pragma unroll
         for (int j = 0; j < RS; ++j) {
             const int i = i0 + (sizeof(T) == 2 ? q * RS + j : j * 4 + q);
-            const bool in = i < rows;
-            const int64_t row = list[in ? i : rows - 1];
-            z[j] = *reinterpret_cast<const uint4*>(Z + row * a.ldz);
+            const int64_t row = list[min(i, rows - 1)];
+            z[j] = *reinterpret_cast<const uint4*>(Z + row * ldz);
 #pragma unroll
-            for (int k = 0; k < KT; ++k) {
-                const int r = r0 + k * 16 + c;
-                h[k][j] = a.H[row * a.R + min(r, a.R - 1)];
-                if (!in) h[k][j] = 0.f;
-            }
-            if (!in) z[j] = make_uint4(0, 0, 0, 0);
+            for (int k = 0; k < KT; ++k) h[k][j] = H[row * R + min(r0 + k * 16 + c, R - 1)];
+        }
+    };
+    auto add = [&](int i0, uint4 (&z)[RS], float (&h)[KT][RS]) {
+        if (i0 + 4 * RS > rows) {  // what lies behind the last row counts nothing, whatever it is
+#pragma unroll
+            for (int j = 0; j < RS; ++j)
+                if (i0 + (sizeof(T) == 2 ? q * RS + j : j * 4 + q) >= rows) {
+                    z[j] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+                    for (int k = 0; k < KT; ++k) h[k][j] = 0.f;
+                }
         }
         if constexpr (sizeof(T) == 2) {
             uint4 hp[KT][3];
@@ -468,35 +569,57 @@ __global__ void __launch_bounds__(256) outer_kernel(OuterArgs a, Groups o) {
                     for (int k = 0; k < KT; ++k) acc[k][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(h[k][i], v, acc[k][j], 0, 0, 0);
                 }
         }
+    };
+    if (rows) {
+        uint4 z[RS];
+        float h[KT][RS];
+        for (int i0 = w * 4 * RS; i0 < rows; i0 += 16 * RS) {
+            load(i0, z, h);
+            add(i0, z, h);
+        }
     }
-    const float s = a.mul ? a.mul[g] : 1.f;
-    float* out = chunk.w >= 0 ? a.part + (int64_t)chunk.w * a.R * a.qp : a.D + g * a.sdd;
+    const float s = a.mul && rows ? a.mul[g] : 1.f;
+    float* out = chunk.w >= 0 ? a.part + (int64_t)chunk.w * R * a.qp : a.D + g * a.sdd;
     const int64_t ld = chunk.w >= 0 ? a.qp : a.ldd;
+    // the four waves' sums, in order, 16 ranks at a time; a thread then has four neighbouring columns of a rank
 #pragma unroll
-    for (int k = 0; k < KT; ++k)
+    for (int k = 0; k < KT; ++k) {
+        if (k) __syncthreads();
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int r = r0 + k * 16 + 4 * q + e;
-            if (r >= a.R) continue;
-            float* d = out + r * ld + col;
-            if (a.vec && col + NC <= a.q) {
+        for (int j = 0; j < NC; ++j) *reinterpret_cast<f32x4*>(red[w][j][lane]) = acc[k][j];
+        __syncthreads();
 #pragma unroll
-                for (int j = 0; j < NC; j += 4)
-                    *reinterpret_cast<f32x4*>(d + j) = f32x4{acc[k][j][e], acc[k][j + 1][e], acc[k][j + 2][e], acc[k][j + 3][e]} * s;
+        for (int i = threadIdx.x; i < 16 * 4 * NC; i += 256) {
+            const int quad = i % (4 * NC), rank = i / (4 * NC), r = r0 + k * 16 + rank, j0 = quad * 4 % NC;
+            const int from = (rank >> 2) * 16 + quad * 4 / NC;
+            const int64_t at = col0 + quad * 4;
+            if (r >= R || at >= a.q) continue;
+            f32x4 x;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                x[e] = (red[0][j0 + e][from][rank & 3] + red[1][j0 + e][from][rank & 3] + red[2][j0 + e][from][rank & 3] +
+                        red[3][j0 + e][from][rank & 3]) * s;
+            float* d = out + r * ld + at;
+            if (a.vec && at + 4 <= a.q) {
+                *reinterpret_cast<f32x4*>(d) = x;
             } else {
 #pragma unroll
-                for (int j = 0; j < NC; ++j)
-                    if (col + j < a.q) d[j] = acc[k][j][e] * s;
+                for (int e = 0; e < 4; ++e)
+                    if (at + e < a.q) d[e] = x[e];
             }
         }
+    }
 }
 
-// Adapters whose rows were cut into chunks: the partial sums in order; adapters without rows: zeros.
-__global__ void __launch_bounds__(256) outer_join_kernel(OuterArgs a, Groups o, int chunk_rows) {
-    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+// adapters whose rows were cut into chunks: the partial sums in order
+__global__ void __launch_bounds__(256) outer_join_kernel(OuterArgs a0, OuterArgs a1, int blocks0, Groups o, int chunk_rows) {
     const int g = blockIdx.z, r = blockIdx.y;
     const int rows = o.start[g + 1] - o.start[g], nc = (rows + chunk_rows - 1) / chunk_rows;
-    if (nc == 1 || c >= a.q) return;
+    if (nc <= 1) return;
+    const bool second = (int)blockIdx.x >= blocks0;
+    const OuterArgs& a = second ? a1 : a0;
+    const int64_t c = (int64_t)(blockIdx.x - (second ? blocks0 : 0)) * 256 + threadIdx.x;
+    if (c >= a.q) return;
     float s = 0.f;
     const float* p = a.part + ((int64_t)o.multi0[g] * a.R + r) * a.qp + c;
     for (int k = 0; k < nc; ++k) s += p[(int64_t)k * a.R * a.qp];
@@ -506,13 +629,16 @@ __global__ void __launch_bounds__(256) outer_join_kernel(OuterArgs a, Groups o, 
 // ------------------------------------------------------------------------------------------
 // The shared product with the adapters' expand: O[i][c] = sum_k A[i][k] B[c][k] + sum_r (scale[a] H[i][r]) W[a][r][c].
 //
-// BM x BN tiles, WM x WN waves; rows are taken in the order of the adapters (gathered by the loads, scattered by the
-// stores, at no cost), so few tiles hold more than one or two. The main loop stages 128 bytes of every row of A and B
-// at a time into two LDS buffers by loads that go to LDS directly. Whole lines: with 64 bytes a stage every line crossed
-// from L2 twice (its other half had left the L1 by the next stage): 1.10 against 1.25 to 1.31 PFLOP/s at 65536 x 16384 ->
-// 1024. A stage is multiplied in two halves, each half's operands read into registers during the half before; in the middle all
-// waves meet once, the other buffer having landed, and the stage after the next starts into this one.
-// After it the pieces of the rows' H (exact in three bf16) and the adapter's W take the buffers' place, 64 bytes of ranks
+// B x B tiles, WM x WN waves; rows are taken in the order of the adapters (gathered by the loads, scattered by the
+// stores, at no cost), so few tiles hold more than one or two. The main loop stages 128 bytes of every row of A and of B
+// at a time by loads that go to LDS directly. Whole lines: with 64 bytes a stage every line crossed from L2 twice (its other
+// half had left the L1 by the next stage): 1.10 against 1.25 PFLOP/s at 65536 x 16384 -> 1024. A stage is multiplied in two
+// halves, each half's operands read into registers during the half before; in the middle all waves meet once, the next stage
+// having landed. LDS is five slots of one operand's stage, taken in turn (A, B, A, B, ..): when a stage has been read, B of the stage
+// after the next and A of the one behind that start into its slots, so A, which comes from HBM, is two stages ahead, and all
+// 160 KB are used (two whole stages of each: 1.28 against 1.38 PFLOP/s; a third would not fit). A thread's loads are spread over
+// the half's matrix instructions.
+// After the loop the pieces of the rows' H (exact in three bf16) and the adapter's W take the slots' place, 64 bytes of ranks
 // at a time, and are multiplied into registers of their own, from where only the adapter's rows are added: a value that is
 // not finite in one adapter reaches no other's rows. The result goes through LDS so that rows are stored 128 bytes at a
 // time (16 rows a store otherwise: 0.58 against 0.53 ms at 16384 x 1024 -> 16384 with bf16 out).
@@ -532,21 +658,21 @@ struct GemmArgs {
     float* part;  // splits > 1: partial sums, splits x M x N
 };
 
-template <typename T, typename O, int BM, int BN, int WM, int WN>
+template <typename T, typename O, int BM, int WM, int WN>
 __global__ void __launch_bounds__(64 * WM * WN, 2)
 gemm_kernel(GemmArgs a, Groups o) {
-    constexpr int NT = 64 * WM * WN, MT = BM / WM / 16, NN = BN / WN / 16, SZ = (BM + BN) * 8;
-    constexpr int PA = BM * 8 / NT, PB = BN * 8 / NT, P = PA + PB;  // loads of a thread in a stage
+    constexpr int BN = BM, NT = 64 * WM * WN, MT = BM / WM / 16, NN = BN / WN / 16, SL = BM * 8;  // SL: chunks of a slot
+    constexpr int PL = BM * 8 / NT;  // loads of a thread for one operand's stage
     // hi, mid and low of H; a result in bf16 does without low (2^-17 of H, against a rounding of 2^-9)
     constexpr int PARTS = sizeof(T) == 4 ? 1 : sizeof(O) == 4 ? 3 : 2, KR = 64 / (int)sizeof(T);
-    static_assert(NT >= BM, "a row a thread");
-    static_assert(P == 8, "the first wait below counts eight loads a stage");
-    static_assert(2 * (PARTS * BM * 4 + BN * 4) <= 2 * SZ, "adapters take the buffers' place");
-    static_assert(WM * WN * MT * 16 * 8 <= 2 * SZ && NN == 4, "so do the stores, 64 columns a wave");
-    __shared__ uint4 lds[2 * SZ + BM * 3 / 4];
-    int32_t* sid = reinterpret_cast<int32_t*>(lds + 2 * SZ);  // the tile's rows' groups
-    int32_t* rows = sid + BM;                                 // where they are
-    int32_t* ends = rows + BM;                                // where in the tile their group ends
+    static_assert(PL == 4, "the waits below count four loads an operand");
+    static_assert(2 * (PARTS * BM * 4 + BN * 4) <= 4 * SL, "adapters take four slots' place");
+    static_assert(WM * WN * MT * 16 * 8 <= 4 * SL && NN == 4, "so do the stores, 64 columns a wave");
+    static_assert(NT >= BM && BM * 3 <= SL * 4, "a row a thread; the fifth slot holds the tables");
+    __shared__ uint4 lds[5 * SL];
+    int32_t* sid = reinterpret_cast<int32_t*>(lds + 4 * SL);  // after the main loop: the tile's rows' groups,
+    int32_t* rows = sid + BM;                                 // where they are,
+    int32_t* ends = rows + BM;                                // and where in the tile their group ends
     // XCD x (block i runs on XCD i % 8) takes a run of tiles; tiles go down 8 row tiles, then along the columns, so the
     // tiles that run at the same time on an XCD share their rows of A and of B in its L2
     const unsigned tiles = a.m_tiles * a.n_tiles, id = (blockIdx.x & 7u) * a.per_xcd + (blockIdx.x >> 3);
@@ -557,24 +683,16 @@ gemm_kernel(GemmArgs a, Groups o) {
     const int n0 = (int)nt * BN, live = (int)min((int64_t)BM, a.M - m0);
     const int k0 = (int)((int64_t)a.steps * split / a.splits), steps = (int)((int64_t)a.steps * (split + 1) / a.splits) - k0;
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, wm = w / WN, wn = w % WN, fr = lane & 15, fq = lane >> 4;
-    int end = 0;
-    if (tid < BM) {
-        const int i = min(tid, live - 1), g = o.sid[m0 + i], row = o.perm[m0 + i];
-        end = o.start[g + 1];
-        sid[tid] = tid < live ? g : a.G;
-        rows[tid] = row;
-    }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the LDS writes alone: `end` is on its way
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    // 16-byte chunk c of row r of a buffer lies at r * 8 + (c ^ (r & 7)): lanes that read one chunk of 16 rows hit all banks
+    const int32_t* __restrict__ perm = o.perm + m0;
+    const int first = o.sid[m0], first_end = (int)min((int64_t)live, o.start[first + 1] - m0);
+    // 16-byte chunk c of row r of a slot lies at r * 8 + (c ^ (r & 7)): lanes that read one chunk of 16 rows hit all banks
     const int srow = tid >> 3, sxc = (tid & 7) ^ (srow & 7);
-    const char* ga[PA];
-    const char* gb[PB];
+    const char* ga[PL];
+    const char* gb[PL];
 #pragma unroll
-    for (int i = 0; i < PA; ++i) ga[i] = a.A + rows[i * (NT / 8) + srow] * a.lda + sxc * 16 + (int64_t)k0 * 128;
+    for (int i = 0; i < PL; ++i) ga[i] = a.A + perm[min(i * (NT / 8) + srow, live - 1)] * a.lda + sxc * 16 + (int64_t)k0 * 128;
 #pragma unroll
-    for (int i = 0; i < PB; ++i) gb[i] = a.B + min(n0 + i * (NT / 8) + srow, a.N - 1) * a.ldb + sxc * 16 + (int64_t)k0 * 128;
+    for (int i = 0; i < PL; ++i) gb[i] = a.B + min(n0 + i * (NT / 8) + srow, a.N - 1) * a.ldb + sxc * 16 + (int64_t)k0 * 128;
     const uint32_t lds0 = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)reinterpret_cast<uintptr_t>(lds + 64 * w));
     // Loads to LDS as inline asm: the compiler does not see what they write, so it puts no wait for all of them before an LDS
     // read; the waits are below. No output register is involved; M0 holds the wave's destination.
@@ -584,35 +702,36 @@ gemm_kernel(GemmArgs a, Groups o) {
         asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(lds0 + (uint32_t)chunk * 16u) : "m0");
     };
 #pragma clang diagnostic pop
-    auto load = [&](int kt, int i) {
-        const char* g = (i < PA ? ga[i < PA ? i : 0] : gb[i >= PA ? i - PA : 0]) + (int64_t)kt * 128;
-        to_lds(g, (kt & 1) * SZ + (i < PA ? i * NT : BM * 8 + (i - PA) * NT));
-    };
+    auto load_a = [&](int kt, int i, int slot) { to_lds(ga[i] + (int64_t)kt * 128, slot * SL + i * NT); };
+    auto load_b = [&](int kt, int i, int slot) { to_lds(gb[i] + (int64_t)kt * 128, slot * SL + i * NT); };
     const int ra = wm * MT * 16 + fr, rb = wn * NN * 16 + fr;
     const int a0 = ra * 8 + (fq ^ (ra & 7)), a1 = ra * 8 + ((4 + fq) ^ (ra & 7));  // a lane's chunk of the two halves
-    const int b0 = BM * 8 + rb * 8 + (fq ^ (rb & 7)), b1 = BM * 8 + rb * 8 + ((4 + fq) ^ (rb & 7));
+    const int b0 = rb * 8 + (fq ^ (rb & 7)), b1 = rb * 8 + ((4 + fq) ^ (rb & 7));
     uint4 fa[2][MT], fb[2][NN];
     f32x4 acc[MT][NN];
 #pragma unroll
     for (int mi = 0; mi < MT; ++mi)
 #pragma unroll
         for (int ni = 0; ni < NN; ++ni) acc[mi][ni] = f32x4{0.f, 0.f, 0.f, 0.f};
-    // x is multiplied while y is read (rd) from s and stage next (>= 0) starts to load; a row of tiles at a time, in this order
-    auto half = [&](uint4 (&xa)[MT], uint4 (&xb)[NN], uint4 (&ya)[MT], uint4 (&yb)[NN], const uint4* s, int oa, int ob, bool rd,
-                    int next) {
-        constexpr int RD = (MT + NN + MT - 1) / MT, LD = P / MT > 2 ? P / MT : 2;
+    // x is multiplied while y is read (rd) from pa and pb, and B of stage next (>= 0) starts into slot sb, A of the stage behind it
+    // into slot sa; a row of tiles at a time, in this order
+    auto half = [&](uint4 (&xa)[MT], uint4 (&xb)[NN], uint4 (&ya)[MT], uint4 (&yb)[NN], const uint4* pa, const uint4* pb, bool rd,
+                    int next, int sb, int sa) {
+        constexpr int RD = (MT + NN + MT - 1) / MT, LD = 2 * PL / MT;
 #pragma unroll
         for (int mi = 0; mi < MT; ++mi) {
             if (rd)
 #pragma unroll
                 for (int r = mi * RD; r < (mi + 1) * RD; ++r) {
-                    if (r < NN) yb[r < NN ? r : 0] = s[ob + r * 128];
-                    else if (r < NN + MT) ya[r >= NN && r < NN + MT ? r - NN : 0] = s[oa + (r - NN) * 128];
+                    if (r < NN) yb[r < NN ? r : 0] = pb[r * 128];
+                    else if (r < NN + MT) ya[r >= NN && r < NN + MT ? r - NN : 0] = pa[(r - NN) * 128];
                 }
             if (next >= 0)
 #pragma unroll
-                for (int d = mi * LD; d < (mi + 1) * LD; ++d)
-                    if (d < P) load(next, d);
+                for (int d = mi * LD; d < (mi + 1) * LD; ++d) {
+                    if (d < PL) load_b(next, d < PL ? d : 0, sb);
+                    else if (next + 1 < steps) load_a(next + 1, d >= PL ? d - PL : 0, sa);
+                }
 #pragma unroll
             for (int ni = 0; ni < NN; ++ni) acc[mi][ni] = mma<T>(xb[ni], xa[mi], acc[mi][ni]);
             __builtin_amdgcn_sched_barrier(0);
@@ -627,11 +746,11 @@ gemm_kernel(GemmArgs a, Groups o) {
     T wx[EW];
     auto F = [](int r) { return (4 - ((r >> 2) & 3)) & 3; };  // chunk c of a row r of 64 bytes lies at r * 4 + (c ^ F(r)): all banks
     const int rp = padded_rank(a.R, sizeof(T));
-    auto fetch = [&](int g, int r0, int buf) {
+    auto fetch = [&](int g, int r0, int buf, auto row_of) {
 #pragma unroll
         for (int i = 0; i < FP; ++i) {
             const int k = i * NT + tid, u = k / (BM * 4), r = (k >> 2) % BM, ch = (k & 3) ^ F(r);
-            to_lds(a.S + (((int64_t)rows[r] * pieces<T>() + u) * rp + r0) * (int)sizeof(T) + ch * 16, buf * BLOCK + i * NT);
+            to_lds(a.S + (((int64_t)row_of(r) * pieces<T>() + u) * rp + r0) * (int)sizeof(T) + ch * 16, buf * BLOCK + i * NT);
         }
         const char* base = a.W + (int64_t)g * a.R * a.ldw + (int64_t)min(n0 + wi, a.N - 1) * (int)sizeof(T);
 #pragma unroll
@@ -650,35 +769,54 @@ gemm_kernel(GemmArgs a, Groups o) {
             sw[wi * 4 + ((we / E + k) ^ F(wi))] = z;
         }
     };
-    for (int kt = 0; kt < 2 && kt < steps; ++kt)
 #pragma unroll
-        for (int i = 0; i < P; ++i) load(kt, i);
-    if (tid < BM) ends[tid] = (int)min((int64_t)live, end - m0);
-    if (steps > 1) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");  // the first of the two stages
+    for (int i = 0; i < PL; ++i) load_a(0, i, 0);
+#pragma unroll
+    for (int i = 0; i < PL; ++i) load_b(0, i, 1);
+    if (steps > 1) {
+#pragma unroll
+        for (int i = 0; i < PL; ++i) load_a(1, i, 2);
+#pragma unroll
+        for (int i = 0; i < PL; ++i) load_b(1, i, 3);
+    }
+    if (steps > 2)
+#pragma unroll
+        for (int i = 0; i < PL; ++i) load_a(2, i, 4);
+    if (steps > 2) asm volatile("s_waitcnt vmcnt(12)" ::: "memory");  // the first stage
+    else if (steps > 1) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
     else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 #pragma unroll
-    for (int ni = 0; ni < NN; ++ni) fb[0][ni] = lds[b0 + ni * 128];
+    for (int ni = 0; ni < NN; ++ni) fb[0][ni] = lds[SL + b0 + ni * 128];
 #pragma unroll
     for (int mi = 0; mi < MT; ++mi) fa[0][mi] = lds[a0 + mi * 128];
-    // in the middle of a stage: this wave's reads of it are in registers, the next one has landed; then so it is for every wave
-    auto meet = [&] {
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    // in the middle of a stage: this wave's reads of it are in registers, the next one has landed (of what it has started, A of
+    // the stage behind that may still be on its way); then so it is for every wave
+    auto meet = [&](bool more) {
+        if (more) asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)" ::: "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
-    int kt = 0;
+    int kt = 0, sa = 0, sb = 1;  // slots of stage kt
     for (; kt + 1 < steps; ++kt) {
-        half(fa[0], fb[0], fa[1], fb[1], lds + (kt & 1) * SZ, a1, b1, true, -1);
-        meet();
-        half(fa[1], fb[1], fa[0], fb[0], lds + ((kt + 1) & 1) * SZ, a0, b0, true, kt + 2 < steps ? kt + 2 : -1);
+        const int na = sb == 4 ? 0 : sb + 1, nb = na == 4 ? 0 : na + 1;
+        half(fa[0], fb[0], fa[1], fb[1], lds + sa * SL + a1, lds + sb * SL + b1, true, -1, 0, 0);
+        meet(kt + 2 < steps);
+        half(fa[1], fb[1], fa[0], fb[0], lds + na * SL + a0, lds + nb * SL + b0, true, kt + 2 < steps ? kt + 2 : -1, sa, sb);
+        sa = na, sb = nb;
     }
-    half(fa[0], fb[0], fa[1], fb[1], lds + (kt & 1) * SZ, a1, b1, true, -1);
-    meet();
-    const int first = __builtin_amdgcn_readfirstlane(sid[0]);
-    if (split == 0 && first < a.G) fetch(first, 0, 0);
-    half(fa[1], fb[1], fa[0], fb[0], lds, a0, b0, false, -1);
+    half(fa[0], fb[0], fa[1], fb[1], lds + sa * SL + a1, lds + sb * SL + b1, true, -1, 0, 0);
+    meet(false);
+    if (tid < BM) {
+        const int i = min(tid, live - 1), g = o.sid[m0 + i];
+        sid[tid] = tid < live ? g : a.G;
+        rows[tid] = perm[i];
+        ends[tid] = (int)min((int64_t)live, o.start[g + 1] - m0);
+    }
+    if (split == 0 && first < a.G) fetch(first, 0, 0, [&](int r) { return perm[min(r, live - 1)]; });
+    half(fa[1], fb[1], fa[0], fb[0], lds, lds, false, -1, 0, 0);
     // 128 bytes of columns of the wave's rows at a time: written to LDS as the lanes hold them, read as rows
     auto store = [&](auto* out, int64_t ldo, bool vec) {
         using V = std::remove_pointer_t<decltype(out)>;
@@ -716,17 +854,17 @@ gemm_kernel(GemmArgs a, Groups o) {
     };
     // the adapters of the tile's rows, one after the other (rows without one come last), KR ranks at a time
     if (split == 0) {
-        int g = first, p0 = 0, p1 = __builtin_amdgcn_readfirstlane(ends[0]), r0 = 0, buf = 0;
+        int g = first, p0 = 0, p1 = first_end, r0 = 0, buf = 0;
         while (g < a.G) {
             place(r0, buf);
-            meet();  // this block has landed for every wave, and the one before has been read
+            meet(false);  // this block has landed for every wave, and the one before has been read
             int g1 = g, q0 = p0, q1 = p1, r1 = r0 + KR;
             if (r1 >= a.R) {
                 r1 = 0, q0 = p1;
                 g1 = q0 < live ? __builtin_amdgcn_readfirstlane(sid[q0]) : a.G;
                 if (g1 < a.G) q1 = __builtin_amdgcn_readfirstlane(ends[q0]);
             }
-            if (g1 < a.G) fetch(g1, r1, buf ^ 1);
+            if (g1 < a.G) fetch(g1, r1, buf ^ 1, [&](int r) { return rows[r]; });
             const uint4* st = lds + buf * BLOCK;
             const uint4* sw = st + PARTS * BM * 4;
 #pragma unroll
@@ -757,15 +895,182 @@ gemm_kernel(GemmArgs a, Groups o) {
     else store((O*)a.out, a.ldo, a.vec);
 }
 
-// the sum of a product's splits, in order
+// the sum of a product's splits, in order; four columns a thread where rows are a multiple of that
 template <typename O>
-__global__ void __launch_bounds__(256) gemm_join_kernel(GemmArgs a) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, all = a.M * a.N;
+__global__ void __launch_bounds__(256) gemm_join_kernel(GemmArgs a, int wide) {
+    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * wide, all = a.M * a.N;
     if (i >= all) return;
-    float s = 0.f;
-    for (unsigned k = 0; k < a.splits; ++k) s += a.part[k * all + i];
-    store_as((O*)a.out + i / a.N * a.ldo + i % a.N, s);
+    O* d = (O*)a.out + i / a.N * a.ldo + i % a.N;
+    if (wide == 4) {
+        f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+        for (unsigned k = 0; k < a.splits; ++k) s += *reinterpret_cast<const f32x4*>(a.part + k * all + i);
+        if (a.vec) put4(d, s);
+        else
+#pragma unroll
+            for (int e = 0; e < 4; ++e) store_as(d + e, s[e]);
+    } else {
+        float s = 0.f;
+#pragma unroll 8
+        for (unsigned k = 0; k < a.splits; ++k) s += a.part[k * all + i];
+        store_as(d, s);
+    }
 }
+
+// ------------------------------------------------------------------------------------------
+// Few rows (up to 64): everything is read once and little is computed, so the contraction is cut over the chip and
+// joined. One launch forms the sums of both products over x, block by block: 32 rows of C by all rows, or 16 KT ranks of one
+// adapter by its rows (16 at a time), over one of `splits` ranges of the contraction; the block's 8 waves take an eighth of the
+// range each and add up in LDS. Bound by reading C and the used adapters' down. The second adds the ranges, in order, and
+// expands: a lane four columns of one row. No sort: the rows of an adapter are found by comparing up to 64 ids.
+constexpr int kFewRows = 64, kFewWaves = 8;
+
+struct FewArgs {
+    const char *X, *C, *W;  // W: the bank contracted with x
+    int64_t ldx, kp;        // bytes of a row of X, and of C and W
+    int n, p, pp, G, R, splits, c_blocks, r_blocks;
+    const int32_t* ids;
+    float *part, *part_h;  // splits x n x pp (p padded to a multiple of 4), splits x n x R
+};
+
+template <typename T, int MT, int NT>
+__device__ __forceinline__ void few_sum(const char* (&a)[MT], const char* (&b)[NT], int l0, int l1, f32x4 (*red)[MT * NT][64], f32x4 (&out)[MT * NT]) {
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    f32x4 acc[MT * NT];
+#pragma unroll
+    for (int i = 0; i < MT * NT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int each = (l1 - l0 + kFewWaves - 1) / kFewWaves, e1 = min(l1, l0 + (w + 1) * each);
+    for (int l = l0 + w * each; l < e1; ++l) {
+        uint4 fa[2][MT], fb[2][NT];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i) fa[h][i] = *reinterpret_cast<const uint4*>(a[i] + (int64_t)l * 128 + h * 64);
+#pragma unroll
+            for (int j = 0; j < NT; ++j) fb[h][j] = *reinterpret_cast<const uint4*>(b[j] + (int64_t)l * 128 + h * 64);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) acc[i * NT + j] = mma<T>(fa[h][i], fb[h][j], acc[i * NT + j]);
+    }
+#pragma unroll
+    for (int i = 0; i < MT * NT; ++i) red[w][i][lane] = acc[i];
+    __syncthreads();
+    // tile i of the sum is left with wave i % 8, in out[i / 8]
+#pragma unroll
+    for (int i = 0; i < MT * NT; ++i) {
+        if (i % kFewWaves != w) continue;
+        f32x4 x = red[0][i][lane];
+#pragma unroll
+        for (int k = 1; k < kFewWaves; ++k) x += red[k][i][lane];
+        out[i / kFewWaves] = x;
+    }
+}
+
+template <typename T, int NT, int KT>
+__global__ void __launch_bounds__(64 * kFewWaves) few_sums_kernel(FewArgs a) {
+    constexpr int MT = 2, TILES = MT * NT > KT ? MT * NT : KT;
+    __shared__ f32x4 red[kFewWaves * TILES * 64];
+    __shared__ int members[17];
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, c = lane & 15, q = lane >> 4;
+    const int lines = (int)(a.kp / 128), split = blockIdx.y;
+    const int l0 = (int)((int64_t)lines * split / a.splits), l1 = (int)((int64_t)lines * (split + 1) / a.splits);
+    if ((int)blockIdx.x < a.c_blocks) {
+        const int c0 = blockIdx.x * 32;
+        const char *pa[MT], *pb[NT];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) pa[i] = a.C + min(c0 + i * 16 + c, a.p - 1) * a.kp + q * 16;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) pb[j] = a.X + min(j * 16 + c, a.n - 1) * a.ldx + q * 16;
+        f32x4 out[MT * NT];
+        few_sum<T, MT, NT>(pa, pb, l0, l1, reinterpret_cast<f32x4(*)[MT * NT][64]>(red), out);
+#pragma unroll
+        for (int i = 0; i < MT * NT; ++i) {
+            const int row = i % NT * 16 + c, col = c0 + i / NT * 16 + 4 * q;
+            if (i % kFewWaves == w && row < a.n && col < a.pp)
+                *reinterpret_cast<f32x4*>(a.part + ((int64_t)split * a.n + row) * a.pp + col) = out[i / kFewWaves];
+        }
+        return;
+    }
+    const int k = blockIdx.x - a.c_blocks, row = k / a.r_blocks, r0 = k % a.r_blocks * 16 * KT;
+    const int g = lane < a.n ? group_of(a.ids[lane], a.G) : a.G, mine = __builtin_amdgcn_readlane(g, row);
+    if (mine == a.G) return;
+    const uint64_t same = __ballot(g == mine);
+    const int before = __popcll(same & ((1ull << row) - 1)), at = __popcll(same & ((1ull << lane) - 1)) - before;
+    if (before % 16) return;  // the block of an earlier row takes this one
+    if (w == 0) {
+        if ((same >> lane & 1) && at >= 0 && at < 16) members[at] = lane;
+        if (lane == 0) members[16] = min(16, (int)__popcll(same) - before);
+    }
+    __syncthreads();
+    const int count = members[16];
+    const char *pa[KT], *pb[1];
+#pragma unroll
+    for (int i = 0; i < KT; ++i) pa[i] = a.W + ((int64_t)mine * a.R + min(r0 + i * 16 + c, a.R - 1)) * a.kp + q * 16;
+    pb[0] = a.X + members[min(c, count - 1)] * a.ldx + q * 16;
+    f32x4 out[KT];
+    few_sum<T, KT, 1>(pa, pb, l0, l1, reinterpret_cast<f32x4(*)[KT][64]>(red), out);
+#pragma unroll
+    for (int i = 0; i < KT; ++i) {
+        if (i % kFewWaves != w || c >= count) continue;
+        const int r = r0 + i * 16 + 4 * q;
+        float* h = a.part_h + ((int64_t)split * a.n + members[c]) * a.R + r;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (r + e < a.R) h[e] = out[i / kFewWaves][e];
+    }
+}
+
+template <typename T, typename O>
+__global__ void __launch_bounds__(64)
+few_join_kernel(FewArgs a, const T* __restrict__ up, int64_t wp, const float* __restrict__ scale, O* __restrict__ Y, int64_t ldy,
+                float* __restrict__ hidden) {
+    __shared__ float h[kMaxRank];
+    const int row = blockIdx.y, lane = threadIdx.x, g = group_of(a.ids[row], a.G);
+    const int col = (blockIdx.x * 64 + lane) * 4;
+    f32x4 y = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (col < a.pp)
+        for (int k = 0; k < a.splits; ++k) y += *reinterpret_cast<const f32x4*>(a.part + ((int64_t)k * a.n + row) * a.pp + col);
+    if (g < a.G || hidden) {
+        const float s = g < a.G && scale ? scale[g] : 1.f;
+        for (int r = lane; r < a.R; r += 64) {
+            float x = 0.f;
+            if (g < a.G)
+                for (int k = 0; k < a.splits; ++k) x += a.part_h[((int64_t)k * a.n + row) * a.R + r];
+            h[r] = x * s;
+            if (hidden && blockIdx.x == 0) hidden[(int64_t)row * a.R + r] = x;
+        }
+    }
+    __syncthreads();
+    if (col >= a.p) return;
+    if (g < a.G) {
+        const T* __restrict__ u = up + (int64_t)g * a.R * wp + col;  // columns up to the padded width are there
+        f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+        for (int r = 0; r < a.R; ++r) {
+            f32x4 v;
+            if constexpr (sizeof(T) == 2) {
+                const uint2 b = *reinterpret_cast<const uint2*>(u + r * wp);
+                v = f32x4{__uint_as_float(b.x << 16), __uint_as_float(b.x & 0xffff0000u), __uint_as_float(b.y << 16),
+                          __uint_as_float(b.y & 0xffff0000u)};
+            } else {
+                v = *reinterpret_cast<const f32x4*>(u + r * wp);
+            }
+            const float f = h[r];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = fmaf(f, v[e], x[e]);
+        }
+        y += x;
+    }
+    O* d = Y + row * ldy + col;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (col + e < a.p) store_as(d + e, y[e]);
+}
+
 int64_t padded(int64_t w, int32_t dtype) {
     const int64_t step = dtype == RP_BF16 ? 64 : 32;
     return (w + step - 1) / step * step;
@@ -783,21 +1088,70 @@ int check_shared(int32_t dtype, int64_t n, int64_t m, int64_t p, int64_t G, int3
 
 int check_operand(const char* name, const void* p, int64_t ld, int64_t width, int32_t dtype) {
     if (!p) return fail(RP_ERR_INVALID, "NULL %s", name);
-    if (ld < width) return fail(RP_ERR_INVALID, "%s: row stride %lld is under its padded width %lld", name, (long long)ld,
+    if (ld < width) return fail(RP_ERR_INVALID, "%s: row stride %lld is under its width %lld", name, (long long)ld,
                                 (long long)width);
     if (((uintptr_t)p & 15) || (ld * (dtype == RP_BF16 ? 2 : 4)) % 16)
         return fail(RP_ERR_INVALID, "%s must have 16-byte aligned rows", name);
     return RP_OK;
 }
 
+// rows that are copied to padded ones first may lie anywhere
+int check_rows(const char* name, const void* p, int64_t ld, int64_t width, int32_t dtype) {
+    if (padded(width, dtype) == width) return check_operand(name, p, ld, width, dtype);
+    if (!p) return fail(RP_ERR_INVALID, "NULL %s", name);
+    if (ld < width || ((uintptr_t)p & (dtype == RP_BF16 ? 1 : 3)))
+        return fail(RP_ERR_INVALID, "%s: row stride under its width, or not aligned to its elements", name);
+    return RP_OK;
+}
+
+// a product with its expand for few rows: O (n x p) = X C^T + the adapters' part, hidden = the rows' H or NULL (p = 0: H alone)
+int64_t few_splits(int64_t n, int64_t p, int R, int64_t line_bytes) {
+    // about 512 blocks, none with less than two lines a wave
+    const int64_t blocks = std::max<int64_t>(1, (p + 31) / 32 + n * ((R + 31) / 32));
+    return std::max<int64_t>(1, std::min<int64_t>({512 / blocks, line_bytes / 128 / (2 * kFewWaves), 16}));
+}
+
+size_t few_bytes(int64_t n, int64_t p, int R, int64_t line_bytes) {
+    return ((size_t)4 * few_splits(n, p, R, line_bytes) * n * ((p + 3) / 4 * 4 + R) + 255) & ~(size_t)255;
+}
+
+template <typename T, typename O>
+int launch_few(const T* X, int64_t ldx, const T* C, int64_t kp, int64_t n, int64_t p, const T* W, const T* U, int64_t wp, int G, int R,
+               const float* scale, const int32_t* ids, O* out, int64_t ldo, float* hidden, char* ws, hipStream_t st) {
+    constexpr int64_t es = sizeof(T);
+    FewArgs a{};
+    a.X = (const char*)X, a.C = (const char*)C, a.W = (const char*)W, a.ldx = ldx * es, a.kp = kp * es;
+    a.n = (int)n, a.p = (int)p, a.pp = (int)((p + 3) / 4 * 4), a.G = G, a.R = R, a.ids = ids;
+    a.splits = (int)few_splits(n, p, R, a.kp);
+    const int kt = R <= 16 ? 1 : 2;
+    a.c_blocks = (int)((p + 31) / 32), a.r_blocks = (R + 16 * kt - 1) / (16 * kt);
+    a.part = (float*)ws, a.part_h = a.part + (int64_t)a.splits * n * a.pp;
+    const dim3 grid((unsigned)(a.c_blocks + n * a.r_blocks), (unsigned)a.splits), block(64 * kFewWaves);
+    const int nt = n <= 16 ? 1 : n <= 32 ? 2 : 4;
+    if (kt == 1) {
+        if (nt == 1) hipLaunchKernelGGL((few_sums_kernel<T, 1, 1>), grid, block, 0, st, a);
+        else if (nt == 2) hipLaunchKernelGGL((few_sums_kernel<T, 2, 1>), grid, block, 0, st, a);
+        else hipLaunchKernelGGL((few_sums_kernel<T, 4, 1>), grid, block, 0, st, a);
+    } else {
+        if (nt == 1) hipLaunchKernelGGL((few_sums_kernel<T, 1, 2>), grid, block, 0, st, a);
+        else if (nt == 2) hipLaunchKernelGGL((few_sums_kernel<T, 2, 2>), grid, block, 0, st, a);
+        else hipLaunchKernelGGL((few_sums_kernel<T, 4, 2>), grid, block, 0, st, a);
+    }
+    HIP_TRY(hipGetLastError());
+    hipLaunchKernelGGL((few_join_kernel<T, O>), dim3((unsigned)std::max<int64_t>(1, (p + 255) / 256), (unsigned)n), dim3(64), 0, st, a, U, wp, scale, out, ldo,
+                       hidden);
+    HIP_TRY(hipGetLastError());
+    return RP_OK;
+}
+
 // Everything a call lays out in its workspace and launches, from its sizes alone.
 struct Plan {
-    int bits, tile_rows, chunk_rows, kt, waves;  // kt: shrink's rank tiles (1, 2, 4 or 8)
+    int bits, tile_rows, chunk_rows, kt;  // kt: shrink's rank tiles (1, 2, 4 or 8)
     bool small;                                  // one block groups the rows
     int64_t each;                                // else rows of a wave that counts
     int n_chunks;
     int64_t max_tiles, max_chunks, max_parts;
-    size_t perm, sid, start, tiles, chunks, tile0, chunk0, multi0, number, hist, pieces, t, part, bytes;
+    size_t perm, sid, start, tiles, chunks, tile0, chunk0, multi0, number, hist, pieces, t, part, shrink, pad_x, pad_dy, bytes;
 };
 
 // split of a product over the contraction: enough blocks for 256 CUs with two each, where there are few tiles, as long as a split has
@@ -816,6 +1170,11 @@ Tiling tiling(int64_t M, int64_t N, int64_t steps) {
     return t;
 }
 
+// of the shrink of few rows: about 1024 blocks, none with less than two lines a wave
+int shrink_splits(int64_t tiles, int64_t row_bytes) {
+    return (int)std::max<int64_t>(1, std::min<int64_t>({1024 / std::max<int64_t>(1, tiles), row_bytes / 128 / 8, 32}));
+}
+
 Plan plan_for(int32_t dtype, int64_t n, int64_t m, int64_t p, int64_t G, int R, int what) {
     Plan l;
     const int es = dtype == RP_BF16 ? 2 : 4;
@@ -823,19 +1182,18 @@ Plan plan_for(int32_t dtype, int64_t n, int64_t m, int64_t p, int64_t G, int R, 
     l.bits = 1;
     while ((G >> l.bits) != 0) ++l.bits;
     l.kt = R <= 16 ? 1 : R <= 32 ? 2 : R <= 64 ? 4 : 8;
-    const int rt = l.kt <= 2 ? 4 : l.kt == 4 ? 2 : 1;
+    const int rt = l.kt <= 4 ? 4 : 2;
     // many rows: as many of them as registers hold under one read of the adapter; few: 16, for more blocks
     const bool many = n >= 512 * 16 * rt;
     l.tile_rows = many ? 16 * rt : 16;
-    l.waves = many ? 4 : 8;
-    // chunks of rows for the banks' gradients: long, unless that leaves under 1024 blocks
-    l.chunk_rows = (int)std::max<int64_t>(64, std::min<int64_t>(kMaxChunk, n * ((m + 511) / 512) / 1024 / 64 * 64));
-    l.small = n <= 4096 && G <= 800;
+    // chunks of rows for the banks' gradients: long, unless that leaves under 2048 blocks
+    l.chunk_rows = (int)std::max<int64_t>(256, std::min<int64_t>(kMaxChunk, n * ((m + 127) / 128) / 2048 / 64 * 64));
+    l.small = n <= kSmallRows && G <= 700;
     l.each = 256;
     while ((n + l.each - 1) / l.each * (G + 1) > (1 << 22)) l.each *= 2;
     l.n_chunks = l.small ? 0 : (int)((n + l.each - 1) / l.each);
     l.max_tiles = n / l.tile_rows + std::min(n, G + 1);
-    l.max_chunks = n / l.chunk_rows + std::min(n, G);
+    l.max_chunks = n / l.chunk_rows + G;
     l.max_parts = 2 * (n / l.chunk_rows);
     size_t at = 0;
     const auto take = [&](size_t b) {
@@ -856,13 +1214,18 @@ Plan plan_for(int32_t dtype, int64_t n, int64_t m, int64_t p, int64_t G, int R, 
         l.part = take(g.splits > 1 ? (size_t)4 * g.splits * n * p : 0);
     } else {
         l.t = take((size_t)4 * n * R);
-        size_t part = (size_t)4 * l.max_parts * R * std::max(mk, pk);
+        size_t part = (size_t)4 * l.max_parts * R * (mk + pk);
         if (what == RP_ADAPT_GRADIENTS_DX) {
             const Tiling g = tiling(n, m, pk * es / 128);
             if (g.splits > 1) part = std::max(part, (size_t)4 * g.splits * n * m);
         }
+        if (n <= kFewRows) part = std::max(part, few_bytes(n, what == RP_ADAPT_GRADIENTS_DX ? m : 0, R, pk * es));
         l.part = take(part);
     }
+    const int splits = l.tile_rows > 16 ? 1 : shrink_splits(l.max_tiles, (what == RP_ADAPT_PROJECT ? mk : pk) * es);
+    l.shrink = take(splits > 1 ? (size_t)splits * l.max_tiles * l.kt * 1024 : 0);
+    l.pad_x = take(mk != m ? (size_t)n * mk * es : 0);
+    l.pad_dy = take(what != RP_ADAPT_PROJECT && pk != p ? (size_t)n * pk * es : 0);
     l.bytes = at;
     return l;
 }
@@ -876,11 +1239,34 @@ Groups groups_of(const Plan& l, char* ws) {
     return o;
 }
 
-int launch_groups(const Plan& l, const Groups& o, const int32_t* ids, int64_t n, int G, hipStream_t st) {
+// X as the kernels read it: itself, or a padded copy made by the call's first launch
+template <typename T>
+Pad pad_of(const T*& X, int64_t& ldx, int64_t n, int64_t width, void* to) {
+    Pad p{};
+    const int64_t kp = padded(width, sizeof(T) == 2 ? RP_BF16 : RP_F32);
+    if (kp == width || n == 0) return p;
+    p = Pad{X, to, ldx, n, (int)width, (int)kp, (int)sizeof(T)};
+    X = (const T*)to, ldx = kp;
+    return p;
+}
+unsigned pad_blocks(const Pad& p, const Pad& q, int threads) {
+    const auto need = [&](const Pad& x) {
+        const int each = x.padded <= 256 ? 64 : x.padded <= 1024 ? 256 : threads;
+        return x.to ? (x.rows + threads / each - 1) / (threads / each) : 0;
+    };
+    return (unsigned)std::min<int64_t>(std::max(need(p), need(q)), 2048);
+}
+
+int launch_groups(const Plan& l, const Groups& o, const int32_t* ids, int64_t n, int G, const Pad& p, const Pad& q, hipStream_t st) {
     if (l.small) {
-        hipLaunchKernelGGL(group_small_kernel, dim3(1), dim3(1024), 4 * (17 * (G + 1) + 1), st, ids, (int)n, G, l.bits, l.tile_rows,
-                           l.chunk_rows, o);
+        const unsigned waves = n <= 256 ? 4 : 16;
+        hipLaunchKernelGGL(group_small_kernel, dim3(1 + pad_blocks(p, q, (int)waves * 64)), dim3(64 * waves), 4 * ((waves + 4) * (G + 1) + 1), st, ids,
+                           (int)n, G, l.bits, l.tile_rows, l.chunk_rows, o, p, q);
     } else {
+        if (const unsigned blocks = pad_blocks(p, q, 256)) {
+            hipLaunchKernelGGL(pad_kernel, dim3(blocks), dim3(256), 0, st, p, q);
+            HIP_TRY(hipGetLastError());
+        }
         const int waves = G < 4000 ? 4 : 1;
         const dim3 grid((unsigned)((l.n_chunks + waves - 1) / waves)), block(64 * waves);
         const size_t lds = (size_t)4 * waves * (G + 1);
@@ -896,38 +1282,47 @@ int launch_groups(const Plan& l, const Groups& o, const int32_t* ids, int64_t n,
 
 template <typename T>
 int launch_shrink(const Plan& l, const ShrinkArgs& a, const Groups& o, hipStream_t st) {
-    const dim3 grid((unsigned)l.max_tiles);
-    if (l.waves == 4) {
-        if (l.kt == 1) hipLaunchKernelGGL((shrink_kernel<T, 4, 1, 4>), grid, dim3(256), 0, st, a, o);
-        else if (l.kt == 2) hipLaunchKernelGGL((shrink_kernel<T, 4, 2, 4>), grid, dim3(256), 0, st, a, o);
-        else if (l.kt == 4) hipLaunchKernelGGL((shrink_kernel<T, 2, 4, 4>), grid, dim3(256), 0, st, a, o);
-        else hipLaunchKernelGGL((shrink_kernel<T, 1, 8, 4>), grid, dim3(256), 0, st, a, o);
-    } else {
-        if (l.kt == 1) hipLaunchKernelGGL((shrink_kernel<T, 1, 1, 8>), grid, dim3(512), 0, st, a, o);
-        else if (l.kt == 2) hipLaunchKernelGGL((shrink_kernel<T, 1, 2, 8>), grid, dim3(512), 0, st, a, o);
-        else if (l.kt == 4) hipLaunchKernelGGL((shrink_kernel<T, 1, 4, 8>), grid, dim3(512), 0, st, a, o);
-        else hipLaunchKernelGGL((shrink_kernel<T, 1, 8, 8>), grid, dim3(512), 0, st, a, o);
+    if (l.tile_rows > 16) {
+        const dim3 grid((unsigned)l.max_tiles), block(256);
+        if (l.kt == 1) hipLaunchKernelGGL((shrink_kernel<T, 4, 1>), grid, block, 0, st, a, o);
+        else if (l.kt == 2) hipLaunchKernelGGL((shrink_kernel<T, 4, 2>), grid, block, 0, st, a, o);
+        else if (l.kt == 4) hipLaunchKernelGGL((shrink_kernel<T, 4, 4>), grid, block, 0, st, a, o);
+        else hipLaunchKernelGGL((shrink_kernel<T, 2, 8>), grid, block, 0, st, a, o);
+        HIP_TRY(hipGetLastError());
+        return RP_OK;
     }
+    const int splits = shrink_splits(l.max_tiles, a.kp * (int64_t)sizeof(T));
+    const dim3 grid((unsigned)l.max_tiles, (unsigned)splits), block(256), tiles((unsigned)l.max_tiles), lanes(64 * l.kt);
+    if (l.kt == 1) hipLaunchKernelGGL((shrink_kernel<T, 1, 1>), grid, block, 0, st, a, o);
+    else if (l.kt == 2) hipLaunchKernelGGL((shrink_kernel<T, 1, 2>), grid, block, 0, st, a, o);
+    else if (l.kt == 4) hipLaunchKernelGGL((shrink_kernel<T, 1, 4>), grid, block, 0, st, a, o);
+    else hipLaunchKernelGGL((shrink_kernel<T, 1, 8>), grid, block, 0, st, a, o);
+    HIP_TRY(hipGetLastError());
+    if (splits == 1) return RP_OK;
+    if (l.kt == 1) hipLaunchKernelGGL((shrink_join_kernel<T, 1>), tiles, lanes, 0, st, a, o, splits);
+    else if (l.kt == 2) hipLaunchKernelGGL((shrink_join_kernel<T, 2>), tiles, lanes, 0, st, a, o, splits);
+    else if (l.kt == 4) hipLaunchKernelGGL((shrink_join_kernel<T, 4>), tiles, lanes, 0, st, a, o, splits);
+    else hipLaunchKernelGGL((shrink_join_kernel<T, 8>), tiles, lanes, 0, st, a, o, splits);
     HIP_TRY(hipGetLastError());
     return RP_OK;
 }
 
 template <typename T>
-int launch_outer(const Plan& l, const OuterArgs& a, const Groups& o, int G, hipStream_t st) {
-    if (l.max_chunks) {
-        const int64_t wide = 4 * 16 * (sizeof(T) == 2 ? 8 : 4);
-        const unsigned qb = (unsigned)((a.q + wide - 1) / wide);
-        if (qb > 65535) return fail(RP_ERR_UNSUPPORTED, "m or p too large");
-        const int kt = a.R <= 16 ? 1 : a.R <= 32 ? 2 : 4;
-        const dim3 grid((unsigned)l.max_chunks, qb, (unsigned)((a.R + 16 * kt - 1) / (16 * kt))), block(256);
-        if (kt == 1) hipLaunchKernelGGL((outer_kernel<T, 1>), grid, block, 0, st, a, o);
-        else if (kt == 2) hipLaunchKernelGGL((outer_kernel<T, 2>), grid, block, 0, st, a, o);
-        else hipLaunchKernelGGL((outer_kernel<T, 4>), grid, block, 0, st, a, o);
+int launch_outer(const Plan& l, const OuterArgs& a, const OuterArgs& b, const Groups& o, int64_t n, int G, hipStream_t st) {
+    const int64_t wide = 16 * (sizeof(T) == 2 ? 8 : 4);
+    const int64_t qa = (a.q + wide - 1) / wide, qb = (b.q + wide - 1) / wide;
+    if ((qa + qb) * l.max_chunks >= ((int64_t)1 << 31)) return fail(RP_ERR_UNSUPPORTED, "too many adapters and columns for one launch");
+    const int kt = a.R <= 16 ? 1 : a.R <= 32 ? 2 : 4;
+    const dim3 grid((unsigned)((qa + qb) * l.max_chunks), 1, (unsigned)((a.R + 16 * kt - 1) / (16 * kt))), block(256);
+    if (kt == 1) hipLaunchKernelGGL((outer_kernel<T, 1>), grid, block, 0, st, a, b, (int)qa, (int)(qa + qb), o);
+    else if (kt == 2) hipLaunchKernelGGL((outer_kernel<T, 2>), grid, block, 0, st, a, b, (int)qa, (int)(qa + qb), o);
+    else hipLaunchKernelGGL((outer_kernel<T, 4>), grid, block, 0, st, a, b, (int)qa, (int)(qa + qb), o);
+    HIP_TRY(hipGetLastError());
+    if (n > l.chunk_rows) {  // else no adapter has two chunks
+        const unsigned ja = (unsigned)((a.q + 255) / 256), jb = (unsigned)((b.q + 255) / 256);
+        hipLaunchKernelGGL(outer_join_kernel, dim3(ja + jb, (unsigned)a.R, (unsigned)G), dim3(256), 0, st, a, b, (int)ja, o, l.chunk_rows);
         HIP_TRY(hipGetLastError());
     }
-    hipLaunchKernelGGL(outer_join_kernel, dim3((unsigned)((a.q + 255) / 256), (unsigned)a.R, (unsigned)G), dim3(256), 0, st, a, o,
-                       l.chunk_rows);
-    HIP_TRY(hipGetLastError());
     return RP_OK;
 }
 
@@ -938,11 +1333,12 @@ int launch_gemm(GemmArgs a, const Groups& o, hipStream_t st) {
     const uint64_t per = ((uint64_t)t.m_tiles * t.n_tiles * t.splits + 7) / 8;
     if (per * 8 >= (1ull << 31)) return fail(RP_ERR_UNSUPPORTED, "too many rows for one launch");
     a.per_xcd = (unsigned)per;
-    if (t.big) hipLaunchKernelGGL((gemm_kernel<T, O, 256, 256, 2, 4>), dim3(a.per_xcd * 8), dim3(512), 0, st, a, o);
-    else hipLaunchKernelGGL((gemm_kernel<T, O, 128, 128, 2, 2>), dim3(a.per_xcd * 8), dim3(256), 0, st, a, o);
+    if (t.big) hipLaunchKernelGGL((gemm_kernel<T, O, 256, 2, 4>), dim3(a.per_xcd * 8), dim3(512), 0, st, a, o);
+    else hipLaunchKernelGGL((gemm_kernel<T, O, 128, 2, 2>), dim3(a.per_xcd * 8), dim3(256), 0, st, a, o);
     HIP_TRY(hipGetLastError());
     if (t.splits > 1) {
-        hipLaunchKernelGGL(gemm_join_kernel<O>, dim3((unsigned)((a.M * a.N + 255) / 256)), dim3(256), 0, st, a);
+        const int wide = a.N % 4 ? 1 : 4;
+        hipLaunchKernelGGL(gemm_join_kernel<O>, dim3((unsigned)((a.M * a.N / wide + 255) / 256)), dim3(256), 0, st, a, wide);
         HIP_TRY(hipGetLastError());
     }
     return RP_OK;
@@ -964,10 +1360,19 @@ int project(const T* X, int64_t ldx, int64_t n, int64_t m, const T* C, int64_t p
             const float* scale, const int32_t* ids, float* Y, int64_t ldy, float* hidden, char* ws, hipStream_t st) {
     constexpr int32_t dt = sizeof(T) == 2 ? RP_BF16 : RP_F32;
     const int64_t mk = padded(m, dt), pk = padded(p, dt);
+    if (n <= kFewRows) {
+        if (mk != m) {
+            const Pad pad = pad_of(X, ldx, n, m, ws + few_bytes(n, p, R, mk * (int64_t)sizeof(T)));
+            hipLaunchKernelGGL(pad_kernel, dim3(pad_blocks(pad, Pad{}, 256)), dim3(256), 0, st, pad, Pad{});
+            HIP_TRY(hipGetLastError());
+        }
+        return launch_few<T, float>(X, ldx, C, mk, n, p, down, up, pk, G, R, scale, ids, Y, ldy, hidden, ws, st);
+    }
     const Plan l = plan_for(dt, n, m, p, G, R, RP_ADAPT_PROJECT);
     const Groups o = groups_of(l, ws);
-    int rc = launch_groups(l, o, ids, n, G, st);
-    if (!rc) rc = launch_shrink<T>(l, ShrinkArgs{X, ldx, mk, down, G, R, scale, hidden, 0, ws + l.pieces}, o, st);
+    const Pad pad = pad_of(X, ldx, n, m, ws + l.pad_x);
+    int rc = launch_groups(l, o, ids, n, G, pad, Pad{}, st);
+    if (!rc) rc = launch_shrink<T>(l, ShrinkArgs{X, ldx, mk, down, G, R, scale, hidden, 0, ws + l.pieces, (f32x4*)(ws + l.shrink)}, o, st);
     if (!rc) rc = launch_gemm<T, float>(gemm_args<T, float>(X, ldx, C, mk, n, p, Y, ldy, ws + l.pieces, up, pk, G, R, ws + l.part), o, st);
     return rc;
 }
@@ -989,11 +1394,19 @@ int gradients(const T* dY, int64_t lddy, const T* X, int64_t ldx, int64_t n, int
     const Plan l = plan_for(dt, n, m, p, G, R, dX ? RP_ADAPT_GRADIENTS_DX : RP_ADAPT_GRADIENTS);
     const Groups o = groups_of(l, ws);
     float* t = (float*)(ws + l.t);
-    int rc = launch_groups(l, o, ids, n, G, st);
-    if (!rc && n) rc = launch_shrink<T>(l, ShrinkArgs{dY, lddy, pk, up, G, R, scale, t, 1, dX ? ws + l.pieces : nullptr}, o, st);
-    if (!rc) rc = launch_outer<T>(l, outer_args<T>(X, ldx, mk, m, R, nullptr, t, d_down, ldd, sdd, ws + l.part), o, G, st);
-    if (!rc) rc = launch_outer<T>(l, outer_args<T>(dY, lddy, pk, p, R, scale, hidden, d_up, ldu, sdu, ws + l.part), o, G, st);
-    if (!rc && dX && n)
+    const Pad px = pad_of(X, ldx, n, m, ws + l.pad_x), py = pad_of(dY, lddy, n, p, ws + l.pad_dy);
+    int rc = launch_groups(l, o, ids, n, G, px, py, st);
+    const bool few = n <= kFewRows;  // then t holds up dy without the scale, which the outer product takes on
+    if (!rc && n && few)
+        rc = launch_few<T, T>(dY, lddy, Ct, pk, n, dX ? m : 0, up, down, mk, G, R, scale, ids, dX, lddx, t, ws + l.part, st);
+    if (!rc && !few) rc = launch_shrink<T>(l, ShrinkArgs{dY, lddy, pk, up, G, R, scale, t, 1, dX ? ws + l.pieces : nullptr,
+                                                                   (f32x4*)(ws + l.shrink)}, o, st);
+    if (!rc) {
+        const OuterArgs a = outer_args<T>(X, ldx, mk, m, R, few ? scale : nullptr, t, d_down, ldd, sdd, ws + l.part);
+        const OuterArgs b = outer_args<T>(dY, lddy, pk, p, R, scale, hidden, d_up, ldu, sdu, ws + l.part + 4 * l.max_parts * R * mk);
+        rc = launch_outer<T>(l, a, b, o, n, G, st);
+    }
+    if (!rc && dX && !few)
         rc = launch_gemm<T, T>(gemm_args<T, T>(dY, lddy, Ct, pk, n, m, dX, lddx, ws + l.pieces, down, mk, G, R, ws + l.part), o, st);
     return rc;
 }
@@ -1005,6 +1418,10 @@ extern "C" {
 int64_t rp_adapt_workspace_bytes(int32_t dtype, int64_t n, int64_t m, int64_t p, int64_t adapters, int32_t rank,
                                  int32_t what) {
     if (check_shared(dtype, n, m, p, adapters, rank)) return -1;
+    if (what == RP_ADAPT_PROJECT && n <= kFewRows) {
+        const int64_t row = padded(m, dtype) * (dtype == RP_BF16 ? 2 : 4);
+        return (int64_t)few_bytes(n, p, rank, row) + (padded(m, dtype) != m ? n * row : 0);
+    }
     return (int64_t)plan_for(dtype, n, m, p, adapters, rank, what).bytes;
 }
 
@@ -1015,7 +1432,7 @@ int rp_adapt_project_device(int device, const void* X, int64_t ldx, int32_t dtyp
     int rc = check_shared(dtype, n, m, p, adapters, rank);
     if (rc) return rc;
     const int64_t mk = padded(m, dtype), pk = padded(p, dtype);
-    if ((rc = check_operand("X", X, ldx, mk, dtype)) || (rc = check_operand("C", C, mk, mk, dtype)) ||
+    if ((rc = check_rows("X", X, ldx, m, dtype)) || (rc = check_operand("C", C, mk, mk, dtype)) ||
         (rc = check_operand("down", down, mk, mk, dtype)) || (rc = check_operand("up", up, pk, pk, dtype)))
         return rc;
     if (!ids || !Y) return fail(RP_ERR_INVALID, "NULL ids or Y");
@@ -1045,7 +1462,7 @@ int rp_adapt_gradients_device(int device, const void* dY, int64_t lddy, const vo
     int rc = check_shared(dtype, n, m, p, adapters, rank);
     if (rc) return rc;
     const int64_t mk = padded(m, dtype), pk = padded(p, dtype);
-    if (n && ((rc = check_operand("dY", dY, lddy, pk, dtype)) || (rc = check_operand("X", X, ldx, mk, dtype)))) return rc;
+    if (n && ((rc = check_rows("dY", dY, lddy, p, dtype)) || (rc = check_rows("X", X, ldx, m, dtype)))) return rc;
     if ((rc = check_operand("down", down, mk, mk, dtype)) || (rc = check_operand("up", up, pk, pk, dtype))) return rc;
     if (!Ct != !dX) return fail(RP_ERR_INVALID, "Ct and dX go together");
     if (Ct && ((rc = check_operand("Ct", Ct, pk, pk, dtype)))) return rc;

@@ -9,6 +9,8 @@ from __future__ import annotations
 import ctypes
 import weakref
 
+import torch
+
 from . import _native as nat
 
 __all__ = ["AdamW", "BLOCK"]
@@ -38,8 +40,6 @@ class AdamW:
 
     def __init__(self, params, grads, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, *, state_bits=32,
                  copies=None, seed=0):
-        import torch
-
         params, grads = list(params), list(grads)
         copies = None if copies is None else list(copies)
         if not params or len(grads) != len(params) or (copies is not None and len(copies) != len(params)):
@@ -92,8 +92,6 @@ class AdamW:
             raise ValueError("lr, eps and weight_decay must not be negative, the betas lie in [0, 1)")
 
     def _stream(self, stream, *tensors):
-        import torch
-
         cur = torch.cuda.current_stream(self.device)
         if stream is None or stream == cur.cuda_stream:
             return cur.cuda_stream
@@ -108,8 +106,6 @@ class AdamW:
         """One step of every tensor, or of those whose entry of ``active`` (a uint8 or bool device tensor, one for each
         tensor) is not zero: the others keep their values, states and step counts. lr: for this step only. Asynchronous on
         ``stream`` (default: torch's current one); can be captured into a graph, with the numbers of the call."""
-        import torch
-
         lr = self.lr if lr is None else lr
         self._check_numbers(lr)
         if active is not None and (active.dtype not in (torch.uint8, torch.bool) or tuple(active.shape) != (len(self.params),)
@@ -121,8 +117,6 @@ class AdamW:
 
     def state_values(self, *, stream=None):
         """(m, sqrt(v)) of all blocks in float32: 256 elements a block, the last block of a tensor padded with zeros."""
-        import torch
-
         if self.state_bits == 32:
             return self.state["exp_avg"].clone(), self.state["exp_avg_sq"].sqrt()
         m, root = (torch.empty(self.state["exp_avg"].numel(), dtype=torch.float32, device=self.device) for _ in range(2))

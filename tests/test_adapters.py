@@ -127,7 +127,7 @@ def test_abi_refuses_before_the_device_is_used():
                     scale=None, ids=a, hidden=a, dX=a, lddx=64, dd=a, dd_r=64, dd_a=256, du=a, du_r=8, du_a=32, ws=a,
                     bytes=1 << 20, stream=None)
     for change, code, text in (
-            ({"lddy": 8}, nat.RP_ERR_INVALID, b"dY"), ({"Ct": None}, nat.RP_ERR_INVALID, b"go together"),
+            ({"lddy": 7}, nat.RP_ERR_INVALID, b"dY"), ({"dY": a + 1}, nat.RP_ERR_INVALID, b"dY"), ({"Ct": None}, nat.RP_ERR_INVALID, b"go together"),
             ({"dX": None}, nat.RP_ERR_INVALID, b"go together"), ({"lddx": 63}, nat.RP_ERR_INVALID, b"dX"),
             ({"dd": None}, nat.RP_ERR_INVALID, b"NULL"), ({"dd_a": 255}, nat.RP_ERR_INVALID, b"strides"),
             ({"du_r": 7}, nat.RP_ERR_INVALID, b"strides"), ({"hidden": None}, nat.RP_ERR_INVALID, b"hidden"),

@@ -36,6 +36,13 @@ def _dtype(compute):
         raise ValueError("compute must be 'fp32' or 'bf16'") from None
 
 
+def raw_stream(device):
+    """The handle of torch's current stream on a device; through torch's own accessor where it has one, since making a Stream
+    object costs as much as a kernel launch."""
+    get = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return get(device) if get is not None else torch.cuda.current_stream(device).cuda_stream
+
+
 @functools.lru_cache(maxsize=4096)
 def _workspace_bytes(code, n, m, p, G, R, what):
     return nat.load().rp_adapt_workspace_bytes(code, n, m, p, G, R, what)
@@ -105,14 +112,16 @@ def _check_device(*tensors):
             raise ValueError("all tensors must be on one device")
     if dev.type != "cuda":
         raise RuntimeError("adapted projections need an MI355X (no CPU fallback)")
-    return dev, torch.cuda.current_stream(dev)
+    return dev
 
 
-def _on_stream(stream, cur, tensors):
-    """The stream to launch on. One other than torch's current stream waits for what is queued there (casts and pads
-    of the operands), and the temporaries made here are kept for it."""
-    if stream is None or stream == cur.cuda_stream:
-        return cur.cuda_stream
+def _on_stream(stream, dev, tensors):
+    """The stream to launch on. One other than torch's current stream waits for what is queued there (casts of the
+    operands), and the temporaries made here are kept for it."""
+    now = raw_stream(dev.index)
+    if stream is None or stream == now:
+        return now
+    cur = torch.cuda.current_stream(dev)
     ext = torch.cuda.ExternalStream(stream, device=cur.device)
     ext.wait_stream(cur)
     for t in tensors:
@@ -148,7 +157,7 @@ def adapted_project_device(X, C, down, up, ids, *, scale=None, out=None, compute
     Uc = _operand("up", up, (G, R, p), compute, prepared)
     if out is not None:
         _strided("out", out, (n, p), torch.float32)
-    dev, cur = _check_device(X, C, down, up, ids, scale, out)
+    dev = _check_device(X, C, down, up, ids, scale, out)
     Xc = _rows(X, compute)
     y = out if out is not None else torch.empty(n, p, dtype=torch.float32, device=dev)
     hidden = torch.empty(n, R, dtype=torch.float32, device=dev) if return_hidden else None
@@ -156,7 +165,7 @@ def adapted_project_device(X, C, down, up, ids, *, scale=None, out=None, compute
         lib, code = nat.load(), _CODE[compute]
         need = _workspace_bytes(code, n, m, p, G, R, nat.RP_ADAPT_PROJECT)
         ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
-        st = _on_stream(stream, cur, (Xc, Cc, Dc, Uc, ids, scale, y, hidden, ws))
+        st = _on_stream(stream, dev, (Xc, Cc, Dc, Uc, ids, scale, y, hidden, ws))
         nat.check(lib.rp_adapt_project_device(
             dev.index, Xc.data_ptr(), _ld(Xc), code, n, m, Cc.data_ptr(), p, Dc.data_ptr(), Uc.data_ptr(), G, R, _ptr(scale),
             ids.data_ptr(), y.data_ptr(), max(y.stride(0), p), _ptr(hidden), ws.data_ptr(), need, st))
@@ -181,7 +190,7 @@ def adapted_project_backward_device(dY, X, Ct, down, up, ids, hidden, *, scale=N
     Uc = _operand("up", up, (G, R, p), compute, prepared)
     if out is not None:
         d_down, d_up = _strided("out[0]", out[0], (G, R, m), torch.float32), _strided("out[1]", out[1], (G, R, p), torch.float32)
-    dev, cur = _check_device(X, dY, Ct, down, up, ids, hidden, scale, *(out or ()))
+    dev = _check_device(X, dY, Ct, down, up, ids, hidden, scale, *(out or ()))
     Xc, Yc = _rows(X, compute), _rows(dY, compute)
     if out is None:
         d_down = torch.empty(G, R, m, dtype=torch.float32, device=dev)
@@ -191,7 +200,7 @@ def adapted_project_backward_device(dY, X, Ct, down, up, ids, hidden, *, scale=N
     what = nat.RP_ADAPT_GRADIENTS if dX is None else nat.RP_ADAPT_GRADIENTS_DX
     need = _workspace_bytes(code, n, m, p, G, R, what)
     ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
-    st = _on_stream(stream, cur, (Xc, Yc, Tc, Dc, Uc, ids, hidden, scale, dX, d_down, d_up, ws))
+    st = _on_stream(stream, dev, (Xc, Yc, Tc, Dc, Uc, ids, hidden, scale, dX, d_down, d_up, ws))
     row = lambda t: max(t.stride(1), t.shape[2])  # noqa: E731
     adapter = lambda t: max(t.stride(0), row(t) * R)  # noqa: E731
     nat.check(lib.rp_adapt_gradients_device(

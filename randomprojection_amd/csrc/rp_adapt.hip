@@ -339,6 +339,16 @@ __device__ __forceinline__ void split3(float x, uint32_t& hi, uint32_t& mid, uin
 __device__ __forceinline__ uint32_t pack_high(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
 __device__ __forceinline__ uint32_t pack_low(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
 
+// 16 bytes that nothing reads again soon, past the caches: they leave the room to what does
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ uint4 load_once(const void* p) {
+    const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
+    return make_uint4(v.x, v.y, v.z, v.w);
+}
+__device__ __forceinline__ void store_once(void* p, uint4 x) {
+    __builtin_nontemporal_store(u32x4{x.x, x.y, x.z, x.w}, reinterpret_cast<u32x4*>(p));
+}
+
 // The factor that the expand reads: `parts` pieces of scale[a] H[i][r] for every row, each of its ranks padded with zeros to 64
 // bytes. bf16: the pieces of split3; f32: the value itself.
 __host__ __device__ __forceinline__ int padded_rank(int R, int size) { return size == 2 ? (R + 31) / 32 * 32 : (R + 15) / 16 * 16; }
@@ -522,7 +532,7 @@ __global__ void __launch_bounds__(256, KT == 1 ? 4 : 2) outer_kernel(OuterArgs a
         for (int j = 0; j < RS; ++j) {
             const int i = i0 + (sizeof(T) == 2 ? q * RS + j : j * 4 + q);
             const int64_t row = list[min(i, rows - 1)];
-            z[j] = *reinterpret_cast<const uint4*>(Z + row * ldz);
+            z[j] = load_once(Z + row * ldz);
 #pragma unroll
             for (int k = 0; k < KT; ++k) h[k][j] = H[row * R + min(r0 + k * 16 + c, R - 1)];
         }
@@ -649,7 +659,7 @@ struct GemmArgs {
     int N, steps;  // stages of 128 bytes of a row
     void* out;
     int64_t ldo;
-    int vec;  // rows of out are 16-byte aligned
+    int vec, stream;  // rows of out are 16-byte aligned; out is larger than the caches
     const char* S;  // the rows' factors (ShrinkArgs)
     const char* W;
     int64_t ldw;    // bytes between ranks
@@ -840,7 +850,8 @@ gemm_kernel(GemmArgs a, Groups o) {
                 if (row >= live || c >= a.N) continue;
                 V* d = out + rows[row] * ldo + c;
                 if (vec && c + E <= a.N) {
-                    *reinterpret_cast<uint4*>(d) = x;
+                    if (a.stream) store_once(d, x);
+                    else *reinterpret_cast<uint4*>(d) = x;
                 } else {
                     V v[E];
                     __builtin_memcpy(v, &x, 16);
@@ -919,83 +930,74 @@ __global__ void __launch_bounds__(256) gemm_join_kernel(GemmArgs a, int wide) {
 
 // ------------------------------------------------------------------------------------------
 // Few rows (up to 64): everything is read once and little is computed, so the contraction is cut over the chip and
-// joined. One launch forms the sums of both products over x, block by block: 32 rows of C by all rows, or 16 KT ranks of one
-// adapter by its rows (16 at a time), over one of `splits` ranges of the contraction; the block's 8 waves take an eighth of the
-// range each and add up in LDS. Bound by reading C and the used adapters' down. The second adds the ranges, in order, and
-// expands: a lane four columns of one row. No sort: the rows of an adapter are found by comparing up to 64 ids.
-constexpr int kFewRows = 64, kFewWaves = 8;
+// joined, and what counts is how much is on its way. One launch forms the sums of both products over x:
+//  * 128 rows of C by all rows over up to 8 lines (128 bytes) of the contraction: the rows' lines go to LDS directly, a line a wave,
+//    each wave loads its 16 rows of C into registers, all at once, and everyone waits once;
+//  * 16 KT ranks of one adapter by its rows (16 at a time) over a range of lines: the 8 waves take an eighth each and add up in LDS.
+// Bound by reading C and the used adapters' down (67 MB at 64 x 16384 -> 1024 with 64 adapters of rank 16). A second launch adds the
+// ranges, in order, and expands: a lane four columns of one row. No sort: the rows of an adapter are found by comparing up to 64 ids.
+constexpr int kFewRows = 64, kFewWaves = 8, kFewLines = 8;
 
 struct FewArgs {
     const char *X, *C, *W;  // W: the bank contracted with x
     int64_t ldx, kp;        // bytes of a row of X, and of C and W
-    int n, p, pp, G, R, splits, c_blocks, r_blocks;
+    int n, p, pp, G, R, c_blocks, c_lines, c_splits, r_blocks, r_splits;
     const int32_t* ids;
-    float *part, *part_h;  // splits x n x pp (p padded to a multiple of 4), splits x n x R
+    float *part, *part_h;  // c_splits x n x pp (p padded to a multiple of 4), r_splits x n x R
 };
 
-template <typename T, int MT, int NT>
-__device__ __forceinline__ void few_sum(const char* (&a)[MT], const char* (&b)[NT], int l0, int l1, f32x4 (*red)[MT * NT][64], f32x4 (&out)[MT * NT]) {
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    f32x4 acc[MT * NT];
-#pragma unroll
-    for (int i = 0; i < MT * NT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const int each = (l1 - l0 + kFewWaves - 1) / kFewWaves, e1 = min(l1, l0 + (w + 1) * each);
-    for (int l = l0 + w * each; l < e1; ++l) {
-        uint4 fa[2][MT], fb[2][NT];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-#pragma unroll
-            for (int i = 0; i < MT; ++i) fa[h][i] = *reinterpret_cast<const uint4*>(a[i] + (int64_t)l * 128 + h * 64);
-#pragma unroll
-            for (int j = 0; j < NT; ++j) fb[h][j] = *reinterpret_cast<const uint4*>(b[j] + (int64_t)l * 128 + h * 64);
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int j = 0; j < NT; ++j) acc[i * NT + j] = mma<T>(fa[h][i], fb[h][j], acc[i * NT + j]);
-    }
-#pragma unroll
-    for (int i = 0; i < MT * NT; ++i) red[w][i][lane] = acc[i];
-    __syncthreads();
-    // tile i of the sum is left with wave i % 8, in out[i / 8]
-#pragma unroll
-    for (int i = 0; i < MT * NT; ++i) {
-        if (i % kFewWaves != w) continue;
-        f32x4 x = red[0][i][lane];
-#pragma unroll
-        for (int k = 1; k < kFewWaves; ++k) x += red[k][i][lane];
-        out[i / kFewWaves] = x;
-    }
-}
-
 template <typename T, int NT, int KT>
-__global__ void __launch_bounds__(64 * kFewWaves) few_sums_kernel(FewArgs a) {
-    constexpr int MT = 2, TILES = MT * NT > KT ? MT * NT : KT;
-    __shared__ f32x4 red[kFewWaves * TILES * 64];
+__global__ void __launch_bounds__(64 * kFewWaves, 4) few_sums_kernel(FewArgs a) {
+    constexpr int XL = 16 * NT * 8;  // chunks of a line of all rows
+    __shared__ uint4 lds[kFewLines * (XL > KT * 64 ? XL : KT * 64)];
     __shared__ int members[17];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, c = lane & 15, q = lane >> 4;
-    const int lines = (int)(a.kp / 128), split = blockIdx.y;
-    const int l0 = (int)((int64_t)lines * split / a.splits), l1 = (int)((int64_t)lines * (split + 1) / a.splits);
-    if ((int)blockIdx.x < a.c_blocks) {
-        const int c0 = blockIdx.x * 32;
-        const char *pa[MT], *pb[NT];
+    const int lines = (int)(a.kp / 128);
+    int id = blockIdx.x;
+    if (id < a.c_blocks * a.c_splits) {
+        const int split = id / a.c_blocks, l0 = split * a.c_lines, count = min(a.c_lines, lines - l0), c0 = id % a.c_blocks * 128 + w * 16;
+        if (w < count) {
+            const uint32_t to = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)reinterpret_cast<uintptr_t>(lds + w * XL));
+            const int r = lane >> 3, ch = (lane & 7) ^ (r & 7);  // chunk ch of row r lies at r * 8 + (ch ^ (r & 7))
 #pragma unroll
-        for (int i = 0; i < MT; ++i) pa[i] = a.C + min(c0 + i * 16 + c, a.p - 1) * a.kp + q * 16;
-#pragma unroll
-        for (int j = 0; j < NT; ++j) pb[j] = a.X + min(j * 16 + c, a.n - 1) * a.ldx + q * 16;
-        f32x4 out[MT * NT];
-        few_sum<T, MT, NT>(pa, pb, l0, l1, reinterpret_cast<f32x4(*)[MT * NT][64]>(red), out);
-#pragma unroll
-        for (int i = 0; i < MT * NT; ++i) {
-            const int row = i % NT * 16 + c, col = c0 + i / NT * 16 + 4 * q;
-            if (i % kFewWaves == w && row < a.n && col < a.pp)
-                *reinterpret_cast<f32x4*>(a.part + ((int64_t)split * a.n + row) * a.pp + col) = out[i / kFewWaves];
+            for (int i = 0; i < 2 * NT; ++i) {
+                const char* from = a.X + min(i * 8 + r, a.n - 1) * a.ldx + (int64_t)(l0 + w) * 128 + ch * 16;
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // m0 is reserved: the clobber keeps the compiler's own uses safe
+                asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(to + (uint32_t)i * 1024u) : "memory", "m0");
+#pragma clang diagnostic pop
+            }
         }
+        const char* pc = a.C + min(c0 + c, a.p - 1) * a.kp + (int64_t)l0 * 128 + q * 16;
+        uint4 f[kFewLines][2];
+#pragma unroll
+        for (int l = 0; l < kFewLines; ++l)
+            if (l < count)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) f[l][h] = *reinterpret_cast<const uint4*>(pc + l * 128 + h * 64);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the wave's line of x has landed too
+        __syncthreads();
+        f32x4 acc[NT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int l = 0; l < kFewLines; ++l) {
+            if (l >= count) break;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+                    acc[j] = mma<T>(f[l][h], lds[l * XL + (j * 16 + c) * 8 + ((4 * h + q) ^ (c & 7))], acc[j]);
+        }
+        const int col = c0 + 4 * q;
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+            if (j * 16 + c < a.n && col < a.pp)
+                *reinterpret_cast<f32x4*>(a.part + ((int64_t)split * a.n + j * 16 + c) * a.pp + col) = acc[j];
         return;
     }
-    const int k = blockIdx.x - a.c_blocks, row = k / a.r_blocks, r0 = k % a.r_blocks * 16 * KT;
+    id -= a.c_blocks * a.c_splits;
+    const int split = id % a.r_splits, k = id / a.r_splits, row = k / a.r_blocks, r0 = k % a.r_blocks * 16 * KT;
     const int g = lane < a.n ? group_of(a.ids[lane], a.G) : a.G, mine = __builtin_amdgcn_readlane(g, row);
     if (mine == a.G) return;
     const uint64_t same = __ballot(g == mine);
@@ -1007,21 +1009,44 @@ __global__ void __launch_bounds__(64 * kFewWaves) few_sums_kernel(FewArgs a) {
     }
     __syncthreads();
     const int count = members[16];
-    const char *pa[KT], *pb[1];
+    const char *pa[KT], *pb = a.X + members[min(c, count - 1)] * a.ldx + q * 16;
 #pragma unroll
     for (int i = 0; i < KT; ++i) pa[i] = a.W + ((int64_t)mine * a.R + min(r0 + i * 16 + c, a.R - 1)) * a.kp + q * 16;
-    pb[0] = a.X + members[min(c, count - 1)] * a.ldx + q * 16;
-    f32x4 out[KT];
-    few_sum<T, KT, 1>(pa, pb, l0, l1, reinterpret_cast<f32x4(*)[KT][64]>(red), out);
+    const int l0 = (int)((int64_t)lines * split / a.r_splits), l1 = (int)((int64_t)lines * (split + 1) / a.r_splits);
+    f32x4 acc[KT];
 #pragma unroll
-    for (int i = 0; i < KT; ++i) {
-        if (i % kFewWaves != w || c >= count) continue;
-        const int r = r0 + i * 16 + 4 * q;
-        float* h = a.part_h + ((int64_t)split * a.n + members[c]) * a.R + r;
+    for (int i = 0; i < KT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const auto add = [&](int l, auto count_of_lines) {
+        constexpr int N = decltype(count_of_lines)::value * 2;  // half lines
+        uint4 fa[N][KT], fb[N];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (r + e < a.R) h[e] = out[i / kFewWaves][e];
-    }
+        for (int h = 0; h < N; ++h) {
+            fb[h] = *reinterpret_cast<const uint4*>(pb + (int64_t)l * 128 + h * 64);
+#pragma unroll
+            for (int i = 0; i < KT; ++i) fa[h][i] = *reinterpret_cast<const uint4*>(pa[i] + (int64_t)l * 128 + h * 64);
+        }
+#pragma unroll
+        for (int h = 0; h < N; ++h)
+#pragma unroll
+            for (int i = 0; i < KT; ++i) acc[i] = mma<T>(fa[h][i], fb[h], acc[i]);
+    };
+    const int each = (l1 - l0 + kFewWaves - 1) / kFewWaves, e1 = min(l1, l0 + (w + 1) * each);
+    int l = l0 + w * each;
+    for (; l + 4 <= e1; l += 4) add(l, std::integral_constant<int, 4>{});
+    for (; l < e1; ++l) add(l, std::integral_constant<int, 1>{});
+    f32x4(*red)[KT][64] = reinterpret_cast<f32x4(*)[KT][64]>(lds);
+#pragma unroll
+    for (int i = 0; i < KT; ++i) red[w][i][lane] = acc[i];
+    __syncthreads();
+    if (w >= KT || c >= count) return;
+    f32x4 x = red[0][w][lane];
+#pragma unroll
+    for (int i = 1; i < kFewWaves; ++i) x += red[i][w][lane];
+    const int r = r0 + w * 16 + 4 * q;
+    float* h = a.part_h + ((int64_t)split * a.n + members[c]) * a.R + r;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (r + e < a.R) h[e] = x[e];
 }
 
 template <typename T, typename O>
@@ -1033,13 +1058,15 @@ few_join_kernel(FewArgs a, const T* __restrict__ up, int64_t wp, const float* __
     const int col = (blockIdx.x * 64 + lane) * 4;
     f32x4 y = f32x4{0.f, 0.f, 0.f, 0.f};
     if (col < a.pp)
-        for (int k = 0; k < a.splits; ++k) y += *reinterpret_cast<const f32x4*>(a.part + ((int64_t)k * a.n + row) * a.pp + col);
+#pragma unroll 8
+        for (int k = 0; k < a.c_splits; ++k) y += *reinterpret_cast<const f32x4*>(a.part + ((int64_t)k * a.n + row) * a.pp + col);
     if (g < a.G || hidden) {
         const float s = g < a.G && scale ? scale[g] : 1.f;
         for (int r = lane; r < a.R; r += 64) {
             float x = 0.f;
             if (g < a.G)
-                for (int k = 0; k < a.splits; ++k) x += a.part_h[((int64_t)k * a.n + row) * a.R + r];
+#pragma unroll 4
+                for (int k = 0; k < a.r_splits; ++k) x += a.part_h[((int64_t)k * a.n + row) * a.R + r];
             h[r] = x * s;
             if (hidden && blockIdx.x == 0) hidden[(int64_t)row * a.R + r] = x;
         }
@@ -1105,14 +1132,22 @@ int check_rows(const char* name, const void* p, int64_t ld, int64_t width, int32
 }
 
 // a product with its expand for few rows: O (n x p) = X C^T + the adapters' part, hidden = the rows' H or NULL (p = 0: H alone)
-int64_t few_splits(int64_t n, int64_t p, int R, int64_t line_bytes) {
-    // about 512 blocks, none with less than two lines a wave
-    const int64_t blocks = std::max<int64_t>(1, (p + 31) / 32 + n * ((R + 31) / 32));
-    return std::max<int64_t>(1, std::min<int64_t>({512 / blocks, line_bytes / 128 / (2 * kFewWaves), 16}));
+struct FewCut {
+    int c_blocks, c_lines, c_splits, r_blocks, r_splits;
+};
+FewCut few_cut(int64_t n, int64_t p, int R, int64_t line_bytes) {
+    FewCut f;
+    const int64_t lines = line_bytes / 128;
+    f.c_blocks = (int)((p + 127) / 128), f.r_blocks = (R + (R <= 16 ? 15 : 31)) / (R <= 16 ? 16 : 32);
+    // 8 lines a block, fewer where that leaves under 256 blocks; an adapter's lines over about 512 blocks, none with less than two a wave
+    f.c_lines = (int)std::max<int64_t>(2, std::min<int64_t>(kFewLines, lines * f.c_blocks / 256));
+    f.c_splits = (int)((lines + f.c_lines - 1) / f.c_lines);
+    f.r_splits = (int)std::max<int64_t>(1, std::min<int64_t>({512 / std::max<int64_t>(1, n * f.r_blocks), lines / (2 * kFewWaves), 16}));
+    return f;
 }
-
 size_t few_bytes(int64_t n, int64_t p, int R, int64_t line_bytes) {
-    return ((size_t)4 * few_splits(n, p, R, line_bytes) * n * ((p + 3) / 4 * 4 + R) + 255) & ~(size_t)255;
+    const FewCut f = few_cut(n, p, R, line_bytes);
+    return ((size_t)4 * n * ((size_t)(p ? f.c_splits : 0) * ((p + 3) / 4 * 4) + (size_t)f.r_splits * R) + 255) & ~(size_t)255;
 }
 
 template <typename T, typename O>
@@ -1122,12 +1157,13 @@ int launch_few(const T* X, int64_t ldx, const T* C, int64_t kp, int64_t n, int64
     FewArgs a{};
     a.X = (const char*)X, a.C = (const char*)C, a.W = (const char*)W, a.ldx = ldx * es, a.kp = kp * es;
     a.n = (int)n, a.p = (int)p, a.pp = (int)((p + 3) / 4 * 4), a.G = G, a.R = R, a.ids = ids;
-    a.splits = (int)few_splits(n, p, R, a.kp);
-    const int kt = R <= 16 ? 1 : 2;
-    a.c_blocks = (int)((p + 31) / 32), a.r_blocks = (R + 16 * kt - 1) / (16 * kt);
-    a.part = (float*)ws, a.part_h = a.part + (int64_t)a.splits * n * a.pp;
-    const dim3 grid((unsigned)(a.c_blocks + n * a.r_blocks), (unsigned)a.splits), block(64 * kFewWaves);
-    const int nt = n <= 16 ? 1 : n <= 32 ? 2 : 4;
+    const FewCut f = few_cut(n, p, R, a.kp);
+    a.c_blocks = f.c_blocks, a.c_lines = f.c_lines, a.c_splits = p ? f.c_splits : 0, a.r_blocks = f.r_blocks, a.r_splits = f.r_splits;
+    a.part = (float*)ws, a.part_h = a.part + (int64_t)a.c_splits * n * a.pp;
+    const int64_t blocks = (int64_t)a.c_blocks * a.c_splits + n * a.r_blocks * a.r_splits;
+    if (blocks >= ((int64_t)1 << 31)) return fail(RP_ERR_UNSUPPORTED, "m or p too large");
+    const dim3 grid((unsigned)blocks), block(64 * kFewWaves);
+    const int kt = R <= 16 ? 1 : 2, nt = n <= 16 ? 1 : n <= 32 ? 2 : 4;
     if (kt == 1) {
         if (nt == 1) hipLaunchKernelGGL((few_sums_kernel<T, 1, 1>), grid, block, 0, st, a);
         else if (nt == 2) hipLaunchKernelGGL((few_sums_kernel<T, 2, 1>), grid, block, 0, st, a);
@@ -1187,7 +1223,7 @@ Plan plan_for(int32_t dtype, int64_t n, int64_t m, int64_t p, int64_t G, int R, 
     const bool many = n >= 512 * 16 * rt;
     l.tile_rows = many ? 16 * rt : 16;
     // chunks of rows for the banks' gradients: long, unless that leaves under 2048 blocks
-    l.chunk_rows = (int)std::max<int64_t>(256, std::min<int64_t>(kMaxChunk, n * ((m + 127) / 128) / 2048 / 64 * 64));
+    l.chunk_rows = (int)std::max<int64_t>(512, std::min<int64_t>(kMaxChunk, n * ((m + 127) / 128) / 2048 / 64 * 64));
     l.small = n <= kSmallRows && G <= 700;
     l.each = 256;
     while ((n + l.each - 1) / l.each * (G + 1) > (1 << 22)) l.each *= 2;
@@ -1351,6 +1387,8 @@ GemmArgs gemm_args(const T* A, int64_t lda, const T* B, int64_t kp, int64_t M, i
     a.A = (const char*)A, a.B = (const char*)B, a.lda = lda * (int64_t)sizeof(T), a.ldb = kp * (int64_t)sizeof(T);
     a.M = M, a.N = (int)N, a.steps = (int)(kp * (int64_t)sizeof(T) / 128), a.out = out, a.ldo = ldo;
     a.vec = !((uintptr_t)out & 15) && ldo * sizeof(O) % 16 == 0;
+    // beyond half of the 256 MB last-level cache: 537 MB of dX written through it cost the next pass's outer products 45 of 156 us
+    a.stream = M * N * (int64_t)sizeof(O) > (128 << 20);
     a.S = S, a.W = (const char*)W, a.ldw = wp * (int64_t)sizeof(T), a.G = G, a.R = R, a.part = (float*)part;
     return a;
 }

@@ -12,6 +12,7 @@ import weakref
 import torch
 
 from . import _native as nat
+from .adapters import raw_stream
 
 __all__ = ["AdamW", "BLOCK"]
 
@@ -92,9 +93,10 @@ class AdamW:
             raise ValueError("lr, eps and weight_decay must not be negative, the betas lie in [0, 1)")
 
     def _stream(self, stream, *tensors):
+        now = raw_stream(self.device.index)
+        if stream is None or stream == now:
+            return now
         cur = torch.cuda.current_stream(self.device)
-        if stream is None or stream == cur.cuda_stream:
-            return cur.cuda_stream
         ext = torch.cuda.ExternalStream(stream, device=self.device)
         ext.wait_stream(cur)
         for t in tensors:

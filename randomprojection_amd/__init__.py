@@ -10,6 +10,9 @@ interfaces:
 * ``Projector`` — R resident in HBM, ``matmul(A)`` == scipy ``A @ R`` (projector.py)
 * ``srp_matrix.sparse_random_matrix`` — sklearn's R generator, bit-identical and vectorised
 * ``driver`` — single-node multi-GPU sharding with one RCCL broadcast of R
+* ``GaussianRandomProjection`` (gaussian.py), the dense projection, and ``AdaptedGaussianProjection``
+  (adapted.py), the same with a learned low-rank adapter for each of many tenants; device-level:
+  ``adapters.adapted_project_device`` and its backward, ``optim.AdamW``
 """
 from . import srp_matrix
 from ._native import NativeUnavailable, RPError
@@ -20,7 +23,7 @@ from .srp_matrix import johnson_lindenstrauss_min_dim
 
 __all__ = [
     "Projector", "get_projector", "random_project_mappartitions_function",
-    "random_project_map_function", "SparseRandomProjection", "SparseVector", "Vectors",
+    "random_project_map_function", "SparseRandomProjection", "AdaptedGaussianProjection", "SparseVector", "Vectors",
     "srp_matrix", "johnson_lindenstrauss_min_dim", "NativeUnavailable", "RPError",
 ]
 __version__ = "0.1.0"
@@ -31,4 +34,8 @@ def __getattr__(name):  # sklearn is imported lazily (the partition path does no
         from .random_projection import SparseRandomProjection
 
         return SparseRandomProjection
+    if name == "AdaptedGaussianProjection":
+        from .adapted import AdaptedGaussianProjection
+
+        return AdaptedGaussianProjection
     raise AttributeError(name)

@@ -158,3 +158,42 @@ def test_workspace_of_every_size():
                     project, gradients, dx = (lib.rp_adapt_workspace_bytes(dtype, n, m, p, G, R, k) for k in (
                         nat.RP_ADAPT_PROJECT, nat.RP_ADAPT_GRADIENTS, nat.RP_ADAPT_GRADIENTS_DX))
                     assert project >= 0 and dx >= gradients >= 4 * n * R
+
+
+def test_estimator_without_a_gpu():
+    """Parameters, shapes, refusals; the components are the base class's for the same random_state."""
+    import pickle
+
+    import numpy as np
+    from sklearn.base import clone
+    from sklearn.exceptions import NotFittedError
+
+    from randomprojection_amd import AdaptedGaussianProjection
+    from randomprojection_amd.gaussian import GaussianRandomProjection
+
+    X = np.random.default_rng(0).standard_normal((20, 33))
+    est = AdaptedGaussianProjection(n_components=7, n_adapters=3, rank=2, random_state=5, compute="bf16", state_bits=8)
+    with pytest.raises(NotFittedError):
+        est.down_
+    with pytest.raises(NotFittedError):
+        est.transform(X, adapters=np.zeros(20, int))
+    assert clone(est).get_params() == est.get_params()
+    est.fit(X)
+    assert np.array_equal(est.components_, GaussianRandomProjection(n_components=7, random_state=5).fit(X).components_)
+    assert est.down_.shape == (3, 2, 33) and est.up_.shape == (3, 2, 7) and not est.up_.any()
+    again = pickle.loads(pickle.dumps(est))
+    assert np.array_equal(again.down_, est.down_) and np.array_equal(clone(est).fit(X).down_, est.down_)
+    for adapters, match in ((np.zeros(19, int), "one whole number"), (np.zeros(20), "one whole number"), (np.full(20, 3), "-1 .. 2"),
+                            (np.full(20, -2), "-1 .. 2")):
+        with pytest.raises(ValueError, match=match):
+            est.transform(X, adapters=adapters)
+        with pytest.raises(ValueError, match=match):
+            est.partial_fit(X, np.zeros((20, 7)), adapters)
+    with pytest.raises(ValueError, match="Y must have shape"):
+        est.partial_fit(X, np.zeros((20, 6)), np.zeros(20, int))
+    for kw, match in (({"rank": 129}, "rank"), ({"rank": 0}, "rank"), ({"n_adapters": 0}, "n_adapters"), ({"compute": "fp64"}, "compute")):
+        with pytest.raises(ValueError, match=match):
+            AdaptedGaussianProjection(n_components=7, **kw).fit(X)
+    if not torch.cuda.is_available():
+        with pytest.raises(RuntimeError, match="MI355X"):
+            est.transform(X, adapters=np.zeros(20, int))

@@ -20,7 +20,7 @@ using namespace rpd;
 
 namespace {
 
-constexpr int kSmallRows = 4096;  // rows that one block groups
+constexpr int kSmallRows = 8192;  // rows that one block groups
 constexpr int kMaxRank = 128, kMaxAdapters = 16383;  // a wave's counts of all groups fit 64 KB of LDS
 
 // rounded to nearest even, two at a time (one instruction); a NaN stays one
@@ -665,12 +665,13 @@ struct GemmArgs {
     int64_t ldw;    // bytes between ranks
     int G, R;
     unsigned m_tiles, n_tiles, splits, per_xcd;
-    float* part;  // splits > 1: partial sums, splits x M x N
+    float* part;  // without the expand: partial sums, splits x M x ldp
+    int64_t ldp;
 };
 
-template <typename T, typename O, int BM, int WM, int WN>
-__global__ void __launch_bounds__(64 * WM * WN, 2)
-gemm_kernel(GemmArgs a, Groups o) {
+// EXPAND: with the adapters' part; else rows are taken as they lie and `o` is not read. lds: 5 slots.
+template <typename T, typename O, int BM, int WM, int WN, bool EXPAND>
+__device__ __forceinline__ void gemm_tile(const GemmArgs& a, const Groups& o, unsigned block, uint4* lds) {
     constexpr int BN = BM, NT = 64 * WM * WN, MT = BM / WM / 16, NN = BN / WN / 16, SL = BM * 8;  // SL: chunks of a slot
     constexpr int PL = BM * 8 / NT;  // loads of a thread for one operand's stage
     // hi, mid and low of H; a result in bf16 does without low (2^-17 of H, against a rounding of 2^-9)
@@ -679,13 +680,12 @@ gemm_kernel(GemmArgs a, Groups o) {
     static_assert(2 * (PARTS * BM * 4 + BN * 4) <= 4 * SL, "adapters take four slots' place");
     static_assert(WM * WN * MT * 16 * 8 <= 4 * SL && NN == 4, "so do the stores, 64 columns a wave");
     static_assert(NT >= BM && BM * 3 <= SL * 4, "a row a thread; the fifth slot holds the tables");
-    __shared__ uint4 lds[5 * SL];
     int32_t* sid = reinterpret_cast<int32_t*>(lds + 4 * SL);  // after the main loop: the tile's rows' groups,
     int32_t* rows = sid + BM;                                 // where they are,
     int32_t* ends = rows + BM;                                // and where in the tile their group ends
     // XCD x (block i runs on XCD i % 8) takes a run of tiles; tiles go down 8 row tiles, then along the columns, so the
     // tiles that run at the same time on an XCD share their rows of A and of B in its L2
-    const unsigned tiles = a.m_tiles * a.n_tiles, id = (blockIdx.x & 7u) * a.per_xcd + (blockIdx.x >> 3);
+    const unsigned tiles = a.m_tiles * a.n_tiles, id = (block & 7u) * a.per_xcd + (block >> 3);
     if (id >= tiles * a.splits) return;
     const unsigned split = id / tiles, t = id % tiles, band = t / (8u * a.n_tiles), in = t % (8u * a.n_tiles);
     const unsigned high = min(8u, a.m_tiles - band * 8u), mt = band * 8u + in % high, nt = in / high;
@@ -693,14 +693,14 @@ gemm_kernel(GemmArgs a, Groups o) {
     const int n0 = (int)nt * BN, live = (int)min((int64_t)BM, a.M - m0);
     const int k0 = (int)((int64_t)a.steps * split / a.splits), steps = (int)((int64_t)a.steps * (split + 1) / a.splits) - k0;
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, wm = w / WN, wn = w % WN, fr = lane & 15, fq = lane >> 4;
-    const int32_t* __restrict__ perm = o.perm + m0;
-    const int first = o.sid[m0], first_end = (int)min((int64_t)live, o.start[first + 1] - m0);
+    const auto row_of = [&](int i) { return EXPAND ? (int64_t)o.perm[m0 + i] : m0 + i; };
+    const int first = EXPAND ? o.sid[m0] : a.G, first_end = EXPAND ? (int)min((int64_t)live, o.start[first + 1] - m0) : 0;
     // 16-byte chunk c of row r of a slot lies at r * 8 + (c ^ (r & 7)): lanes that read one chunk of 16 rows hit all banks
     const int srow = tid >> 3, sxc = (tid & 7) ^ (srow & 7);
     const char* ga[PL];
     const char* gb[PL];
 #pragma unroll
-    for (int i = 0; i < PL; ++i) ga[i] = a.A + perm[min(i * (NT / 8) + srow, live - 1)] * a.lda + sxc * 16 + (int64_t)k0 * 128;
+    for (int i = 0; i < PL; ++i) ga[i] = a.A + row_of(min(i * (NT / 8) + srow, live - 1)) * a.lda + sxc * 16 + (int64_t)k0 * 128;
 #pragma unroll
     for (int i = 0; i < PL; ++i) gb[i] = a.B + min(n0 + i * (NT / 8) + srow, a.N - 1) * a.ldb + sxc * 16 + (int64_t)k0 * 128;
     const uint32_t lds0 = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)reinterpret_cast<uintptr_t>(lds + 64 * w));
@@ -756,11 +756,11 @@ gemm_kernel(GemmArgs a, Groups o) {
     T wx[EW];
     auto F = [](int r) { return (4 - ((r >> 2) & 3)) & 3; };  // chunk c of a row r of 64 bytes lies at r * 4 + (c ^ F(r)): all banks
     const int rp = padded_rank(a.R, sizeof(T));
-    auto fetch = [&](int g, int r0, int buf, auto row_of) {
+    auto fetch = [&](int g, int r0, int buf, auto row_at) {
 #pragma unroll
         for (int i = 0; i < FP; ++i) {
             const int k = i * NT + tid, u = k / (BM * 4), r = (k >> 2) % BM, ch = (k & 3) ^ F(r);
-            to_lds(a.S + (((int64_t)row_of(r) * pieces<T>() + u) * rp + r0) * (int)sizeof(T) + ch * 16, buf * BLOCK + i * NT);
+            to_lds(a.S + (((int64_t)row_at(r) * pieces<T>() + u) * rp + r0) * (int)sizeof(T) + ch * 16, buf * BLOCK + i * NT);
         }
         const char* base = a.W + (int64_t)g * a.R * a.ldw + (int64_t)min(n0 + wi, a.N - 1) * (int)sizeof(T);
 #pragma unroll
@@ -819,13 +819,13 @@ gemm_kernel(GemmArgs a, Groups o) {
     }
     half(fa[0], fb[0], fa[1], fb[1], lds + sa * SL + a1, lds + sb * SL + b1, true, -1, 0, 0);
     meet(false);
-    if (tid < BM) {
+    if (EXPAND && tid < BM) {
         const int i = min(tid, live - 1), g = o.sid[m0 + i];
         sid[tid] = tid < live ? g : a.G;
-        rows[tid] = perm[i];
+        rows[tid] = o.perm[m0 + i];
         ends[tid] = (int)min((int64_t)live, o.start[g + 1] - m0);
     }
-    if (split == 0 && first < a.G) fetch(first, 0, 0, [&](int r) { return perm[min(r, live - 1)]; });
+    if (EXPAND && first < a.G) fetch(first, 0, 0, [&](int r) { return o.perm[m0 + min(r, live - 1)]; });
     half(fa[1], fb[1], fa[0], fb[0], lds, lds, false, -1, 0, 0);
     // 128 bytes of columns of the wave's rows at a time: written to LDS as the lanes hold them, read as rows
     auto store = [&](auto* out, int64_t ldo, bool vec) {
@@ -848,7 +848,7 @@ gemm_kernel(GemmArgs a, Groups o) {
                 const int r = i * 8 + (lane >> 3), row = wm * MT * 16 + r;
                 const uint4 x = *reinterpret_cast<const uint4*>(mine + r * 128 + ((lane & 7) ^ (r & 7)) * 16);
                 if (row >= live || c >= a.N) continue;
-                V* d = out + rows[row] * ldo + c;
+                V* d = out + (EXPAND ? (int64_t)rows[row] : m0 + row) * ldo + c;
                 if (vec && c + E <= a.N) {
                     if (a.stream) store_once(d, x);
                     else *reinterpret_cast<uint4*>(d) = x;
@@ -864,7 +864,7 @@ gemm_kernel(GemmArgs a, Groups o) {
         }
     };
     // the adapters of the tile's rows, one after the other (rows without one come last), KR ranks at a time
-    if (split == 0) {
+    if (EXPAND) {
         int g = first, p0 = 0, p1 = first_end, r0 = 0, buf = 0;
         while (g < a.G) {
             place(r0, buf);
@@ -902,31 +902,16 @@ gemm_kernel(GemmArgs a, Groups o) {
     }
     // lane: row ra + 16 mi, columns rb - fr + 16 ni + 4 fq + e
     __syncthreads();  // the buffers have been read by all
-    if (a.splits > 1) store(a.part + (int64_t)split * a.M * a.N, a.N, !(a.N & 3));
-    else store((O*)a.out, a.ldo, a.vec);
+    if constexpr (EXPAND) store((O*)a.out, a.ldo, a.vec);
+    else store(a.part + (int64_t)split * a.M * a.ldp, a.ldp, true);
 }
 
-// the sum of a product's splits, in order; four columns a thread where rows are a multiple of that
-template <typename O>
-__global__ void __launch_bounds__(256) gemm_join_kernel(GemmArgs a, int wide) {
-    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * wide, all = a.M * a.N;
-    if (i >= all) return;
-    O* d = (O*)a.out + i / a.N * a.ldo + i % a.N;
-    if (wide == 4) {
-        f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-        for (unsigned k = 0; k < a.splits; ++k) s += *reinterpret_cast<const f32x4*>(a.part + k * all + i);
-        if (a.vec) put4(d, s);
-        else
-#pragma unroll
-            for (int e = 0; e < 4; ++e) store_as(d + e, s[e]);
-    } else {
-        float s = 0.f;
-#pragma unroll 8
-        for (unsigned k = 0; k < a.splits; ++k) s += a.part[k * all + i];
-        store_as(d, s);
-    }
+template <typename T, typename O, int BM, int WM, int WN>
+__global__ void __launch_bounds__(64 * WM * WN, 2) gemm_kernel(GemmArgs a, Groups o) {
+    __shared__ uint4 lds[5 * BM * 8];
+    gemm_tile<T, O, BM, WM, WN, true>(a, o, blockIdx.x, lds);
 }
+
 
 // ------------------------------------------------------------------------------------------
 // Few rows (up to 64): everything is read once and little is computed, so the contraction is cut over the chip and
@@ -1054,8 +1039,8 @@ __global__ void __launch_bounds__(64)
 few_join_kernel(FewArgs a, const T* __restrict__ up, int64_t wp, const float* __restrict__ scale, O* __restrict__ Y, int64_t ldy,
                 float* __restrict__ hidden) {
     __shared__ float h[kMaxRank];
-    const int row = blockIdx.y, lane = threadIdx.x, g = group_of(a.ids[row], a.G);
-    const int col = (blockIdx.x * 64 + lane) * 4;
+    const int row = blockIdx.x, lane = threadIdx.x, g = group_of(a.ids[row], a.G);
+    const int col = (blockIdx.y * 64 + lane) * 4;
     f32x4 y = f32x4{0.f, 0.f, 0.f, 0.f};
     if (col < a.pp)
 #pragma unroll 8
@@ -1068,7 +1053,7 @@ few_join_kernel(FewArgs a, const T* __restrict__ up, int64_t wp, const float* __
 #pragma unroll 4
                 for (int k = 0; k < a.r_splits; ++k) x += a.part_h[((int64_t)k * a.n + row) * a.R + r];
             h[r] = x * s;
-            if (hidden && blockIdx.x == 0) hidden[(int64_t)row * a.R + r] = x;
+            if (hidden && blockIdx.y == 0) hidden[(int64_t)row * a.R + r] = x;
         }
     }
     __syncthreads();
@@ -1096,6 +1081,63 @@ few_join_kernel(FewArgs a, const T* __restrict__ up, int64_t wp, const float* __
 #pragma unroll
     for (int e = 0; e < 4; ++e)
         if (col + e < a.p) store_as(d + e, y[e]);
+}
+
+// ------------------------------------------------------------------------------------------
+// Some rows (over 64, but too few tiles for the chip): the product over splits of the contraction and, in blocks of the same launch, the
+// shrink over ranges of it, since neither needs the other; few_join_kernel adds both up and expands.
+template <typename T, int KT>
+__global__ void __launch_bounds__(256, 2) some_sums_kernel(GemmArgs g, ShrinkArgs s, Groups o, float* part_h, int r_blocks, int r_splits, int64_t n) {
+    __shared__ uint4 lds[5 * 128 * 8];
+    const unsigned products = g.per_xcd * 8;
+    if (blockIdx.x < products) {
+        gemm_tile<T, float, 128, 2, 2, false>(g, o, blockIdx.x, lds);
+        return;
+    }
+    const int id = (int)(blockIdx.x - products), split = id % r_splits, k = id / r_splits, r0 = k % r_blocks * 16 * KT;
+    if (k / r_blocks >= o.number[0]) return;
+    const int4 tile = o.tiles[k / r_blocks];
+    if (tile.x == s.G) return;
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, c = lane & 15, q = lane >> 4;
+    const char* z = reinterpret_cast<const char*>((const T*)s.Z + o.perm[tile.y + min(c, tile.z - 1)] * s.ldz) + q * 16;
+    const char* b[KT];
+#pragma unroll
+    for (int j = 0; j < KT; ++j)
+        b[j] = reinterpret_cast<const char*>((const T*)s.W + ((int64_t)tile.x * s.R + min(r0 + j * 16 + c, s.R - 1)) * s.kp) + q * 16;
+    const int lines = (int)(s.kp * (int64_t)sizeof(T) / 128);
+    const int l0 = (int)((int64_t)lines * split / r_splits), l1 = (int)((int64_t)lines * (split + 1) / r_splits), each = (l1 - l0 + 3) / 4;
+    const int e1 = min(l1, l0 + (w + 1) * each);
+    f32x4 acc[KT];
+#pragma unroll
+    for (int j = 0; j < KT; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const auto add = [&](int l, auto count_of_lines) {
+        constexpr int N = decltype(count_of_lines)::value * 2;  // half lines
+        uint4 zf[N], bf[N][KT];
+#pragma unroll
+        for (int h = 0; h < N; ++h) {
+            zf[h] = *reinterpret_cast<const uint4*>(z + (int64_t)l * 128 + h * 64);
+#pragma unroll
+            for (int j = 0; j < KT; ++j) bf[h][j] = *reinterpret_cast<const uint4*>(b[j] + (int64_t)l * 128 + h * 64);
+        }
+#pragma unroll
+        for (int h = 0; h < N; ++h)
+#pragma unroll
+            for (int j = 0; j < KT; ++j) acc[j] = mma<T>(bf[h][j], zf[h], acc[j]);
+    };
+    int l = l0 + w * each;
+    for (; l + 4 <= e1; l += 4) add(l, std::integral_constant<int, 4>{});
+    for (; l < e1; ++l) add(l, std::integral_constant<int, 1>{});
+    f32x4(*red)[KT][64] = reinterpret_cast<f32x4(*)[KT][64]>(lds);
+#pragma unroll
+    for (int j = 0; j < KT; ++j) red[w][j][lane] = acc[j];
+    __syncthreads();
+    if (w >= KT || c >= tile.z) return;
+    const f32x4 x = red[0][w][lane] + red[1][w][lane] + red[2][w][lane] + red[3][w][lane];
+    const int r = r0 + w * 16 + 4 * q;
+    float* h = part_h + (split * n + o.perm[tile.y + c]) * s.R + r;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (r + e < s.R) h[e] = x[e];
 }
 
 int64_t padded(int64_t w, int32_t dtype) {
@@ -1174,7 +1216,7 @@ int launch_few(const T* X, int64_t ldx, const T* C, int64_t kp, int64_t n, int64
         else hipLaunchKernelGGL((few_sums_kernel<T, 4, 2>), grid, block, 0, st, a);
     }
     HIP_TRY(hipGetLastError());
-    hipLaunchKernelGGL((few_join_kernel<T, O>), dim3((unsigned)std::max<int64_t>(1, (p + 255) / 256), (unsigned)n), dim3(64), 0, st, a, U, wp, scale, out, ldo,
+    hipLaunchKernelGGL((few_join_kernel<T, O>), dim3((unsigned)n, (unsigned)std::max<int64_t>(1, (p + 255) / 256)), dim3(64), 0, st, a, U, wp, scale, out, ldo,
                        hidden);
     HIP_TRY(hipGetLastError());
     return RP_OK;
@@ -1184,26 +1226,43 @@ int launch_few(const T* X, int64_t ldx, const T* C, int64_t kp, int64_t n, int64
 struct Plan {
     int bits, tile_rows, chunk_rows, kt;  // kt: shrink's rank tiles (1, 2, 4 or 8)
     bool small;                                  // one block groups the rows
+    bool some;                                   // too few tiles for the chip (Tiling::few)
     int64_t each;                                // else rows of a wave that counts
     int n_chunks;
     int64_t max_tiles, max_chunks, max_parts;
     size_t perm, sid, start, tiles, chunks, tile0, chunk0, multi0, number, hist, pieces, t, part, shrink, pad_x, pad_dy, bytes;
 };
 
-// split of a product over the contraction: enough blocks for 256 CUs with two each, where there are few tiles, as long as a split has
-// 8 stages (1 KB of a row)
+// Tiles of a product: 256 x 256 where that makes 192 of them (three quarters of the chip), else 128 x 128, two on a compute unit; under
+// 128 of these (`few`), the contraction is split for about 512 blocks, each with 8 stages in bf16 and 2 in f32, whose matrix
+// instructions take 16 times as long, and the adapters' part is left to the join.
 struct Tiling {
-    bool big;
+    bool big, few;
     unsigned m_tiles, n_tiles, splits;
 };
-Tiling tiling(int64_t M, int64_t N, int64_t steps) {
+Tiling tiling(int64_t M, int64_t N, int64_t row_bytes, int es) {
     Tiling t;
     t.big = ((M + 255) / 256) * ((N + 255) / 256) >= 192;
     const int64_t b = t.big ? 256 : 128;
     t.m_tiles = (unsigned)((M + b - 1) / b), t.n_tiles = (unsigned)((N + b - 1) / b);
-    const int64_t tiles = std::max<int64_t>(1, (int64_t)t.m_tiles * t.n_tiles);
-    t.splits = t.big || tiles >= 256 ? 1 : (unsigned)std::max<int64_t>(1, std::min<int64_t>({512 / tiles, steps / 8, 32}));
+    const int64_t tiles = std::max<int64_t>(1, (int64_t)t.m_tiles * t.n_tiles), stages = row_bytes / 128;
+    t.few = !t.big && tiles < 128;
+    t.splits = !t.few ? 1 : (unsigned)std::max<int64_t>(1, std::min<int64_t>({512 / tiles, stages / (es == 2 ? 8 : 2), 16}));
     return t;
+}
+
+// the shrink beside a split product: about 512 blocks, none with less than two lines a wave
+struct SomeCut {
+    int r_blocks, r_splits;
+};
+SomeCut some_cut(int64_t tiles, int R, int64_t row_bytes) {
+    SomeCut c;
+    c.r_blocks = (R + (R <= 16 ? 15 : 31)) / (R <= 16 ? 16 : 32);
+    c.r_splits = (int)std::max<int64_t>(1, std::min<int64_t>({512 / std::max<int64_t>(1, tiles * c.r_blocks), row_bytes / 128 / 8, 16}));
+    return c;
+}
+size_t some_bytes(const Tiling& t, int64_t tiles, int64_t n, int64_t p, int R, int64_t row_bytes) {
+    return (size_t)4 * n * ((size_t)t.splits * ((p + 3) / 4 * 4) + (size_t)some_cut(tiles, R, row_bytes).r_splits * R);
 }
 
 // of the shrink of few rows: about 1024 blocks, none with less than two lines a wave
@@ -1215,7 +1274,7 @@ Plan plan_for(int32_t dtype, int64_t n, int64_t m, int64_t p, int64_t G, int R, 
     Plan l;
     const int es = dtype == RP_BF16 ? 2 : 4;
     const int64_t mk = padded(m, dtype), pk = padded(p, dtype);
-    l.bits = 1;
+    l.bits = 1, l.some = false;
     while ((G >> l.bits) != 0) ++l.bits;
     l.kt = R <= 16 ? 1 : R <= 32 ? 2 : R <= 64 ? 4 : 8;
     const int rt = l.kt <= 4 ? 4 : 2;
@@ -1225,7 +1284,7 @@ Plan plan_for(int32_t dtype, int64_t n, int64_t m, int64_t p, int64_t G, int R, 
     // chunks of rows for the banks' gradients: long, unless that leaves under 2048 blocks
     l.chunk_rows = (int)std::max<int64_t>(512, std::min<int64_t>(kMaxChunk, n * ((m + 127) / 128) / 2048 / 64 * 64));
     l.small = n <= kSmallRows && G <= 700;
-    l.each = 256;
+    l.each = std::max<int64_t>(256, (n / 128 + 63) / 64 * 64);
     while ((n + l.each - 1) / l.each * (G + 1) > (1 << 22)) l.each *= 2;
     l.n_chunks = l.small ? 0 : (int)((n + l.each - 1) / l.each);
     l.max_tiles = n / l.tile_rows + std::min(n, G + 1);
@@ -1246,15 +1305,17 @@ Plan plan_for(int32_t dtype, int64_t n, int64_t m, int64_t p, int64_t G, int R, 
     const size_t factors = (size_t)n * (dtype == RP_BF16 ? 3 : 1) * padded_rank(R, es) * es;
     l.pieces = take(what == RP_ADAPT_GRADIENTS ? 0 : factors);
     if (what == RP_ADAPT_PROJECT) {
-        const Tiling g = tiling(n, p, mk * es / 128);
-        l.part = take(g.splits > 1 ? (size_t)4 * g.splits * n * p : 0);
+        const Tiling g = tiling(n, p, mk * es, es);
+        l.some = g.few;
+        l.part = take(l.some ? some_bytes(g, l.max_tiles, n, p, R, mk * es) : 0);
     } else {
         l.t = take((size_t)4 * n * R);
         size_t part = (size_t)4 * l.max_parts * R * (mk + pk);
-        if (what == RP_ADAPT_GRADIENTS_DX) {
-            const Tiling g = tiling(n, m, pk * es / 128);
-            if (g.splits > 1) part = std::max(part, (size_t)4 * g.splits * n * m);
-        }
+        // with or without dX, t is summed in one order: the banks' gradients are the same bits
+        Tiling g = tiling(n, m, pk * es, es);
+        l.some = g.few;
+        if (what != RP_ADAPT_GRADIENTS_DX) g.splits = 0;
+        if (l.some) part = std::max(part, some_bytes(g, l.max_tiles, n, m, R, pk * es));
         if (n <= kFewRows) part = std::max(part, few_bytes(n, what == RP_ADAPT_GRADIENTS_DX ? m : 0, R, pk * es));
         l.part = take(part);
     }
@@ -1362,21 +1423,21 @@ int launch_outer(const Plan& l, const OuterArgs& a, const OuterArgs& b, const Gr
     return RP_OK;
 }
 
-template <typename T, typename O>
-int launch_gemm(GemmArgs a, const Groups& o, hipStream_t st) {
-    const Tiling t = tiling(a.M, a.N, a.steps);
+int place_tiles(GemmArgs& a, const Tiling& t) {
     a.m_tiles = t.m_tiles, a.n_tiles = t.n_tiles, a.splits = t.splits;
     const uint64_t per = ((uint64_t)t.m_tiles * t.n_tiles * t.splits + 7) / 8;
-    if (per * 8 >= (1ull << 31)) return fail(RP_ERR_UNSUPPORTED, "too many rows for one launch");
+    if (per * 8 >= (1ull << 30)) return fail(RP_ERR_UNSUPPORTED, "too many rows for one launch");
     a.per_xcd = (unsigned)per;
+    return RP_OK;
+}
+
+template <typename T, typename O>
+int launch_gemm(GemmArgs a, const Groups& o, hipStream_t st) {
+    const Tiling t = tiling(a.M, a.N, (int64_t)a.steps * 128, sizeof(T));
+    if (const int rc = place_tiles(a, t)) return rc;
     if (t.big) hipLaunchKernelGGL((gemm_kernel<T, O, 256, 2, 4>), dim3(a.per_xcd * 8), dim3(512), 0, st, a, o);
     else hipLaunchKernelGGL((gemm_kernel<T, O, 128, 2, 2>), dim3(a.per_xcd * 8), dim3(256), 0, st, a, o);
     HIP_TRY(hipGetLastError());
-    if (t.splits > 1) {
-        const int wide = a.N % 4 ? 1 : 4;
-        hipLaunchKernelGGL(gemm_join_kernel<O>, dim3((unsigned)((a.M * a.N / wide + 255) / 256)), dim3(256), 0, st, a, wide);
-        HIP_TRY(hipGetLastError());
-    }
     return RP_OK;
 }
 
@@ -1391,6 +1452,31 @@ GemmArgs gemm_args(const T* A, int64_t lda, const T* B, int64_t kp, int64_t M, i
     a.stream = M * N * (int64_t)sizeof(O) > (128 << 20);
     a.S = S, a.W = (const char*)W, a.ldw = wp * (int64_t)sizeof(T), a.G = G, a.R = R, a.part = (float*)part;
     return a;
+}
+
+// the product and the shrink of some rows in one launch, then the join; H: without the scale, or NULL. p = 0: H alone.
+template <typename T, typename O>
+int launch_some(const Plan& l, const T* X, int64_t ldx, const T* C, int64_t kp, int64_t n, int64_t p, const T* W, const T* U, int64_t wp, int G,
+                int R, const float* scale, const int32_t* ids, const Groups& o, O* out, int64_t ldo, float* H, char* ws, hipStream_t st) {
+    GemmArgs g = gemm_args<T, float>(X, ldx, C, kp, n, p, (float*)nullptr, 0, nullptr, U, wp, G, R, ws);
+    Tiling t = tiling(n, p, kp * (int64_t)sizeof(T), sizeof(T));
+    if (!p) t.splits = 0;
+    if (const int rc = place_tiles(g, t)) return rc;
+    const SomeCut c = some_cut(l.max_tiles, R, kp * (int64_t)sizeof(T));
+    g.ldp = (p + 3) / 4 * 4;
+    float* part_h = g.part + t.splits * n * g.ldp;
+    const ShrinkArgs s{X, ldx, kp, W, G, R, nullptr, nullptr, 0, nullptr, nullptr};
+    const dim3 grid(g.per_xcd * 8 + (unsigned)(l.max_tiles * c.r_blocks * c.r_splits)), block(256);
+    if (R <= 16) hipLaunchKernelGGL((some_sums_kernel<T, 1>), grid, block, 0, st, g, s, o, part_h, c.r_blocks, c.r_splits, n);
+    else hipLaunchKernelGGL((some_sums_kernel<T, 2>), grid, block, 0, st, g, s, o, part_h, c.r_blocks, c.r_splits, n);
+    HIP_TRY(hipGetLastError());
+    FewArgs a{};
+    a.n = (int)n, a.p = (int)p, a.pp = (int)g.ldp, a.G = G, a.R = R, a.ids = ids;
+    a.c_splits = (int)t.splits, a.r_splits = c.r_splits, a.part = g.part, a.part_h = part_h;
+    hipLaunchKernelGGL((few_join_kernel<T, O>), dim3((unsigned)n, (unsigned)std::max<int64_t>(1, (p + 255) / 256)), dim3(64), 0, st, a, U, wp,
+                       scale, out, ldo, H);
+    HIP_TRY(hipGetLastError());
+    return RP_OK;
 }
 
 template <typename T>
@@ -1410,6 +1496,8 @@ int project(const T* X, int64_t ldx, int64_t n, int64_t m, const T* C, int64_t p
     const Groups o = groups_of(l, ws);
     const Pad pad = pad_of(X, ldx, n, m, ws + l.pad_x);
     int rc = launch_groups(l, o, ids, n, G, pad, Pad{}, st);
+    if (!rc && l.some)
+        return launch_some<T, float>(l, X, ldx, C, mk, n, p, down, up, pk, G, R, scale, ids, o, Y, ldy, hidden, ws + l.part, st);
     if (!rc) rc = launch_shrink<T>(l, ShrinkArgs{X, ldx, mk, down, G, R, scale, hidden, 0, ws + l.pieces, (f32x4*)(ws + l.shrink)}, o, st);
     if (!rc) rc = launch_gemm<T, float>(gemm_args<T, float>(X, ldx, C, mk, n, p, Y, ldy, ws + l.pieces, up, pk, G, R, ws + l.part), o, st);
     return rc;
@@ -1434,17 +1522,20 @@ int gradients(const T* dY, int64_t lddy, const T* X, int64_t ldx, int64_t n, int
     float* t = (float*)(ws + l.t);
     const Pad px = pad_of(X, ldx, n, m, ws + l.pad_x), py = pad_of(dY, lddy, n, p, ws + l.pad_dy);
     int rc = launch_groups(l, o, ids, n, G, px, py, st);
-    const bool few = n <= kFewRows;  // then t holds up dy without the scale, which the outer product takes on
+    // with few rows, or some, t holds up dy without the scale, which the outer product takes on
+    const bool few = n <= kFewRows, some = !few && l.some, bare = few || some;
     if (!rc && n && few)
         rc = launch_few<T, T>(dY, lddy, Ct, pk, n, dX ? m : 0, up, down, mk, G, R, scale, ids, dX, lddx, t, ws + l.part, st);
-    if (!rc && !few) rc = launch_shrink<T>(l, ShrinkArgs{dY, lddy, pk, up, G, R, scale, t, 1, dX ? ws + l.pieces : nullptr,
+    if (!rc && some)
+        rc = launch_some<T, T>(l, dY, lddy, Ct, pk, n, dX ? m : 0, up, down, mk, G, R, scale, ids, o, dX, lddx, t, ws + l.part, st);
+    if (!rc && !bare) rc = launch_shrink<T>(l, ShrinkArgs{dY, lddy, pk, up, G, R, scale, t, 1, dX ? ws + l.pieces : nullptr,
                                                                    (f32x4*)(ws + l.shrink)}, o, st);
     if (!rc) {
-        const OuterArgs a = outer_args<T>(X, ldx, mk, m, R, few ? scale : nullptr, t, d_down, ldd, sdd, ws + l.part);
+        const OuterArgs a = outer_args<T>(X, ldx, mk, m, R, bare ? scale : nullptr, t, d_down, ldd, sdd, ws + l.part);
         const OuterArgs b = outer_args<T>(dY, lddy, pk, p, R, scale, hidden, d_up, ldu, sdu, ws + l.part + 4 * l.max_parts * R * mk);
         rc = launch_outer<T>(l, a, b, o, n, G, st);
     }
-    if (!rc && dX && !few)
+    if (!rc && dX && !bare)
         rc = launch_gemm<T, T>(gemm_args<T, T>(dY, lddy, Ct, pk, n, m, dX, lddx, ws + l.pieces, down, mk, G, R, ws + l.part), o, st);
     return rc;
 }

@@ -7,7 +7,7 @@ of any mix of tenants (``adapters.py`` has the products, ``optim.py`` the AdamW 
 from __future__ import annotations
 
 import numpy as np
-from sklearn.utils import check_random_state
+from sklearn.utils import check_array, check_random_state
 from sklearn.utils.validation import check_is_fitted, validate_data
 
 from .gaussian import _STEP, GaussianRandomProjection
@@ -26,6 +26,7 @@ class _Bank:
         from .optim import AdamW
 
         dev, mode, G = torch.device("cuda", est.device), est._mode(), down.shape[0]
+        self.made_for = est._made_for()
         pad = lambda a: torch.nn.functional.pad(torch.as_tensor(a, device=dev), (0, -a.shape[-1] % _STEP[mode]))  # noqa: E731
         C = torch.as_tensor(np.ascontiguousarray(components, dtype=np.float32), device=dev)
         self.p, self.m = components.shape
@@ -33,7 +34,7 @@ class _Bank:
         self.params = pad(down).contiguous(), pad(up).contiguous()
         self.grads = tuple(torch.zeros_like(t) for t in self.params)
         self.low = tuple(t.to(torch.bfloat16) for t in self.params) if mode == "bf16" else self.params
-        self.scale = torch.full((G,), est._scale(), device=dev)
+        self.scale = torch.ones(G, device=dev)
         each = lambda ts: [t[g] for t in ts for g in range(G)]  # noqa: E731
         self.opt = AdamW(each(self.params), each(self.grads), lr=est.learning_rate, betas=est.betas, weight_decay=est.weight_decay,
                          state_bits=est.state_bits, copies=each(self.low) if mode == "bf16" else None, seed=int(est.seed))
@@ -59,7 +60,9 @@ class AdaptedGaussianProjection(GaussianRandomProjection):
     components stay as they are. ``down_`` starts Gaussian with variance 1 / n_features and ``up_`` at zero, so a new adapter changes nothing.
 
     compute: "fp32" (also "auto") or "bf16" for the adapted products, both summed and returned in float32. state_bits: 32 or 8, how the
-    optimizer holds its moments; seed: of the random rounding to 8 bits."""
+    optimizer holds its moments; seed: of the random rounding to 8 bits. What ``set_params`` changes after ``fit`` holds from the next call
+    on, but for the adapters' number, rank and seed, which are as fitted, and ``compute`` and
+    ``state_bits``, which cannot change once a step was taken."""
 
     def __init__(self, n_components="auto", *, n_adapters=1, rank=8, alpha=None, learning_rate=1e-3, betas=(0.9, 0.999),
                  weight_decay=0.0, state_bits=32, seed=0, eps=0.1, compute_inverse_components=False, random_state=None, device=0,
@@ -81,7 +84,11 @@ class AdaptedGaussianProjection(GaussianRandomProjection):
         return "bf16" if self.compute == "bf16" else "fp32"
 
     def _scale(self):
-        return float((self.rank if self.alpha is None else self.alpha) / self.rank)
+        rank = self._down.shape[1]
+        return float((rank if self.alpha is None else self.alpha) / rank)
+
+    def _made_for(self):
+        return self.device, self._mode(), self.state_bits
 
     def fit(self, X, y=None):
         from .adapters import MAX_ADAPTERS, MAX_RANK
@@ -96,16 +103,29 @@ class AdaptedGaussianProjection(GaussianRandomProjection):
             self.random_state).randint(2 ** 31 - 1)))
         self._down = rng.normal(0, m ** -0.5, (self.n_adapters, self.rank, m)).astype(np.float32)
         self._up = np.zeros((self.n_adapters, self.rank, p), np.float32)
-        self._bank, self._state = None, None
+        self._bank, self._state, self._state_of = None, None, None
         return self
 
     def _on_device(self):
         from .gaussian import _torch
 
         _torch()
+        if self._bank is not None and self._bank.made_for != self._made_for():  # another device or compute type since
+            self.__dict__.update(self._held())
         if self._bank is None:
+            if self._state is not None and self._state_of != (self._mode(), self.state_bits):
+                raise ValueError("compute and state_bits cannot change once a step was taken: fit again")
             self._bank = _Bank(self, self.components_, self._down, self._up, self._state)
-        return self._bank
+        bank = self._bank
+        bank.scale.fill_(self._scale())
+        bank.opt.lr, bank.opt.betas, bank.opt.weight_decay = self.learning_rate, tuple(self.betas), self.weight_decay
+        return bank
+
+    def _held(self):
+        """What the bank on the device holds, as the attributes that a new one starts from."""
+        (down, up), state = self._bank.arrays(), self._bank.state()
+        return {"_down": down, "_up": up, "_state": state if state["steps"].any() else None, "_state_of": self._bank.made_for[1:],
+                "_bank": None}
 
     @property
     def down_(self):
@@ -121,8 +141,8 @@ class AdaptedGaussianProjection(GaussianRandomProjection):
         ids = np.asarray(adapters)
         if ids.shape != (n,) or ids.dtype.kind not in "iu":
             raise ValueError(f"adapters must hold one whole number for each of the {n} rows, got {ids.dtype} {ids.shape}")
-        if n and (ids.min() < -1 or ids.max() >= self.n_adapters):
-            raise ValueError(f"adapters must lie in -1 .. {self.n_adapters - 1}")
+        if n and (ids.min() < -1 or ids.max() >= len(self._down)):
+            raise ValueError(f"adapters must lie in -1 .. {len(self._down) - 1}")
         return ids.astype(np.int32)
 
     def _chunks(self, X, ids, mode):
@@ -161,7 +181,7 @@ class AdaptedGaussianProjection(GaussianRandomProjection):
             self.fit(X)
         X = validate_data(self, X, accept_sparse=["csr"], reset=False, dtype=[np.float64, np.float32])
         ids, mode = self._ids(adapters, X.shape[0]), self._mode()
-        Y = np.asarray(Y, dtype=np.float32)
+        Y = check_array(Y, dtype=np.float32)
         if Y.shape != (X.shape[0], self.components_.shape[0]):
             raise ValueError(f"Y must have shape {(X.shape[0], self.components_.shape[0])}, got {Y.shape}")
         import torch
@@ -174,8 +194,8 @@ class AdaptedGaussianProjection(GaussianRandomProjection):
             y, hidden = adapted_project_device(xb, bank.C, *bank.low, ib, return_hidden=True, **kw)
             off = y - target
             adapted_project_backward_device((off * (2.0 / xb.shape[0])).to(xb.dtype), xb, None, *bank.low, ib, hidden, out=grads, **kw)
-            has = torch.zeros(self.n_adapters + 1, dtype=torch.uint8, device=xb.device)
-            has[torch.where(ib < 0, self.n_adapters, ib).long()] = 1
+            has = torch.zeros(len(self._down) + 1, dtype=torch.uint8, device=xb.device)
+            has[ib.long()] = 1  # -1: the entry behind the last
             bank.opt.step(has[:-1].repeat(2))
             self.loss_ = float(off.square().sum(1).mean())
         return self
@@ -183,9 +203,7 @@ class AdaptedGaussianProjection(GaussianRandomProjection):
     def __getstate__(self):
         state = dict(super().__getstate__())
         if state.get("_bank") is not None:  # device memory does not travel: what it holds does
-            state["_down"], state["_up"] = state["_bank"].arrays()
-            state["_state"] = state["_bank"].state()
-            state["_bank"] = None
+            state.update(self._held())
         return state
 
     def __setstate__(self, state):

@@ -141,6 +141,29 @@ def _strided(name, t, shape, dtype):
     return t
 
 
+def _share(a, b):
+    """Whether two tensors, unit column strides or contiguous, hold a byte in common. Rows side by side in one buffer (same row stride,
+    columns apart) do not, though they lie between each other."""
+    if not a.numel() or not b.numel():
+        return False
+    span = lambda t: sum((k - 1) * s for k, s in zip(t.shape, t.stride())) * t.element_size() + t.element_size()  # noqa: E731
+    pa, pb = a.data_ptr(), b.data_ptr()
+    if pa + span(a) <= pb or pb + span(b) <= pa:
+        return False
+    row = a.stride(-2) * a.element_size() if a.dim() > 1 else 0
+    for t in (a, b):
+        if not row or t.dim() < 2 or t.stride(-1) != 1 or any(s * t.element_size() % row for s, k in zip(t.stride()[:-1], t.shape) if k > 1):
+            return True
+    at, wide = (pb - pa) % row, [t.shape[-1] * t.element_size() for t in (a, b)]
+    return at < wide[0] or at + wide[1] > row
+
+
+def _own_memory(name, out, *read):
+    for t in read:
+        if t is not None and _share(out, t):
+            raise ValueError(f"{name} must not share memory with what the call reads or its other output")
+
+
 def adapted_project_device(X, C, down, up, ids, *, scale=None, out=None, compute: str = "fp32", stream=None,
                            prepared: bool = False, return_hidden: bool = False):
     """``X @ C.T`` plus each row's adapter for device tensors X (n x m), C (p x m), down (G x R x m), up (G x R x p) and
@@ -156,7 +179,7 @@ def adapted_project_device(X, C, down, up, ids, *, scale=None, out=None, compute
     Dc = _operand("down", down, (G, R, m), compute, prepared)
     Uc = _operand("up", up, (G, R, p), compute, prepared)
     if out is not None:
-        _strided("out", out, (n, p), torch.float32)
+        _own_memory("out", _strided("out", out, (n, p), torch.float32), X, C, down, up, ids, scale)
     dev = _check_device(X, C, down, up, ids, scale, out)
     Xc = _rows(X, compute)
     y = out if out is not None else torch.empty(n, p, dtype=torch.float32, device=dev)
@@ -190,6 +213,8 @@ def adapted_project_backward_device(dY, X, Ct, down, up, ids, hidden, *, scale=N
     Uc = _operand("up", up, (G, R, p), compute, prepared)
     if out is not None:
         d_down, d_up = _strided("out[0]", out[0], (G, R, m), torch.float32), _strided("out[1]", out[1], (G, R, p), torch.float32)
+        for i, t in enumerate((d_down, d_up)):
+            _own_memory(f"out[{i}]", t, X, dY, Ct, down, up, ids, hidden, scale, d_up if i == 0 else None)
     dev = _check_device(X, dY, Ct, down, up, ids, hidden, scale, *(out or ()))
     Xc, Yc = _rows(X, compute), _rows(dY, compute)
     if out is None:

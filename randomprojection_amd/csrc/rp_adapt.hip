@@ -922,6 +922,8 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm_kernel(GemmArgs a, Group
 // Bound by reading C and the used adapters' down (67 MB at 64 x 16384 -> 1024 with 64 adapters of rank 16). A second launch adds the
 // ranges, in order, and expands: a lane four columns of one row. No sort: the rows of an adapter are found by comparing up to 64 ids.
 constexpr int kFewRows = 64, kFewWaves = 8, kFewLines = 8;
+// of results up to the width that the join's grid (256 columns a block) can cover
+bool few_rows(int64_t n, int64_t width) { return n <= kFewRows && width <= (int64_t)65535 * 256; }
 
 struct FewArgs {
     const char *X, *C, *W;  // W: the bank contracted with x
@@ -1150,7 +1152,7 @@ int check_shared(int32_t dtype, int64_t n, int64_t m, int64_t p, int64_t G, int3
     if (dtype != RP_F32 && dtype != RP_BF16) return fail(RP_ERR_INVALID, "dtype must be RP_F32 or RP_BF16");
     if (n < 0 || m <= 0 || p <= 0 || G <= 0 || R <= 0) return fail(RP_ERR_INVALID, "bad shape");
     if (R > kMaxRank) return fail(RP_ERR_UNSUPPORTED, "rank %d is over %d", (int)R, kMaxRank);
-    if (n > INT32_MAX || m > INT32_MAX - 64 || p > INT32_MAX - 64 || G > kMaxAdapters)
+    if (n > INT32_MAX || m > INT32_MAX - 512 || p > INT32_MAX - 512 || G > kMaxAdapters)
         return fail(RP_ERR_UNSUPPORTED, "n, m, p or the number of adapters too large");
     return RP_OK;
 }
@@ -1316,7 +1318,7 @@ Plan plan_for(int32_t dtype, int64_t n, int64_t m, int64_t p, int64_t G, int R, 
         l.some = g.few;
         if (what != RP_ADAPT_GRADIENTS_DX) g.splits = 0;
         if (l.some) part = std::max(part, some_bytes(g, l.max_tiles, n, m, R, pk * es));
-        if (n <= kFewRows) part = std::max(part, few_bytes(n, what == RP_ADAPT_GRADIENTS_DX ? m : 0, R, pk * es));
+        if (few_rows(n, m)) part = std::max(part, few_bytes(n, what == RP_ADAPT_GRADIENTS_DX ? m : 0, R, pk * es));
         l.part = take(part);
     }
     const int splits = l.tile_rows > 16 ? 1 : shrink_splits(l.max_tiles, (what == RP_ADAPT_PROJECT ? mk : pk) * es);
@@ -1484,7 +1486,7 @@ int project(const T* X, int64_t ldx, int64_t n, int64_t m, const T* C, int64_t p
             const float* scale, const int32_t* ids, float* Y, int64_t ldy, float* hidden, char* ws, hipStream_t st) {
     constexpr int32_t dt = sizeof(T) == 2 ? RP_BF16 : RP_F32;
     const int64_t mk = padded(m, dt), pk = padded(p, dt);
-    if (n <= kFewRows) {
+    if (few_rows(n, p)) {
         if (mk != m) {
             const Pad pad = pad_of(X, ldx, n, m, ws + few_bytes(n, p, R, mk * (int64_t)sizeof(T)));
             hipLaunchKernelGGL(pad_kernel, dim3(pad_blocks(pad, Pad{}, 256)), dim3(256), 0, st, pad, Pad{});
@@ -1523,7 +1525,7 @@ int gradients(const T* dY, int64_t lddy, const T* X, int64_t ldx, int64_t n, int
     const Pad px = pad_of(X, ldx, n, m, ws + l.pad_x), py = pad_of(dY, lddy, n, p, ws + l.pad_dy);
     int rc = launch_groups(l, o, ids, n, G, px, py, st);
     // with few rows, or some, t holds up dy without the scale, which the outer product takes on
-    const bool few = n <= kFewRows, some = !few && l.some, bare = few || some;
+    const bool few = few_rows(n, m), some = !few && l.some, bare = few || some;
     if (!rc && n && few)
         rc = launch_few<T, T>(dY, lddy, Ct, pk, n, dX ? m : 0, up, down, mk, G, R, scale, ids, dX, lddx, t, ws + l.part, st);
     if (!rc && some)
@@ -1547,7 +1549,7 @@ extern "C" {
 int64_t rp_adapt_workspace_bytes(int32_t dtype, int64_t n, int64_t m, int64_t p, int64_t adapters, int32_t rank,
                                  int32_t what) {
     if (check_shared(dtype, n, m, p, adapters, rank)) return -1;
-    if (what == RP_ADAPT_PROJECT && n <= kFewRows) {
+    if (what == RP_ADAPT_PROJECT && few_rows(n, p)) {
         const int64_t row = padded(m, dtype) * (dtype == RP_BF16 ? 2 : 4);
         return (int64_t)few_bytes(n, p, rank, row) + (padded(m, dtype) != m ? n * row : 0);
     }

@@ -21,15 +21,24 @@ _STATES = {32: ("steps", "exp_avg", "exp_avg_sq"),
            8: ("steps", "exp_avg", "exp_avg_root", "exp_avg_scale", "exp_avg_root_scale")}
 
 
-def _overlap(tensors):
-    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in tensors if t.numel())
-    return any(a[1] > b[0] for a, b in zip(spans, spans[1:]))
+def _overlap(written, read):
+    """Whether a written tensor shares memory with any other."""
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), w) for ts, w in ((written, True), (read, False))
+                   for t in ts if t.numel())
+    end = end_written = 0
+    for start, stop, w in spans:
+        if start < (end if w else end_written):
+            return True
+        end = max(end, stop)
+        end_written = max(end_written, stop) if w else end_written
+    return False
 
 
 class AdamW:
     """``AdamW(params, grads)``: params float32, grads (all float32 or all bfloat16) of the same sizes, read at every
     ``step``; copies: bfloat16 tensors of the same sizes that receive the rounded parameters, or None. The tensors are
-    contiguous, on one GPU, and are used in place: their memory must not be exchanged while the optimizer lives.
+    contiguous, on one GPU, and are used in place: their memory must not be exchanged while the optimizer lives, and the optimizer
+    must outlive the graphs that hold its steps.
 
     Per tensor, with t its own step count:
         m = b1 m + (1 - b1) g,   v = b2 v + (1 - b2) g^2
@@ -60,8 +69,8 @@ class AdamW:
                 if t.dtype != dt or t.numel() != params[i].numel() or not t.is_contiguous() or t.device != dev:
                     raise ValueError(f"{name}[{i}] must be a contiguous {dt} tensor of {params[i].numel()} elements on {dev}, "
                                      f"got {t.dtype} {tuple(t.shape)} on {t.device}")
-        if _overlap(params + (copies or [])) or any(_overlap([p, g]) for p, g in zip(params, grads)):
-            raise ValueError("params and copies must not share memory")
+        if _overlap(params + (copies or []), grads):
+            raise ValueError("params and copies must not share memory, nor with a gradient")
         if dev.type != "cuda":
             raise RuntimeError("AdamW needs an MI355X (no CPU fallback)")
         self.params, self.grads, self.copies, self.state_bits, self.seed, self.device = params, grads, copies, state_bits, seed, dev

@@ -197,3 +197,42 @@ def test_estimator_without_a_gpu():
     if not torch.cuda.is_available():
         with pytest.raises(RuntimeError, match="MI355X"):
             est.transform(X, adapters=np.zeros(20, int))
+
+
+def test_outputs_that_share_memory_with_inputs_are_refused():
+    """Columns of one buffer side by side are fine; bytes in common are not."""
+    a = _forward_args(n=5, m=64, p=8)
+    wide = torch.randn(5, 80)
+    for X, out, ok in ((wide[:, :64], wide[:, 64:72], True), (wide[:, 16:], wide[:, 8:16], True), (wide[:, :64], wide[:, 60:68], False),
+                       (wide[:, 16:], wide[:, 9:17], False), (wide[:, :64], wide.view(-1)[:40].view(5, 8), False)):
+        with pytest.raises(RuntimeError if ok else ValueError, match="MI355X" if ok else "share memory"):
+            adapted_project_device(X, a["C"], a["down"], a["up"], a["ids"], out=out)
+    with pytest.raises(ValueError, match="share memory"):
+        adapted_project_device(a["X"], a["C"], a["down"], a["up"], a["ids"], out=a["C"][:5, :8])
+    both = torch.zeros(3, 2, 100)
+    grads = lambda x, y: adapted_project_backward_device(torch.randn(5, 8), a["X"], None, a["down"], a["up"], a["ids"],  # noqa: E731
+                                                         torch.zeros(5, 2), out=(x, y))
+    with pytest.raises(RuntimeError, match="MI355X"):
+        grads(both[..., :64], both[..., 64:72])
+    for x, y in ((both[..., :64], both[..., 63:71]), (a["down"], both[..., :8]), (both[..., :64], a["up"])):
+        with pytest.raises(ValueError, match="share memory"):
+            grads(x, y)
+
+
+def test_adamw_refuses_a_gradient_inside_another_parameter():
+    flat = torch.zeros(20)
+    with pytest.raises(ValueError, match="share memory"):
+        AdamW([flat[:6], flat[6:12]], [flat[12:18], flat[3:9]])
+    with pytest.raises(ValueError, match="share memory"):
+        AdamW([flat[:4]], [torch.zeros(8).view(torch.bfloat16)[:4]], copies=[flat.view(torch.bfloat16)[6:10]])
+    one = torch.zeros(6)
+    with pytest.raises(RuntimeError, match="MI355X"):  # a gradient may serve two parameters
+        AdamW([flat[:6], flat[6:12]], [one, one])
+
+
+def test_workspace_for_more_columns_than_the_join_covers():
+    lib = nat.load()
+    edge = 65535 * 256
+    below, above = (lib.rp_adapt_workspace_bytes(nat.RP_BF16, 2, 64, p, 1, 1, nat.RP_ADAPT_PROJECT) for p in (edge, edge + 1))
+    assert below > 4 * 2 * edge > above > 0  # partial sums for few rows; none beyond
+    assert lib.rp_adapt_workspace_bytes(nat.RP_F32, 1, 2 ** 31 - 100, 8, 1, 1, nat.RP_ADAPT_PROJECT) == -1

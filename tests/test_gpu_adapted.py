@@ -91,3 +91,30 @@ def test_partial_fit(bits, compute):
         other.partial_fit(X, T, ids)
     assert np.array_equal(est.down_, other.down_) and np.array_equal(est.up_, other.up_)
     assert np.array_equal(est.transform(X, adapters=ids), other.transform(X, adapters=ids))
+
+
+def test_parameters_set_after_fit():
+    """They hold from the next call on; what the states' layout depends on is refused once a step was taken."""
+    est, X, ids, rng = make("fp32")
+    T = rng.standard_normal((500, 90)).astype(np.float32)
+    bf = pickle.loads(pickle.dumps(est))
+    first = bf.transform(X, adapters=ids)
+    bf.set_params(compute="bf16")  # no step yet
+    assert not np.array_equal(bf.transform(X, adapters=ids), first) and bf._bank.low[0].dtype == torch.bfloat16
+    est.partial_fit(X, T, ids)
+    down, up = est.down_, est.up_
+    est.set_params(learning_rate=0.0, alpha=0.0, n_adapters=9, rank=2).partial_fit(X, T, ids)
+    assert np.array_equal(est.down_, down) and np.array_equal(est.up_, up)
+    shared = est.transform(X, adapters=np.full(500, -1))
+    assert np.array_equal(est.transform(X, adapters=ids), shared)
+    est.set_params(alpha=9.0)
+    assert not np.array_equal(est.transform(X, adapters=ids)[ids >= 0], shared[ids >= 0])
+    with pytest.raises(ValueError, match="-1 .. 4"):
+        est.transform(X, adapters=np.full(500, 5))
+    for change, back in (({"compute": "bf16"}, {"compute": "fp32"}), ({"state_bits": 8}, {"state_bits": 32})):
+        with pytest.raises(ValueError, match="cannot change"):
+            est.set_params(**change).transform(X, adapters=ids)
+        est.set_params(**back)
+    assert np.array_equal(est.down_, down)
+    with pytest.raises(ValueError, match="NaN"):
+        est.partial_fit(X, np.full_like(T, np.nan), ids)

@@ -264,3 +264,131 @@ def test_many_adapters_and_wide_rows():
     """More adapters than rows in a tile, a row count past a block, far offsets in the banks."""
     t = make(777, 4096, 64, 2000, 3, "bf16", seed=11)
     check(t, "bf16")
+
+
+# with 128 tiles and more the product is one launch of whole contractions, with 192 larger ones of the larger tile; over 8192 rows or 700
+# adapters are grouped by several blocks; from 32768 rows on (16384 over rank 64) the shrink takes more rows at a time
+LARGE = [(2049, 1100, 1150, 7, 40), (3001, 1030, 700, 3, 128), (2050, 4100, 1090, 700, 1), (4100, 2950, 3000, 11, 17), (9001, 200, 2000, 5, 64),
+         (8193, 64, 64, 701, 4), (8192, 100, 130, 700, 2), (33000, 96, 1040, 3, 9), (17000, 72, 1101, 2, 100), (20000, 128, 300, 5000, 2),
+         (300, 70, 65, 16383, 1)]
+
+
+@pytest.mark.parametrize("compute", ["bf16", "fp32"])
+@pytest.mark.parametrize("shape", LARGE)
+def test_large_against_the_formulas(shape, compute):
+    G = shape[3]
+    g = torch.Generator().manual_seed(sum(shape))
+    # runs of rows, as requests have, but for a third of them
+    ids = torch.repeat_interleave(torch.randint(-1, G, (shape[0] // 40 + 1,), generator=g), 40)[:shape[0]]
+    ids = torch.where(torch.rand(shape[0], generator=g) < 0.33, torch.randint(-1, G, (shape[0],), generator=g), ids)
+    check(make(*shape, compute, seed=G, ids=ids), compute, prepared=True)
+
+
+@pytest.mark.parametrize("compute", ["bf16", "fp32"])
+@pytest.mark.parametrize("shape", [(2500, 900, 1001, 5, 6), (4200, 2880, 2999, 4, 20)])
+def test_large_outputs_keep_to_their_rows(shape, compute):
+    """Not finite values stay where they are, and what lies around strided outputs stays, where whole tiles are multiplied too."""
+    from randomprojection_amd.adapters import adapted_project_backward_device, adapted_project_device
+
+    n, m, p, G, R = shape
+    t = make(*shape, compute, seed=7, ids=np.arange(n) % (G + 1) - 1)
+    buf = torch.full((n + 5, p + 9), 7.0, device="cuda")
+
+    def run(t, out=None):
+        Y, h = adapted_project_device(t["X"], t["C"], t["down"], t["up"], t["ids"], scale=t["scale"], compute=compute, return_hidden=True, out=out)
+        return (Y, h, *adapted_project_backward_device(t["dY"], t["X"], t["C"].T, t["down"], t["up"], t["ids"], h, scale=t["scale"],
+                                                       compute=compute))
+
+    clean = run(t)
+    again = run(t, out=buf[2:n + 2, 3:p + 3])
+    assert all(torch.equal(a, b) for a, b in zip(clean, again))
+    buf[2:n + 2, 3:p + 3] = 7
+    assert bool((buf == 7).all())
+    for value in (float("nan"), -float("inf")):
+        u = dict(t, X=t["X"].clone(), dY=t["dY"].clone(), down=t["down"].clone(), up=t["up"].clone())
+        u["X"][0, 33] = value  # no adapter
+        u["dY"][n - 1, 5] = value
+        u["down"][2], u["up"][2] = value, value
+        got = run(u)
+        rows = t["ids"] != 2
+        rows[0] = rows[n - 1] = False
+        for k in range(3):
+            assert torch.equal(got[k][rows], clean[k][rows]), k
+        whole = [g for g in range(G) if g not in (2, int(t["ids"][n - 1]))]
+        for k in (3, 4):
+            assert torch.equal(got[k][whole], clean[k][whole])
+
+
+def test_large_graph_on_another_stream():
+    """A captured forward and backward pass of whole tiles, replayed with other inputs between, while eager calls run beside it."""
+    from randomprojection_amd.adapters import adapted_project_backward_device, adapted_project_device, prepare_bank
+
+    shape = (9000, 1000, 700, 6, 8)
+    t, other = make(*shape, "bf16", seed=2), make(*shape, "bf16", seed=4)
+    ops, Ct = [prepare_bank(t[k], "bf16") for k in ("C", "down", "up")], prepare_bank(t["C"].T, "bf16")
+
+    def run(X, dY, ids):
+        Y, h = adapted_project_device(X, *ops, ids, scale=t["scale"], compute="bf16", prepared=True, return_hidden=True)
+        return (Y, h, *adapted_project_backward_device(dY, X, Ct, *ops[1:], ids, h, scale=t["scale"], compute="bf16", prepared=True))
+
+    want = [run(s["X"], s["dY"], s["ids"]) for s in (t, other)]
+    X, dY, ids = (t[k].clone() for k in ("X", "dY", "ids"))
+    torch.cuda.synchronize()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph):
+        out = run(X, dY, ids)
+    for k in range(4):
+        for name, b in (("X", X), ("dY", dY), ("ids", ids)):
+            b.copy_((t, other)[k % 2][name])
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            graph.replay()
+        beside = run(t["X"], t["dY"], t["ids"])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want[k % 2])) and all(torch.equal(a, b) for a, b in zip(beside, want[0])), k
+
+
+def test_offsets_past_32_bits():
+    """X of 5.2 GB, a bank's row and its gradients by rows and columns drawn from all of them."""
+    from randomprojection_amd.adapters import adapted_project_backward_device, adapted_project_device
+
+    n, m, p, G, R = 40000, 65536, 70, 2, 4
+    g = torch.Generator(device="cuda").manual_seed(1)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda", dtype=torch.bfloat16)  # noqa: E731
+    X, C, down, up, dY = r(n, m), r(p, m), r(G, R, m), r(G, R, p), r(n, p)
+    ids = (torch.arange(n, device="cuda") * 3 // n - 1).int()
+    Y, h = adapted_project_device(X, C, down, up, ids, compute="bf16", return_hidden=True)
+    dX, dd, du = adapted_project_backward_device(dY, X, C.T, down, up, ids, h, compute="bf16")
+    rows = torch.tensor([0, 1, 13333, 16384, 26666, 26667, 32767, 32768, 39998, 39999], device="cuda")
+    cols = torch.tensor([0, 1, 32767, 32768, 65534, 65535], device="cuda")
+    c, d, u = C.double(), down.double(), up.double()
+    for i in rows.tolist():
+        x, y, a = X[i].double(), dY[i].double(), int(ids[i])
+        hid = d[a] @ x if a >= 0 else torch.zeros(R, device="cuda", dtype=torch.double)
+        size_h = d[a].abs() @ x.abs() if a >= 0 else hid
+        near(h[i], hid, size_h, m + 8)
+        near(Y[i], c @ x + (hid @ u[a] if a >= 0 else 0), c.abs() @ x.abs() + (size_h @ u[a].abs() if a >= 0 else 0), m + R + 8)
+        tt = u[a] @ y if a >= 0 else hid
+        size_t = u[a].abs() @ y.abs() if a >= 0 else hid
+        near(dX[i], y @ c + (tt @ d[a] if a >= 0 else 0), y.abs() @ c.abs() + (size_t @ d[a].abs() if a >= 0 else 0), p + R + 8, 2.0 ** -8)
+    for a in range(G):
+        at = ids == a
+        y, x, hid = dY[at].double(), X[at][:, cols].double(), h[at].double()
+        near(dd[a][:, cols], (u[a] @ y.T) @ x, (u[a].abs() @ y.abs().T) @ x.abs(), n + p + 8)
+        near(du[a], hid.T @ y, hid.abs().T @ y.abs(), n + 8)
+
+
+def test_more_columns_than_the_join_covers():
+    """Two rows by 17 million components, C of 2.2 GB."""
+    from randomprojection_amd.adapters import adapted_project_device
+
+    n, m, p = 2, 64, 17_000_000
+    g = torch.Generator(device="cuda").manual_seed(1)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda", dtype=torch.bfloat16)  # noqa: E731
+    X, C, down, up = r(n, m), r(p, m), r(1, 1, m), r(1, 1, p)
+    Y = adapted_project_device(X, C, down, up, torch.tensor([0, -1], dtype=torch.int32, device="cuda"), compute="bf16")
+    for part in (slice(0, 1000), slice(65535 * 256 - 500, 65535 * 256 + 500), slice(p - 1000, p)):
+        x, c, u = X.double(), C[part].double(), up[0, 0, part].double()
+        hid = x[0] @ down[0, 0].double()
+        near(Y[0, part], x[0] @ c.T + hid * u, x[0].abs() @ c.abs().T + x[0].abs() @ down[0, 0].double().abs() * u.abs(), m + 9)
+        near(Y[1, part], x[1] @ c.T, x[1].abs() @ c.abs().T, m + 9)

@@ -116,7 +116,8 @@ class AdamW:
     def step(self, active=None, *, lr=None, stream=None):
         """One step of every tensor, or of those whose entry of ``active`` (a uint8 or bool device tensor, one for each
         tensor) is not zero: the others keep their values, states and step counts. lr: for this step only. Asynchronous on
-        ``stream`` (default: torch's current one); can be captured into a graph, with the numbers of the call."""
+        ``stream`` (default: torch's current one); can be captured into a graph, with the numbers of the call. Steps of one
+        optimizer follow each other: two streams need an event between theirs."""
         lr = self.lr if lr is None else lr
         self._check_numbers(lr)
         if active is not None and (active.dtype not in (torch.uint8, torch.bool) or tuple(active.shape) != (len(self.params),)

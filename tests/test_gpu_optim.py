@@ -331,3 +331,41 @@ def test_projection_gradient_and_step_together():
             want[at] += X[at].double() @ down[g].T @ up[g]
             size[at] += X[at].double().abs() @ down[g].T.abs() @ up[g].abs()
         assert bool(((Y.double() - want).abs() <= (m + R + 8) * 2.0 ** -23 * size).all())
+
+
+@pytest.mark.parametrize("grads", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("more", [[768 * 256 - 321 * 256], [768 * 256 - 321 * 256 + 1], [9000 * 256 + 5], [1] * 244, [1] * 245, [0] * 600])
+def test_longer_lists_step_alike(more, bits, grads):
+    """The first tensors of a list get the same bits whatever follows them, whichever form of the step its length takes; eagerly, with
+    tensors left out, and from a graph."""
+    short, long = make(SIZES, bits, grads), make(SIZES + more, bits, grads)
+    T = len(SIZES)
+    for a, b in zip(long.params[:T] + long.grads[:T], short.params + short.grads):  # drawn after all parameters, the gradients differ
+        a.copy_(b)
+    assert sum(-(-s // 256) for s in SIZES) == 321
+    some = torch.tensor([i % 3 != 1 for i in range(T)] + [i % 2 == 0 for i in range(len(more))], device="cuda")
+    graphs = []
+    for opt in (short, long):
+        active = some[:len(opt.params)].clone()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            opt.step()
+            opt.step(active)
+        graphs.append((opt, graph, active))
+    for k in range(3):
+        for opt, graph, active in graphs:
+            opt.step()
+            opt.step(active)
+            for _ in range(2):
+                graph.replay()
+            for g in opt.grads:
+                g.mul_(-0.5)
+    torch.cuda.synchronize()
+    for a, b in zip(short.params + short.copies, long.params[:T] + long.copies[:T]):
+        assert torch.equal(a, b)
+    for x, y in zip(held(short), held(long)):
+        assert all(np.array_equal(a, b) for a, b in zip(x, y))
+    want = [18 if s else 9 for s in some.tolist()]
+    assert long.state_dict()["steps"].tolist() == want and short.state_dict()["steps"].tolist() == want[:T]

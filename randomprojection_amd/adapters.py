@@ -218,18 +218,19 @@ def adapted_project_backward_device(dY, X, Ct, down, up, ids, hidden, *, scale=N
     dev = _check_device(X, dY, Ct, down, up, ids, hidden, scale, *(out or ()))
     Xc, Yc = _rows(X, compute), _rows(dY, compute)
     if out is None:
-        d_down = torch.empty(G, R, m, dtype=torch.float32, device=dev)
-        d_up = torch.empty(G, R, p, dtype=torch.float32, device=dev)
+        d_down, d_up = (torch.empty(G, R, w, dtype=torch.float32, device=dev) for w in (m, p))
+        strides = m, R * m, p, R * p
+    else:
+        row = lambda t: max(t.stride(1), t.shape[2])  # noqa: E731
+        strides = tuple(x for t in (d_down, d_up) for x in (row(t), max(t.stride(0), row(t) * R)))
     dX = None if Ct is None else torch.empty(n, m, dtype=_dtype(compute), device=dev)
     lib, code = nat.load(), _CODE[compute]
     what = nat.RP_ADAPT_GRADIENTS if dX is None else nat.RP_ADAPT_GRADIENTS_DX
     need = _workspace_bytes(code, n, m, p, G, R, what)
     ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
     st = _on_stream(stream, dev, (Xc, Yc, Tc, Dc, Uc, ids, hidden, scale, dX, d_down, d_up, ws))
-    row = lambda t: max(t.stride(1), t.shape[2])  # noqa: E731
-    adapter = lambda t: max(t.stride(0), row(t) * R)  # noqa: E731
     nat.check(lib.rp_adapt_gradients_device(
         dev.index, Yc.data_ptr(), _ld(Yc), Xc.data_ptr(), _ld(Xc), code, n, m, p, _ptr(Tc) if n else None, Dc.data_ptr(),
         Uc.data_ptr(), G, R, _ptr(scale), ids.data_ptr(), hidden.data_ptr(), _ptr(dX) if n else None, m, d_down.data_ptr(),
-        row(d_down), adapter(d_down), d_up.data_ptr(), row(d_up), adapter(d_up), ws.data_ptr(), need, st))
+        *strides[:2], d_up.data_ptr(), *strides[2:], ws.data_ptr(), need, st))
     return dX, d_down, d_up

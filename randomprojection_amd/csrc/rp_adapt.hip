@@ -162,23 +162,31 @@ struct Pad {
     int64_t ld, rows;
     int width, padded, size;  // size: bytes of an element
 };
-__device__ __forceinline__ void pad_rows(const Pad& p, int64_t block, int64_t blocks) {
-    if (!p.to) return;
-    const int each = p.padded <= 256 ? 64 : p.padded <= 1024 ? 256 : blockDim.x;  // threads of a row
-    const int per = blockDim.x / each, lane = threadIdx.x % each;
+constexpr int pad_threads(int64_t chunks, int threads) { return chunks <= 64 ? 64 : chunks <= 256 ? 256 : threads; }  // of a row
+// 16 bytes a thread, loaded from wherever they begin: an element at a time 255 MB of bf16 took 303 us
+template <typename T>
+__device__ __forceinline__ void pad_rows_of(const Pad& p, int64_t block, int64_t blocks) {
+    constexpr int E = 16 / (int)sizeof(T);
+    const int chunks = p.padded / E, each = pad_threads(chunks, blockDim.x), per = blockDim.x / each, lane = threadIdx.x % each;
     for (int64_t r = block * per + threadIdx.x / each; r < p.rows; r += blocks * per) {
-        if (p.size == 2) {
-            const uint16_t* from = (const uint16_t*)p.from + r * p.ld;
-            uint16_t* to = (uint16_t*)p.to + r * p.padded;
-#pragma unroll 4
-            for (int c = lane; c < p.padded; c += each) to[c] = c < p.width ? from[c] : (uint16_t)0;
-        } else {
-            const float* from = (const float*)p.from + r * p.ld;
-            float* to = (float*)p.to + r * p.padded;
-#pragma unroll 4
-            for (int c = lane; c < p.padded; c += each) to[c] = c < p.width ? from[c] : 0.f;
+        const T* from = (const T*)p.from + r * p.ld;
+        uint4* to = (uint4*)((T*)p.to + r * p.padded);
+        for (int c = lane; c < chunks; c += each) {
+            T x[E];
+            if ((c + 1) * E <= p.width) {
+                __builtin_memcpy(x, from + c * E, 16);
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; ++e) x[e] = c * E + e < p.width ? from[c * E + e] : T(0);
+            }
+            __builtin_memcpy(to + c, x, 16);
         }
     }
+}
+__device__ __forceinline__ void pad_rows(const Pad& p, int64_t block, int64_t blocks) {
+    if (!p.to) return;
+    if (p.size == 2) pad_rows_of<uint16_t>(p, block, blocks);
+    else pad_rows_of<float>(p, block, blocks);
 }
 __global__ void __launch_bounds__(256) pad_kernel(Pad p, Pad q) {
     pad_rows(p, blockIdx.x, gridDim.x);
@@ -341,8 +349,9 @@ __device__ __forceinline__ uint32_t pack_low(uint32_t a, uint32_t b) { return __
 
 // 16 bytes that nothing reads again soon, past the caches: they leave the room to what does
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4_anywhere __attribute__((ext_vector_type(4), aligned(2)));
 __device__ __forceinline__ uint4 load_once(const void* p) {
-    const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
+    const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4_anywhere*>(p));
     return make_uint4(v.x, v.y, v.z, v.w);
 }
 __device__ __forceinline__ void store_once(void* p, uint4 x) {
@@ -484,14 +493,14 @@ __global__ void __launch_bounds__(64 * KT) shrink_join_kernel(ShrinkArgs a, Grou
 
 // D[g][r][c] (+ partial sums) = (mul ? mul[g] : 1) sum over rows i of adapter g of H[i][r] Z[i][c]. A block takes 16
 // KT ranks by 128 (bf16) or 64 (f32) columns over a chunk of one group's rows, a wave every fourth step of them, its lanes
-// reading 16 bytes of neighbouring columns of each row: no LDS for Z, which is read once (per 16 KT ranks) and bounds the kernel.
+// reading 16 bytes of neighbouring columns of each row, aligned or not: no LDS for Z, which is read once (per 16 KT ranks) and bounds the kernel.
 //   bf16: 32 rows a step, lane (c, q) rows 8 q .. 8 q + 7, columns 8 c .. 8 c + 7: 8 x 8 values turned round in
 //         registers (a byte permutation for two values), so column j of every lane is one matrix operand. H is split exactly
 //         into three bf16.
 //   f32:  4 rows a matrix instruction, lane (c, q) row q, columns 4 c .. 4 c + 3.
 struct OuterArgs {
     const void* Z;
-    int64_t ldz, qp, q;  // qp: readable columns
+    int64_t ldz, qp, q, wide;  // qp: columns of the partial sums' rows; wide: readable ones of Z
     int R;
     const float *mul, *H;
     float* D;
@@ -518,7 +527,10 @@ __global__ void __launch_bounds__(256, KT == 1 ? 4 : 2) outer_kernel(OuterArgs a
     __syncthreads();
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = lane & 15, q = lane >> 4;
     const int64_t col0 = (int64_t)(block - (second ? blocks0 : 0)) * (16 * NC), col = col0 + c * NC;
-    const T* __restrict__ Z = (const T*)a.Z + min(col, a.qp - NC);
+    // a lane whose columns reach past the readable ones takes the last of these: `shift` of them are its neighbour's
+    const int64_t from = min(col, a.wide - NC);
+    const int shift = (int)(col - from);
+    const T* __restrict__ Z = (const T*)a.Z + from;
     const float* __restrict__ H = a.H;
     const int64_t ldz = a.ldz;
     const int r0 = blockIdx.z * 16 * KT, R = a.R;
@@ -596,19 +608,20 @@ __global__ void __launch_bounds__(256, KT == 1 ? 4 : 2) outer_kernel(OuterArgs a
     for (int k = 0; k < KT; ++k) {
         if (k) __syncthreads();
 #pragma unroll
-        for (int j = 0; j < NC; ++j) *reinterpret_cast<f32x4*>(red[w][j][lane]) = acc[k][j];
+        for (int j = 0; j < NC; ++j)
+            if (j >= shift) *reinterpret_cast<f32x4*>(red[w][j - shift][lane]) = acc[k][j];
         __syncthreads();
 #pragma unroll
         for (int i = threadIdx.x; i < 16 * 4 * NC; i += 256) {
             const int quad = i % (4 * NC), rank = i / (4 * NC), r = r0 + k * 16 + rank, j0 = quad * 4 % NC;
-            const int from = (rank >> 2) * 16 + quad * 4 / NC;
+            const int at_lane = (rank >> 2) * 16 + quad * 4 / NC;
             const int64_t at = col0 + quad * 4;
             if (r >= R || at >= a.q) continue;
             f32x4 x;
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                x[e] = (red[0][j0 + e][from][rank & 3] + red[1][j0 + e][from][rank & 3] + red[2][j0 + e][from][rank & 3] +
-                        red[3][j0 + e][from][rank & 3]) * s;
+                x[e] = (red[0][j0 + e][at_lane][rank & 3] + red[1][j0 + e][at_lane][rank & 3] + red[2][j0 + e][at_lane][rank & 3] +
+                        red[3][j0 + e][at_lane][rank & 3]) * s;
             float* d = out + r * ld + at;
             if (a.vec && at + 4 <= a.q) {
                 *reinterpret_cast<f32x4*>(d) = x;
@@ -674,8 +687,8 @@ template <typename T, typename O, int BM, int WM, int WN, bool EXPAND>
 __device__ __forceinline__ void gemm_tile(const GemmArgs& a, const Groups& o, unsigned block, uint4* lds) {
     constexpr int BN = BM, NT = 64 * WM * WN, MT = BM / WM / 16, NN = BN / WN / 16, SL = BM * 8;  // SL: chunks of a slot
     constexpr int PL = BM * 8 / NT;  // loads of a thread for one operand's stage
-    // hi, mid and low of H; a result in bf16 does without low (2^-17 of H, against a rounding of 2^-9)
-    constexpr int PARTS = sizeof(T) == 4 ? 1 : sizeof(O) == 4 ? 3 : 2, KR = 64 / (int)sizeof(T);
+    // hi, mid and low of H, for a result in bf16 too: where the product and the adapters' part cancel, low is not below its rounding
+    constexpr int PARTS = pieces<T>(), KR = 64 / (int)sizeof(T);
     static_assert(PL == 4, "the waits below count four loads an operand");
     static_assert(2 * (PARTS * BM * 4 + BN * 4) <= 4 * SL, "adapters take four slots' place");
     static_assert(WM * WN * MT * 16 * 8 <= 4 * SL && NN == 4, "so do the stores, 64 columns a wave");
@@ -1235,21 +1248,30 @@ struct Plan {
     size_t perm, sid, start, tiles, chunks, tile0, chunk0, multi0, number, hist, pieces, t, part, shrink, pad_x, pad_dy, bytes;
 };
 
-// Tiles of a product: 256 x 256 where that makes 192 of them (three quarters of the chip), else 128 x 128, two on a compute unit; under
-// 128 of these (`few`), the contraction is split for about 512 blocks, each with 8 stages in bf16 and 2 in f32, whose matrix
-// instructions take 16 times as long, and the adapters' part is left to the join.
+// Tiles of a product: 128 x 128, two on a compute unit, or 256 x 256, one. What a round of 256 units takes, in twentieths of a small tile's
+// time beside another: 40 for two small tiles a unit, 25 for one (20 in f32, where the matrix instructions alone bind), 60 for a large
+// one (76). The cheaper kind is taken. Whole calls in us, small and large: bf16, rank 64, from 4096 to 4096: 103 and 129 at 1777 rows, 141
+// and 132 at 2304, 220 and 242 at 5000; f32, rank 8 and 16: 415 and 520 at 3000 x 2000 -> 2900, 2098 and 2010 at 8192 x 4096 -> 4096.
+// Small tiles that leave much of the chip idle are split over the contraction (`few`), for up to 512 blocks of 8 stages and more (2 in
+// f32), and the adapters' part is left to the join: where the part of the time that is idle (0.6 us a stage for a block alone, 1.75 in
+// f32) is more than the partial sums take. Whole and split: 61 and 45 us at 2100 x 4096 -> 1024, 66 and 69 at 3900 rows, 29 and 37 at
+// 3900 x 512, 38 and 28 at 300 x 2000 -> 2900; f32 279 and 43 at 1003 x 4001 -> 200, 94 and 100 at 3900 x 1024 -> 1024.
 struct Tiling {
     bool big, few;
     unsigned m_tiles, n_tiles, splits;
 };
 Tiling tiling(int64_t M, int64_t N, int64_t row_bytes, int es) {
     Tiling t;
-    t.big = ((M + 255) / 256) * ((N + 255) / 256) >= 192;
-    const int64_t b = t.big ? 256 : 128;
+    const auto tiles_of = [&](int64_t b) { return ((M + b - 1) / b) * ((N + b - 1) / b); };
+    const int64_t left = tiles_of(128) % 512;
+    const int64_t small = tiles_of(128) / 512 * 40 + (left > 256 ? 40 : left == 0 ? 0 : es == 2 ? 25 : 20);
+    t.big = (tiles_of(256) + 255) / 256 * (es == 2 ? 60 : 76) < small;
+    const int64_t b = t.big ? 256 : 128, tiles = std::max<int64_t>(1, tiles_of(b)), stages = row_bytes / 128;
     t.m_tiles = (unsigned)((M + b - 1) / b), t.n_tiles = (unsigned)((N + b - 1) / b);
-    const int64_t tiles = std::max<int64_t>(1, (int64_t)t.m_tiles * t.n_tiles), stages = row_bytes / 128;
-    t.few = !t.big && tiles < 128;
-    t.splits = !t.few ? 1 : (unsigned)std::max<int64_t>(1, std::min<int64_t>({512 / tiles, stages / (es == 2 ? 8 : 2), 16}));
+    t.splits = (unsigned)std::max<int64_t>(1, std::min<int64_t>({512 / tiles, stages / (es == 2 ? 8 : 2), 16}));
+    const double idle = 1 - (double)tiles / (es == 2 ? 320 : 256);  // in bf16 two blocks on a unit have 1.25 times the rate of one
+    t.few = !t.big && (double)stages * (es == 2 ? 0.6 : 1.75) * idle > 0.028 * (double)(tiles * t.splits);
+    if (!t.few) t.splits = 1;
     return t;
 }
 
@@ -1276,12 +1298,14 @@ Plan plan_for(int32_t dtype, int64_t n, int64_t m, int64_t p, int64_t G, int R, 
     Plan l;
     const int es = dtype == RP_BF16 ? 2 : 4;
     const int64_t mk = padded(m, dtype), pk = padded(p, dtype);
-    l.bits = 1, l.some = false;
+    l.bits = 1;
     while ((G >> l.bits) != 0) ++l.bits;
     l.kt = R <= 16 ? 1 : R <= 32 ? 2 : R <= 64 ? 4 : 8;
     const int rt = l.kt <= 4 ? 4 : 2;
-    // many rows: as many of them as registers hold under one read of the adapter; few: 16, for more blocks
-    const bool many = n >= 512 * 16 * rt;
+    Tiling g = what == RP_ADAPT_PROJECT ? tiling(n, p, mk * es, es) : tiling(n, m, pk * es, es);
+    l.some = g.few;
+    // many rows: as many of them as registers hold under one read of the adapter; few: 16, for more blocks, and beside a split product
+    const bool many = n >= 512 * 16 * rt && !l.some;
     l.tile_rows = many ? 16 * rt : 16;
     // chunks of rows for the banks' gradients: long, unless that leaves under 2048 blocks
     l.chunk_rows = (int)std::max<int64_t>(512, std::min<int64_t>(kMaxChunk, n * ((m + 127) / 128) / 2048 / 64 * 64));
@@ -1307,15 +1331,11 @@ Plan plan_for(int32_t dtype, int64_t n, int64_t m, int64_t p, int64_t G, int R, 
     const size_t factors = (size_t)n * (dtype == RP_BF16 ? 3 : 1) * padded_rank(R, es) * es;
     l.pieces = take(what == RP_ADAPT_GRADIENTS ? 0 : factors);
     if (what == RP_ADAPT_PROJECT) {
-        const Tiling g = tiling(n, p, mk * es, es);
-        l.some = g.few;
         l.part = take(l.some ? some_bytes(g, l.max_tiles, n, p, R, mk * es) : 0);
     } else {
         l.t = take((size_t)4 * n * R);
         size_t part = (size_t)4 * l.max_parts * R * (mk + pk);
         // with or without dX, t is summed in one order: the banks' gradients are the same bits
-        Tiling g = tiling(n, m, pk * es, es);
-        l.some = g.few;
         if (what != RP_ADAPT_GRADIENTS_DX) g.splits = 0;
         if (l.some) part = std::max(part, some_bytes(g, l.max_tiles, n, m, R, pk * es));
         if (few_rows(n, m)) part = std::max(part, few_bytes(n, what == RP_ADAPT_GRADIENTS_DX ? m : 0, R, pk * es));
@@ -1323,7 +1343,7 @@ Plan plan_for(int32_t dtype, int64_t n, int64_t m, int64_t p, int64_t G, int R, 
     }
     const int splits = l.tile_rows > 16 ? 1 : shrink_splits(l.max_tiles, (what == RP_ADAPT_PROJECT ? mk : pk) * es);
     l.shrink = take(splits > 1 ? (size_t)splits * l.max_tiles * l.kt * 1024 : 0);
-    l.pad_x = take(mk != m ? (size_t)n * mk * es : 0);
+    l.pad_x = take(mk != m && (what == RP_ADAPT_PROJECT || m < 16 / es) ? (size_t)n * mk * es : 0);  // for the gradients only if narrow
     l.pad_dy = take(what != RP_ADAPT_PROJECT && pk != p ? (size_t)n * pk * es : 0);
     l.bytes = at;
     return l;
@@ -1350,7 +1370,7 @@ Pad pad_of(const T*& X, int64_t& ldx, int64_t n, int64_t width, void* to) {
 }
 unsigned pad_blocks(const Pad& p, const Pad& q, int threads) {
     const auto need = [&](const Pad& x) {
-        const int each = x.padded <= 256 ? 64 : x.padded <= 1024 ? 256 : threads;
+        const int each = pad_threads((int64_t)x.padded * x.size / 16, threads);
         return x.to ? (x.rows + threads / each - 1) / (threads / each) : 0;
     };
     return (unsigned)std::min<int64_t>(std::max(need(p), need(q)), 2048);
@@ -1506,9 +1526,9 @@ int project(const T* X, int64_t ldx, int64_t n, int64_t m, const T* C, int64_t p
 }
 
 template <typename T>
-OuterArgs outer_args(const T* Z, int64_t ldz, int64_t qp, int64_t q, int R, const float* mul, const float* H, float* D, int64_t ldd,
+OuterArgs outer_args(const T* Z, int64_t ldz, int64_t qp, int64_t q, int64_t wide, int R, const float* mul, const float* H, float* D, int64_t ldd,
                      int64_t sdd, char* part) {
-    OuterArgs a{Z, ldz, qp, q, R, mul, H, D, ldd, sdd, (float*)part, 0};
+    OuterArgs a{Z, ldz, qp, q, wide, R, mul, H, D, ldd, sdd, (float*)part, 0};
     a.vec = !((uintptr_t)D & 15) && ldd % 4 == 0 && sdd % 4 == 0;
     return a;
 }
@@ -1522,7 +1542,9 @@ int gradients(const T* dY, int64_t lddy, const T* X, int64_t ldx, int64_t n, int
     const Plan l = plan_for(dt, n, m, p, G, R, dX ? RP_ADAPT_GRADIENTS_DX : RP_ADAPT_GRADIENTS);
     const Groups o = groups_of(l, ws);
     float* t = (float*)(ws + l.t);
-    const Pad px = pad_of(X, ldx, n, m, ws + l.pad_x), py = pad_of(dY, lddy, n, p, ws + l.pad_dy);
+    // X goes into the outer product alone, which takes rows of any alignment: 7981 x 15997 in bf16, all
+    // launches: 92 us, 162 with a padded copy
+    const Pad px = m < (int64_t)(16 / sizeof(T)) ? pad_of(X, ldx, n, m, ws + l.pad_x) : Pad{}, py = pad_of(dY, lddy, n, p, ws + l.pad_dy);
     int rc = launch_groups(l, o, ids, n, G, px, py, st);
     // with few rows, or some, t holds up dy without the scale, which the outer product takes on
     const bool few = few_rows(n, m), some = !few && l.some, bare = few || some;
@@ -1533,8 +1555,8 @@ int gradients(const T* dY, int64_t lddy, const T* X, int64_t ldx, int64_t n, int
     if (!rc && !bare) rc = launch_shrink<T>(l, ShrinkArgs{dY, lddy, pk, up, G, R, scale, t, 1, dX ? ws + l.pieces : nullptr,
                                                                    (f32x4*)(ws + l.shrink)}, o, st);
     if (!rc) {
-        const OuterArgs a = outer_args<T>(X, ldx, mk, m, R, bare ? scale : nullptr, t, d_down, ldd, sdd, ws + l.part);
-        const OuterArgs b = outer_args<T>(dY, lddy, pk, p, R, scale, hidden, d_up, ldu, sdu, ws + l.part + 4 * l.max_parts * R * mk);
+        const OuterArgs a = outer_args<T>(X, ldx, mk, m, px.to ? mk : m, R, bare ? scale : nullptr, t, d_down, ldd, sdd, ws + l.part);
+        const OuterArgs b = outer_args<T>(dY, lddy, pk, p, pk, R, scale, hidden, d_up, ldu, sdu, ws + l.part + 4 * l.max_parts * R * mk);
         rc = launch_outer<T>(l, a, b, o, n, G, st);
     }
     if (!rc && dX && !bare)

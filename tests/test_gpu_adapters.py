@@ -392,3 +392,19 @@ def test_more_columns_than_the_join_covers():
         hid = x[0] @ down[0, 0].double()
         near(Y[0, part], x[0] @ c.T + hid * u, x[0].abs() @ c.abs().T + x[0].abs() @ down[0, 0].double().abs() * u.abs(), m + 9)
         near(Y[1, part], x[1] @ c.T, x[1].abs() @ c.abs().T, m + 9)
+
+
+@pytest.mark.parametrize("compute", ["bf16", "fp32"])
+@pytest.mark.parametrize("shape", [(1, 1, 1, 1, 1), (70, 7, 5, 3, 4), (33, 3, 2, 2, 2), (200, 9, 15, 3, 16), (90, 8, 4, 2, 3), (513, 5, 3, 4, 17), (9000, 4, 130, 3, 2),
+                                   (600, 129, 127, 2, 9), (700, 121, 1100, 3, 70), (20000, 15, 9, 5, 3)])
+def test_narrow_and_odd_widths(shape, compute):
+    """Rows shorter than a lane's loads, and rows that end inside one, lying between others that are not numbers."""
+    n, m, p, G, R = shape
+    t = make(*shape, compute, seed=sum(shape))
+    want = check(t, compute)
+    for k, w, left in (("X", m, 3), ("dY", p, 5)):
+        wide = torch.full((n + 1, w + 11), float("nan"), device="cuda", dtype=TYPE[compute])
+        inside = wide.view(-1)[left:left + n * (w + 11)].view(n, w + 11)[:, :w]
+        inside.copy_(t[k])
+        t[k] = inside
+    assert all(torch.equal(a, b) for a, b in zip(check(t, compute), want))

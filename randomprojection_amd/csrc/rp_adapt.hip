@@ -20,7 +20,9 @@ using namespace rpd;
 
 namespace {
 
-constexpr int kSmallRows = 8192;  // rows that one block groups
+// rows that one block groups (up to 700 adapters, whose counts by 16 waves fit its LDS), else three launches: a call of 6225 rows 60 us, 70
+// with three; 16384 rows grouped in 22 us and in 17.5
+constexpr int kSmallRows = 8192;
 constexpr int kMaxRank = 128, kMaxAdapters = 16383;  // a wave's counts of all groups fit 64 KB of LDS
 
 // rounded to nearest even, two at a time (one instruction); a NaN stays one
@@ -41,7 +43,8 @@ struct Groups {
     int32_t* sid;     // sorted position -> group (0 .. G)
     int32_t* start;   // group -> first sorted position; G + 2 entries
     int4* tiles;      // {group, first sorted position, rows, 0}: at most tile_rows rows of one group (G included)
-    int4* chunks;     // {group, first sorted position, rows, its partial sums' number or -1}: at most chunk_rows rows (none where the group has none), group < G
+    int4* chunks;     // {group, first sorted position, rows, its partial sums' number or -1}: at most chunk_rows rows (none where the
+                      // group has none), group < G
     int32_t* tile0;   // group -> its first tile; G + 1 entries
     int32_t* chunk0;  // group -> its first chunk; G + 1 entries
     int32_t* multi0;  // group -> the first of its partial sums, where it has more than one chunk; G + 1 entries
@@ -493,7 +496,8 @@ __global__ void __launch_bounds__(64 * KT) shrink_join_kernel(ShrinkArgs a, Grou
 
 // D[g][r][c] (+ partial sums) = (mul ? mul[g] : 1) sum over rows i of adapter g of H[i][r] Z[i][c]. A block takes 16
 // KT ranks by 128 (bf16) or 64 (f32) columns over a chunk of one group's rows, a wave every fourth step of them, its lanes
-// reading 16 bytes of neighbouring columns of each row, aligned or not: no LDS for Z, which is read once (per 16 KT ranks) and bounds the kernel.
+// reading 16 bytes of neighbouring columns of each row, aligned or not: no LDS for Z, which is read once (per 16 KT ranks) and bounds the kernel
+// (16384 x 16384 and 16384 x 1024 in bf16, rank 16: 0.11 ms, 5.2 TB/s).
 //   bf16: 32 rows a step, lane (c, q) rows 8 q .. 8 q + 7, columns 8 c .. 8 c + 7: 8 x 8 values turned round in
 //         registers (a byte permutation for two values), so column j of every lane is one matrix operand. H is split exactly
 //         into three bf16.
@@ -664,7 +668,11 @@ __global__ void __launch_bounds__(256) outer_join_kernel(OuterArgs a0, OuterArgs
 // After the loop the pieces of the rows' H (exact in three bf16) and the adapter's W take the slots' place, 64 bytes of ranks
 // at a time, and are multiplied into registers of their own, from where only the adapter's rows are added: a value that is
 // not finite in one adapter reaches no other's rows. The result goes through LDS so that rows are stored 128 bytes at a
-// time (16 rows a store otherwise: 0.58 against 0.53 ms at 16384 x 1024 -> 16384 with bf16 out).
+// time (16 rows a store otherwise: a tenth longer at 16384 x 1024 -> 16384 with bf16 out).
+// Measured: 65536 x 16384 -> 1024 1.61 ms with rank 16, 1.37 PFLOP/s, matrix units busy 0.71 of the time; 16384 x 1024 -> 16384 with bf16
+// out 0.60 ms, busy half of it: 16 stages a tile, and a unit holds one tile, whose first loads, adapters (0.05 ms in all) and stores (0.05
+// ms) nothing overlaps. Blocks that go from tile to tile and load the next one's first stage behind the stores need more than the 256
+// registers that a tile of 256 x 256 leaves nothing of: what is spilled made it 0.92 ms.
 struct GemmArgs {
     const char *A, *B;
     int64_t lda, ldb;  // bytes
@@ -932,8 +940,9 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm_kernel(GemmArgs a, Group
 //  * 128 rows of C by all rows over up to 8 lines (128 bytes) of the contraction: the rows' lines go to LDS directly, a line a wave,
 //    each wave loads its 16 rows of C into registers, all at once, and everyone waits once;
 //  * 16 KT ranks of one adapter by its rows (16 at a time) over a range of lines: the 8 waves take an eighth each and add up in LDS.
-// Bound by reading C and the used adapters' down (67 MB at 64 x 16384 -> 1024 with 64 adapters of rank 16). A second launch adds the
-// ranges, in order, and expands: a lane four columns of one row. No sort: the rows of an adapter are found by comparing up to 64 ids.
+// Bound by reading C and the used adapters' down (73 MB at 64 x 16384 -> 1024 with 64 adapters of rank 16: 18 us, 4.1 TB/s). A second launch adds the
+// ranges, in order, and expands: a lane four columns of one row. No sort: the rows of an adapter are found by comparing up to 64 ids, a
+// lane an id. Replayed in a graph, against the launches of more rows: 21 and 26 us there, 10 and 15 us at 16 x 4096 -> 1024.
 constexpr int kFewRows = 64, kFewWaves = 8, kFewLines = 8;
 // of results up to the width that the join's grid (256 columns a block) can cover
 bool few_rows(int64_t n, int64_t width) { return n <= kFewRows && width <= (int64_t)65535 * 256; }
@@ -1252,10 +1261,11 @@ struct Plan {
 // time beside another: 40 for two small tiles a unit, 25 for one (20 in f32, where the matrix instructions alone bind), 60 for a large
 // one (76). The cheaper kind is taken. Whole calls in us, small and large: bf16, rank 64, from 4096 to 4096: 103 and 129 at 1777 rows, 141
 // and 132 at 2304, 220 and 242 at 5000; f32, rank 8 and 16: 415 and 520 at 3000 x 2000 -> 2900, 2098 and 2010 at 8192 x 4096 -> 4096.
-// Small tiles that leave much of the chip idle are split over the contraction (`few`), for up to 512 blocks of 8 stages and more (2 in
-// f32), and the adapters' part is left to the join: where the part of the time that is idle (0.6 us a stage for a block alone, 1.75 in
-// f32) is more than the partial sums take. Whole and split: 61 and 45 us at 2100 x 4096 -> 1024, 66 and 69 at 3900 rows, 29 and 37 at
-// 3900 x 512, 38 and 28 at 300 x 2000 -> 2900; f32 279 and 43 at 1003 x 4001 -> 200, 94 and 100 at 3900 x 1024 -> 1024.
+// Small tiles that leave much of the chip idle are split over the contraction (`few`), for up to 512 blocks of 8 stages and more (256 of
+// 2 in f32, where two on a unit take twice as long: 27 and 31 us of sums at 1003 x 4001 -> 200), and the adapters' part is left to the
+// join: where the part of the time that is idle (0.6 us a stage for a block alone, 1.75 in f32) is more than the partial sums take.
+// Whole and split: 61 and 45 us at 2100 x 4096 -> 1024, 66 and 69 at 3900 rows, 29 and 37 at 3900 x 512, 38 and 28 at 300 x 2000 -> 2900;
+// f32 279 and 40 at 1003 x 4001 -> 200, 94 and 100 at 3900 x 1024 -> 1024.
 struct Tiling {
     bool big, few;
     unsigned m_tiles, n_tiles, splits;
@@ -1268,7 +1278,7 @@ Tiling tiling(int64_t M, int64_t N, int64_t row_bytes, int es) {
     t.big = (tiles_of(256) + 255) / 256 * (es == 2 ? 60 : 76) < small;
     const int64_t b = t.big ? 256 : 128, tiles = std::max<int64_t>(1, tiles_of(b)), stages = row_bytes / 128;
     t.m_tiles = (unsigned)((M + b - 1) / b), t.n_tiles = (unsigned)((N + b - 1) / b);
-    t.splits = (unsigned)std::max<int64_t>(1, std::min<int64_t>({512 / tiles, stages / (es == 2 ? 8 : 2), 16}));
+    t.splits = (unsigned)std::max<int64_t>(1, es == 2 ? std::min<int64_t>({512 / tiles, stages / 8, 16}) : std::min<int64_t>({256 / tiles, stages / 2, 32}));
     const double idle = 1 - (double)tiles / (es == 2 ? 320 : 256);  // in bf16 two blocks on a unit have 1.25 times the rate of one
     t.few = !t.big && (double)stages * (es == 2 ? 0.6 : 1.75) * idle > 0.028 * (double)(tiles * t.splits);
     if (!t.few) t.splits = 1;
@@ -1289,7 +1299,8 @@ size_t some_bytes(const Tiling& t, int64_t tiles, int64_t n, int64_t p, int R, i
     return (size_t)4 * n * ((size_t)t.splits * ((p + 3) / 4 * 4) + (size_t)some_cut(tiles, R, row_bytes).r_splits * R);
 }
 
-// of the shrink of few rows: about 1024 blocks, none with less than two lines a wave
+// of the shrink of few rows: about 1024 blocks, none with less than two lines a wave (whole calls of 1777 x 4096 -> 4096 and 4000 x 16384 ->
+// 1024: 103 and 196 us, 104 and 203 unsplit)
 int shrink_splits(int64_t tiles, int64_t row_bytes) {
     return (int)std::max<int64_t>(1, std::min<int64_t>({1024 / std::max<int64_t>(1, tiles), row_bytes / 128 / 8, 32}));
 }
@@ -1304,10 +1315,12 @@ Plan plan_for(int32_t dtype, int64_t n, int64_t m, int64_t p, int64_t G, int R, 
     const int rt = l.kt <= 4 ? 4 : 2;
     Tiling g = what == RP_ADAPT_PROJECT ? tiling(n, p, mk * es, es) : tiling(n, m, pk * es, es);
     l.some = g.few;
-    // many rows: as many of them as registers hold under one read of the adapter; few: 16, for more blocks, and beside a split product
+    // many rows: as many of them as registers hold under one read of the adapter (65536 x 16384 -> 1024: 2.06 ms, 2.16 with 16); few: 16,
+    // for more blocks (16384 x 4096: 164 us, 172 with 64), and beside a split product, whose blocks take 16
     const bool many = n >= 512 * 16 * rt && !l.some;
     l.tile_rows = many ? 16 * rt : 16;
-    // chunks of rows for the banks' gradients: long, unless that leaves under 2048 blocks
+    // chunks of rows for the banks' gradients: long, unless that leaves under 2048 blocks (16384 x 16384, 16 adapters: the partial sums
+    // joined in 11 us, 17 with 512 rows)
     l.chunk_rows = (int)std::max<int64_t>(512, std::min<int64_t>(kMaxChunk, n * ((m + 127) / 128) / 2048 / 64 * 64));
     l.small = n <= kSmallRows && G <= 700;
     l.each = std::max<int64_t>(256, (n / 128 + 63) / 64 * 64);

@@ -408,3 +408,23 @@ def test_narrow_and_odd_widths(shape, compute):
         inside.copy_(t[k])
         t[k] = inside
     assert all(torch.equal(a, b) for a, b in zip(check(t, compute), want))
+
+
+@pytest.mark.parametrize("n,G", [(300001, 7), (270000, 1000), (100000, 16383), (12289, 701)])
+def test_grouping_of_many_rows(n, G):
+    """Exact whole numbers: each row gets its own adapter's part, each adapter the sum over its own rows."""
+    from randomprojection_amd.adapters import adapted_project_backward_device, adapted_project_device
+
+    g = torch.Generator().manual_seed(n)
+    ids = torch.randint(-2, G + 2, (n,), generator=g, dtype=torch.int32).cuda()
+    X = (torch.arange(n) % 5 - 2).float()[:, None].cuda()
+    a = torch.arange(G, device="cuda").float()[:, None, None]
+    down, up, C = a % 127 + 1, a // 127 + 1, torch.ones(1, 1, device="cuda")
+    Y, h = adapted_project_device(X, C, down, up, ids, return_hidden=True)
+    ok = (ids >= 0) & (ids < G)
+    at = torch.where(ok, ids, 0).long()
+    d, u = torch.where(ok, down[at, 0, 0], 0), torch.where(ok, up[at, 0, 0], 0)
+    assert torch.equal(h, X * d[:, None]) and torch.equal(Y, X + X * (d * u)[:, None])
+    _, dd, du = adapted_project_backward_device(torch.ones_like(Y), X, None, down, up, ids, h)
+    want = torch.zeros(G, dtype=torch.float64, device="cuda").index_add_(0, at, torch.where(ok, X[:, 0], 0).double())
+    assert torch.equal(dd[:, 0, 0].double(), want * up[:, 0, 0]) and torch.equal(du[:, 0, 0].double(), want * down[:, 0, 0])

@@ -165,6 +165,21 @@ struct Pad {
     int64_t ld, rows;
     int width, padded, size;  // size: bytes of an element
 };
+// E elements (16 bytes) of a row from its element c on, zeros behind its end
+template <typename T>
+__device__ __forceinline__ uint4 load_of_row(const T* row, int c, int width) {
+    constexpr int E = 16 / (int)sizeof(T);
+    T x[E];
+    if (c + E <= width) {
+        __builtin_memcpy(x, row + c, 16);
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] = c + e < width ? row[c + e] : T(0);
+    }
+    uint4 y;
+    __builtin_memcpy(&y, x, 16);
+    return y;
+}
 constexpr int pad_threads(int64_t chunks, int threads) { return chunks <= 64 ? 64 : chunks <= 256 ? 256 : threads; }  // of a row
 // 16 bytes a thread, loaded from wherever they begin: an element at a time 255 MB of bf16 took 303 us
 template <typename T>
@@ -174,16 +189,7 @@ __device__ __forceinline__ void pad_rows_of(const Pad& p, int64_t block, int64_t
     for (int64_t r = block * per + threadIdx.x / each; r < p.rows; r += blocks * per) {
         const T* from = (const T*)p.from + r * p.ld;
         uint4* to = (uint4*)((T*)p.to + r * p.padded);
-        for (int c = lane; c < chunks; c += each) {
-            T x[E];
-            if ((c + 1) * E <= p.width) {
-                __builtin_memcpy(x, from + c * E, 16);
-            } else {
-#pragma unroll
-                for (int e = 0; e < E; ++e) x[e] = c * E + e < p.width ? from[c * E + e] : T(0);
-            }
-            __builtin_memcpy(to + c, x, 16);
-        }
+        for (int c = lane; c < chunks; c += each) to[c] = load_of_row(from, c * E, p.width);
     }
 }
 __device__ __forceinline__ void pad_rows(const Pad& p, int64_t block, int64_t blocks) {
@@ -267,6 +273,27 @@ group_small_kernel(const int32_t* __restrict__ ids, int n, int G, int bits, int 
         for (int k = lane; k < nc; k += 64)
             o.chunks[chunk0[h] + k] = make_int4(h, s + k * chunk_rows, min(chunk_rows, rows - k * chunk_rows), nc > 1 ? multi0[h] + k : -1);
     }
+}
+
+// up to 64 rows: a row's place is the number of those before it, a group's first row the number of rows of lower ones. Each adapter has one
+// chunk; there is no list of tiles.
+__device__ __forceinline__ void group_few(const int32_t* __restrict__ ids, int n, int G, int32_t* g, const Groups& o) {
+    const int tid = threadIdx.x;
+    if (tid < 64) g[tid] = tid < n ? group_of(ids[tid], G) : G + 1;
+    __syncthreads();
+    if (tid < n) {
+        int to = 0;
+        for (int i = 0; i < n; ++i) to += g[i] < g[tid] || (g[i] == g[tid] && i < tid);
+        o.perm[to] = tid;
+        o.sid[to] = g[tid];
+    }
+    for (int h = tid; h <= G + 1; h += blockDim.x) {
+        int first = 0, rows = 0;
+        for (int i = 0; i < n; ++i) first += g[i] < h, rows += g[i] == h;
+        o.start[h] = first;
+        if (h < G) o.chunks[h] = make_int4(h, first, rows, -1), o.multi0[h] = 0;
+    }
+    if (tid == 0) o.number[0] = 0, o.number[1] = G;
 }
 
 // many rows: counts of each wave's rows (4 waves a block) to hist[group][chunk]
@@ -962,19 +989,26 @@ bool few_rows(int64_t n, int64_t width) { return n <= kFewRows && width <= (int6
 struct FewArgs {
     const char *X, *C, *W;  // W: the bank contracted with x
     int64_t ldx, kp;        // bytes of a row of X, and of C and W
+    int width;              // of a row of X
     int n, p, pp, G, R, c_blocks, c_lines, c_splits, r_blocks, r_splits;
     const int32_t* ids;
     float *part, *part_h;  // c_splits x n x pp (p padded to a multiple of 4), r_splits x n x R
 };
 
-template <typename T, int NT, int KT>
-__global__ void __launch_bounds__(64 * kFewWaves, 4) few_sums_kernel(FewArgs a) {
-    constexpr int XL = 16 * NT * 8;  // chunks of a line of all rows
+// ODD: rows of X end inside a line, and begin anywhere: they are loaded into registers, without what lies behind their end. One more block
+// groups the rows where the gradients of the banks are to come.
+template <typename T, int NT, int KT, bool ODD>
+__global__ void __launch_bounds__(64 * kFewWaves, 4) few_sums_kernel(FewArgs a, Groups o) {
+    constexpr int XL = 16 * NT * 8, E = 16 / (int)sizeof(T), LE = 128 / (int)sizeof(T);  // chunks of a line of all rows; elements of a chunk, of a line
     __shared__ uint4 lds[kFewLines * (XL > KT * 64 ? XL : KT * 64)];
     __shared__ int members[17];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, c = lane & 15, q = lane >> 4;
     const int lines = (int)(a.kp / 128);
     int id = blockIdx.x;
+    if (id == a.c_blocks * a.c_splits + a.n * a.r_blocks * a.r_splits) {
+        group_few(a.ids, a.n, a.G, reinterpret_cast<int32_t*>(lds), o);
+        return;
+    }
     if (id < a.c_blocks * a.c_splits) {
         const int split = id / a.c_blocks, l0 = split * a.c_lines, count = min(a.c_lines, lines - l0), c0 = id % a.c_blocks * 128 + w * 16;
         if (w < count) {
@@ -982,7 +1016,12 @@ __global__ void __launch_bounds__(64 * kFewWaves, 4) few_sums_kernel(FewArgs a) 
             const int r = lane >> 3, ch = (lane & 7) ^ (r & 7);  // chunk ch of row r lies at r * 8 + (ch ^ (r & 7))
 #pragma unroll
             for (int i = 0; i < 2 * NT; ++i) {
-                const char* from = a.X + min(i * 8 + r, a.n - 1) * a.ldx + (int64_t)(l0 + w) * 128 + ch * 16;
+                const char* row = a.X + min(i * 8 + r, a.n - 1) * a.ldx;
+                if constexpr (ODD) {
+                    lds[w * XL + i * 64 + lane] = load_of_row((const T*)row, (l0 + w) * LE + ch * E, a.width);
+                    continue;
+                }
+                const char* from = row + (int64_t)(l0 + w) * 128 + ch * 16;
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"  // m0 is reserved: the clobber keeps the compiler's own uses safe
                 asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(to + (uint32_t)i * 1024u) : "memory", "m0");
@@ -1030,7 +1069,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, 4) few_sums_kernel(FewArgs a) 
     }
     __syncthreads();
     const int count = members[16];
-    const char *pa[KT], *pb = a.X + members[min(c, count - 1)] * a.ldx + q * 16;
+    const char *pa[KT], *pb = a.X + members[min(c, count - 1)] * a.ldx;
 #pragma unroll
     for (int i = 0; i < KT; ++i) pa[i] = a.W + ((int64_t)mine * a.R + min(r0 + i * 16 + c, a.R - 1)) * a.kp + q * 16;
     const int l0 = (int)((int64_t)lines * split / a.r_splits), l1 = (int)((int64_t)lines * (split + 1) / a.r_splits);
@@ -1042,7 +1081,10 @@ __global__ void __launch_bounds__(64 * kFewWaves, 4) few_sums_kernel(FewArgs a) 
         uint4 fa[N][KT], fb[N];
 #pragma unroll
         for (int h = 0; h < N; ++h) {
-            fb[h] = *reinterpret_cast<const uint4*>(pb + (int64_t)l * 128 + h * 64);
+            // four lines: all inside the row
+            if constexpr (ODD && N == 2) fb[h] = load_of_row((const T*)pb, l * LE + h * 4 * E + q * E, a.width);
+            else if constexpr (ODD) __builtin_memcpy(&fb[h], (const T*)pb + l * LE + h * 4 * E + q * E, 16);
+            else fb[h] = *reinterpret_cast<const uint4*>(pb + (int64_t)l * 128 + h * 64 + q * 16);
 #pragma unroll
             for (int i = 0; i < KT; ++i) fa[h][i] = *reinterpret_cast<const uint4*>(pa[i] + (int64_t)l * 128 + h * 64);
         }
@@ -1053,7 +1095,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, 4) few_sums_kernel(FewArgs a) 
     };
     const int each = (l1 - l0 + kFewWaves - 1) / kFewWaves, e1 = min(l1, l0 + (w + 1) * each);
     int l = l0 + w * each;
-    for (; l + 4 <= e1; l += 4) add(l, std::integral_constant<int, 4>{});
+    for (const int inside = ODD ? min(e1, a.width / LE) : e1; l + 4 <= inside; l += 4) add(l, std::integral_constant<int, 4>{});
     for (; l < e1; ++l) add(l, std::integral_constant<int, 1>{});
     f32x4(*red)[KT][64] = reinterpret_cast<f32x4(*)[KT][64]>(lds);
 #pragma unroll
@@ -1229,28 +1271,30 @@ size_t few_bytes(int64_t n, int64_t p, int R, int64_t line_bytes) {
 }
 
 template <typename T, typename O>
-int launch_few(const T* X, int64_t ldx, const T* C, int64_t kp, int64_t n, int64_t p, const T* W, const T* U, int64_t wp, int G, int R,
-               const float* scale, const int32_t* ids, O* out, int64_t ldo, float* hidden, char* ws, hipStream_t st) {
+int launch_few(const T* X, int64_t ldx, int64_t width, const T* C, int64_t kp, int64_t n, int64_t p, const T* W, const T* U, int64_t wp, int G, int R,
+               const float* scale, const int32_t* ids, const Groups* groups, O* out, int64_t ldo, float* hidden, char* ws, hipStream_t st) {
     constexpr int64_t es = sizeof(T);
     FewArgs a{};
-    a.X = (const char*)X, a.C = (const char*)C, a.W = (const char*)W, a.ldx = ldx * es, a.kp = kp * es;
+    a.X = (const char*)X, a.C = (const char*)C, a.W = (const char*)W, a.ldx = ldx * es, a.kp = kp * es, a.width = (int)width;
     a.n = (int)n, a.p = (int)p, a.pp = (int)((p + 3) / 4 * 4), a.G = G, a.R = R, a.ids = ids;
     const FewCut f = few_cut(n, p, R, a.kp);
     a.c_blocks = f.c_blocks, a.c_lines = f.c_lines, a.c_splits = p ? f.c_splits : 0, a.r_blocks = f.r_blocks, a.r_splits = f.r_splits;
     a.part = (float*)ws, a.part_h = a.part + (int64_t)a.c_splits * n * a.pp;
-    const int64_t blocks = (int64_t)a.c_blocks * a.c_splits + n * a.r_blocks * a.r_splits;
+    const int64_t blocks = (int64_t)a.c_blocks * a.c_splits + n * a.r_blocks * a.r_splits + (groups ? 1 : 0);
+    const Groups o = groups ? *groups : Groups{};
     if (blocks >= ((int64_t)1 << 31)) return fail(RP_ERR_UNSUPPORTED, "m or p too large");
     const dim3 grid((unsigned)blocks), block(64 * kFewWaves);
-    const int kt = R <= 16 ? 1 : 2, nt = n <= 16 ? 1 : n <= 32 ? 2 : 4;
-    if (kt == 1) {
-        if (nt == 1) hipLaunchKernelGGL((few_sums_kernel<T, 1, 1>), grid, block, 0, st, a);
-        else if (nt == 2) hipLaunchKernelGGL((few_sums_kernel<T, 2, 1>), grid, block, 0, st, a);
-        else hipLaunchKernelGGL((few_sums_kernel<T, 4, 1>), grid, block, 0, st, a);
-    } else {
-        if (nt == 1) hipLaunchKernelGGL((few_sums_kernel<T, 1, 2>), grid, block, 0, st, a);
-        else if (nt == 2) hipLaunchKernelGGL((few_sums_kernel<T, 2, 2>), grid, block, 0, st, a);
-        else hipLaunchKernelGGL((few_sums_kernel<T, 4, 2>), grid, block, 0, st, a);
-    }
+    const int nt = n <= 16 ? 1 : n <= 32 ? 2 : 4;
+    const auto launch = [&](auto k_tiles, auto odd) {
+        constexpr int KT = decltype(k_tiles)::value;
+        constexpr bool ODD = decltype(odd)::value;
+        if (nt == 1) hipLaunchKernelGGL((few_sums_kernel<T, 1, KT, ODD>), grid, block, 0, st, a, o);
+        else if (nt == 2) hipLaunchKernelGGL((few_sums_kernel<T, 2, KT, ODD>), grid, block, 0, st, a, o);
+        else hipLaunchKernelGGL((few_sums_kernel<T, 4, KT, ODD>), grid, block, 0, st, a, o);
+    };
+    using std::integral_constant, std::true_type, std::false_type;
+    if (R <= 16) kp == width ? launch(integral_constant<int, 1>{}, false_type{}) : launch(integral_constant<int, 1>{}, true_type{});
+    else kp == width ? launch(integral_constant<int, 2>{}, false_type{}) : launch(integral_constant<int, 2>{}, true_type{});
     HIP_TRY(hipGetLastError());
     hipLaunchKernelGGL((few_join_kernel<T, O>), dim3((unsigned)n, (unsigned)std::max<int64_t>(1, (p + 255) / 256)), dim3(64), 0, st, a, U, wp, scale, out, ldo,
                        hidden);
@@ -1533,14 +1577,8 @@ int project(const T* X, int64_t ldx, int64_t n, int64_t m, const T* C, int64_t p
             const float* scale, const int32_t* ids, float* Y, int64_t ldy, float* hidden, char* ws, hipStream_t st) {
     constexpr int32_t dt = sizeof(T) == 2 ? RP_BF16 : RP_F32;
     const int64_t mk = padded(m, dt), pk = padded(p, dt);
-    if (few_rows(n, p)) {
-        if (mk != m) {
-            const Pad pad = pad_of(X, ldx, n, m, ws + few_bytes(n, p, R, mk * (int64_t)sizeof(T)));
-            hipLaunchKernelGGL(pad_kernel, dim3(pad_blocks(pad, Pad{}, 256)), dim3(256), 0, st, pad, Pad{});
-            HIP_TRY(hipGetLastError());
-        }
-        return launch_few<T, float>(X, ldx, C, mk, n, p, down, up, pk, G, R, scale, ids, Y, ldy, hidden, ws, st);
-    }
+    if (few_rows(n, p))
+        return launch_few<T, float>(X, ldx, m, C, mk, n, p, down, up, pk, G, R, scale, ids, nullptr, Y, ldy, hidden, ws, st);
     const Plan l = plan_for(dt, n, m, p, G, R, RP_ADAPT_PROJECT);
     const Groups o = groups_of(l, ws);
     const Pad pad = pad_of(X, ldx, n, m, ws + l.pad_x);
@@ -1569,21 +1607,31 @@ int gradients(const T* dY, int64_t lddy, const T* X, int64_t ldx, int64_t n, int
     const Plan l = plan_for(dt, n, m, p, G, R, dX ? RP_ADAPT_GRADIENTS_DX : RP_ADAPT_GRADIENTS);
     const Groups o = groups_of(l, ws);
     float* t = (float*)(ws + l.t);
-    // X goes into the outer product alone, which takes rows of any alignment: 7981 x 15997 in bf16, all
-    // launches: 92 us, 162 with a padded copy
-    const Pad px = m < (int64_t)(16 / sizeof(T)) ? pad_of(X, ldx, n, m, ws + l.pad_x) : Pad{}, py = pad_of(dY, lddy, n, p, ws + l.pad_dy);
-    int rc = launch_groups(l, o, ids, n, G, px, py, st);
+    const bool few = n && few_rows(n, m), some = n && !few && l.some, bare = few || some || n == 0;
+    // The outer products take rows of any alignment, and so do the few rows' sums: X is copied only if narrower than a lane's load, dY
+    // for the products of more rows. 7981 x 15997 in bf16, all launches: 92 us, 162 with a padded copy of X.
+    constexpr int64_t lane = 16 / sizeof(T);
+    const Pad px = m < lane ? pad_of(X, ldx, n, m, ws + l.pad_x) : Pad{};
+    const Pad py = p < lane || !few ? pad_of(dY, lddy, n, p, ws + l.pad_dy) : Pad{};
+    const int64_t dy_wide = py.to ? pk : p;
+    int rc = RP_OK;
     // with few rows, or some, t holds up dy without the scale, which the outer product takes on
-    const bool few = few_rows(n, m), some = !few && l.some, bare = few || some;
-    if (!rc && n && few)
-        rc = launch_few<T, T>(dY, lddy, Ct, pk, n, dX ? m : 0, up, down, mk, G, R, scale, ids, dX, lddx, t, ws + l.part, st);
+    if (few) {
+        if (px.to || py.to) {
+            hipLaunchKernelGGL(pad_kernel, dim3(pad_blocks(px, py, 256)), dim3(256), 0, st, px, py);
+            HIP_TRY(hipGetLastError());
+        }
+        rc = launch_few<T, T>(dY, lddy, dy_wide, Ct, pk, n, dX ? m : 0, up, down, mk, G, R, scale, ids, &o, dX, lddx, t, ws + l.part, st);
+    } else {
+        rc = launch_groups(l, o, ids, n, G, px, py, st);
+    }
     if (!rc && some)
         rc = launch_some<T, T>(l, dY, lddy, Ct, pk, n, dX ? m : 0, up, down, mk, G, R, scale, ids, o, dX, lddx, t, ws + l.part, st);
     if (!rc && !bare) rc = launch_shrink<T>(l, ShrinkArgs{dY, lddy, pk, up, G, R, scale, t, 1, dX ? ws + l.pieces : nullptr,
                                                                    (f32x4*)(ws + l.shrink)}, o, st);
     if (!rc) {
         const OuterArgs a = outer_args<T>(X, ldx, mk, m, px.to ? mk : m, R, bare ? scale : nullptr, t, d_down, ldd, sdd, ws + l.part);
-        const OuterArgs b = outer_args<T>(dY, lddy, pk, p, pk, R, scale, hidden, d_up, ldu, sdu, ws + l.part + 4 * l.max_parts * R * mk);
+        const OuterArgs b = outer_args<T>(dY, lddy, pk, p, dy_wide, R, scale, hidden, d_up, ldu, sdu, ws + l.part + 4 * l.max_parts * R * mk);
         rc = launch_outer<T>(l, a, b, o, n, G, st);
     }
     if (!rc && dX && !bare)
@@ -1598,10 +1646,7 @@ extern "C" {
 int64_t rp_adapt_workspace_bytes(int32_t dtype, int64_t n, int64_t m, int64_t p, int64_t adapters, int32_t rank,
                                  int32_t what) {
     if (check_shared(dtype, n, m, p, adapters, rank)) return -1;
-    if (what == RP_ADAPT_PROJECT && few_rows(n, p)) {
-        const int64_t row = padded(m, dtype) * (dtype == RP_BF16 ? 2 : 4);
-        return (int64_t)few_bytes(n, p, rank, row) + (padded(m, dtype) != m ? n * row : 0);
-    }
+    if (what == RP_ADAPT_PROJECT && few_rows(n, p)) return (int64_t)few_bytes(n, p, rank, padded(m, dtype) * (dtype == RP_BF16 ? 2 : 4));
     return (int64_t)plan_for(dtype, n, m, p, adapters, rank, what).bytes;
 }
 

@@ -428,3 +428,39 @@ def test_grouping_of_many_rows(n, G):
     _, dd, du = adapted_project_backward_device(torch.ones_like(Y), X, None, down, up, ids, h)
     want = torch.zeros(G, dtype=torch.float64, device="cuda").index_add_(0, at, torch.where(ok, X[:, 0], 0).double())
     assert torch.equal(dd[:, 0, 0].double(), want * up[:, 0, 0]) and torch.equal(du[:, 0, 0].double(), want * down[:, 0, 0])
+
+
+@pytest.mark.parametrize("compute", ["bf16", "fp32"])
+@pytest.mark.parametrize("G", [1, 3, 800, 16383])
+@pytest.mark.parametrize("n,m,p,R", [(1, 63, 65, 1), (2, 4097, 7, 20), (16, 31, 1029, 16), (17, 127, 129, 3), (33, 2050, 61, 33), (64, 999, 1001, 16)])
+def test_few_odd_rows(n, m, p, R, G, compute):
+    """Up to 64 rows that end inside a line, between others that are not numbers, in every order of their adapters."""
+    if G == 16383 and R > 16:
+        R = 2
+    g = torch.Generator().manual_seed(n + G)
+    ids = torch.randint(-1, min(G, 9), (n,), generator=g) * max(1, (G - 1) // 9)
+    t = make(n, m, p, 1 if G == 1 else G, R, compute, seed=n, ids=ids)
+    for k, w, left in (("X", m, 1), ("dY", p, 3)):
+        wide = torch.full((n + 1, w + 6), float("nan"), device="cuda", dtype=TYPE[compute])
+        inside = wide.view(-1)[left:left + n * (w + 6)].view(n, w + 6)[:, :w]
+        inside.copy_(t[k])
+        t[k] = inside
+    if G <= 3:
+        check(t, compute)
+        return
+    # many adapters: the few that have rows in 64 bits, the others' gradients zero
+    from randomprojection_amd.adapters import adapted_project_backward_device, adapted_project_device
+
+    used = sorted(set(int(i) for i in ids if 0 <= i < G))
+    small = dict(t, down=t["down"][used], up=t["up"][used], scale=t["scale"][used],
+                 ids=torch.tensor([used.index(int(i)) if int(i) in used else -1 for i in ids], dtype=torch.int32, device="cuda"))
+    if not used:
+        return
+    Y, h, dX, dd, du = check(small, compute)
+    Y2, h2 = adapted_project_device(t["X"], t["C"], t["down"], t["up"], t["ids"], scale=t["scale"], compute=compute, return_hidden=True)
+    dX2, dd2, du2 = adapted_project_backward_device(t["dY"], t["X"], t["C"].T, t["down"], t["up"], t["ids"], h2, scale=t["scale"], compute=compute)
+    assert torch.equal(Y, Y2) and torch.equal(h, h2) and torch.equal(dX, dX2)
+    assert torch.equal(dd2[used], dd) and torch.equal(du2[used], du)
+    rest = torch.ones(G, dtype=torch.bool, device="cuda")
+    rest[used] = False
+    assert not dd2[rest].any() and not du2[rest].any()

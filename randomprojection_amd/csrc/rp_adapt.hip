@@ -695,7 +695,7 @@ __global__ void __launch_bounds__(256) outer_join_kernel(OuterArgs a0, OuterArgs
 // ------------------------------------------------------------------------------------------
 // The shared product with the adapters' expand: O[i][c] = sum_k A[i][k] B[c][k] + sum_r (scale[a] H[i][r]) W[a][r][c].
 //
-// B x B tiles, WM x WN waves; rows are taken in the order of the adapters (gathered by the loads, scattered by the
+// BM x BN tiles, WM x WN waves; rows are taken in the order of the adapters (gathered by the loads, scattered by the
 // stores, at no cost), so few tiles hold more than one or two. The main loop stages 128 bytes of every row of A and of B
 // at a time by loads that go to LDS directly. Whole lines: with 64 bytes a stage every line crossed from L2 twice (its other
 // half had left the L1 by the next stage): 1.10 against 1.25 PFLOP/s at 65536 x 16384 -> 1024. A stage is multiplied in two
@@ -730,13 +730,13 @@ struct GemmArgs {
 };
 
 // EXPAND: with the adapters' part; else rows are taken as they lie and `o` is not read. lds: 5 slots.
-template <typename T, typename O, int BM, int WM, int WN, bool EXPAND>
+template <typename T, typename O, int BM, int BN, int WM, int WN, bool EXPAND>
 __device__ __forceinline__ void gemm_tile(const GemmArgs& a, const Groups& o, unsigned block, uint4* lds) {
-    constexpr int BN = BM, NT = 64 * WM * WN, MT = BM / WM / 16, NN = BN / WN / 16, SL = BM * 8;  // SL: chunks of a slot
-    constexpr int PL = BM * 8 / NT;  // loads of a thread for one operand's stage
+    constexpr int NT = 64 * WM * WN, MT = BM / WM / 16, NN = BN / WN / 16, SL = BM * 8;  // SL: chunks of a slot
+    constexpr int PL = BM * 8 / NT, PB = BN * 8 / NT;  // loads of a thread for a stage of A and of B
     // hi, mid and low of H, for a result in bf16 too: where the product and the adapters' part cancel, low is not below its rounding
     constexpr int PARTS = pieces<T>(), KR = 64 / (int)sizeof(T);
-    static_assert(PL == 4, "the waits below count four loads an operand");
+    static_assert(PL == 4 && (PB == 4 || PB == 2), "the waits below count these loads");
     static_assert(2 * (PARTS * BM * 4 + BN * 4) <= 4 * SL, "adapters take four slots' place");
     static_assert(WM * WN * MT * 16 * 8 <= 4 * SL && NN == 4, "so do the stores, 64 columns a wave");
     static_assert(NT >= BM && BM * 3 <= SL * 4, "a row a thread; the fifth slot holds the tables");
@@ -758,11 +758,11 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& a, const Groups& o, un
     // 16-byte chunk c of row r of a slot lies at r * 8 + (c ^ (r & 7)): lanes that read one chunk of 16 rows hit all banks
     const int srow = tid >> 3, sxc = (tid & 7) ^ (srow & 7);
     const char* ga[PL];
-    const char* gb[PL];
+    const char* gb[PB];
 #pragma unroll
     for (int i = 0; i < PL; ++i) ga[i] = a.A + row_of(min(i * (NT / 8) + srow, live - 1)) * a.lda + sxc * 16 + (int64_t)k0 * 128;
 #pragma unroll
-    for (int i = 0; i < PL; ++i) gb[i] = a.B + min(n0 + i * (NT / 8) + srow, a.N - 1) * a.ldb + sxc * 16 + (int64_t)k0 * 128;
+    for (int i = 0; i < PB; ++i) gb[i] = a.B + min(n0 + i * (NT / 8) + srow, a.N - 1) * a.ldb + sxc * 16 + (int64_t)k0 * 128;
     const uint32_t lds0 = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)reinterpret_cast<uintptr_t>(lds + 64 * w));
     // Loads to LDS as inline asm: the compiler does not see what they write, so it puts no wait for all of them before an LDS
     // read; the waits are below. No output register is involved; M0 holds the wave's destination.
@@ -787,7 +787,7 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& a, const Groups& o, un
     // into slot sa; a row of tiles at a time, in this order
     auto half = [&](uint4 (&xa)[MT], uint4 (&xb)[NN], uint4 (&ya)[MT], uint4 (&yb)[NN], const uint4* pa, const uint4* pb, bool rd,
                     int next, int sb, int sa) {
-        constexpr int RD = (MT + NN + MT - 1) / MT, LD = 2 * PL / MT;
+        constexpr int RD = (MT + NN + MT - 1) / MT, LD = (PL + PB) / MT;
 #pragma unroll
         for (int mi = 0; mi < MT; ++mi) {
             if (rd)
@@ -799,8 +799,8 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& a, const Groups& o, un
             if (next >= 0)
 #pragma unroll
                 for (int d = mi * LD; d < (mi + 1) * LD; ++d) {
-                    if (d < PL) load_b(next, d < PL ? d : 0, sb);
-                    else if (next + 1 < steps) load_a(next + 1, d >= PL ? d - PL : 0, sa);
+                    if (d < PB) load_b(next, d < PB ? d : 0, sb);
+                    else if (next + 1 < steps) load_a(next + 1, d >= PB ? d - PB : 0, sa);
                 }
 #pragma unroll
             for (int ni = 0; ni < NN; ++ni) acc[mi][ni] = mma<T>(xb[ni], xa[mi], acc[mi][ni]);
@@ -811,7 +811,8 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& a, const Groups& o, un
     // other adapters' rows come along and are not used) and W into registers, `place` turns it round into LDS. Two blocks lie in LDS,
     // so the next is fetched while one is multiplied, and the first during the last half stage of the main loop.
     constexpr int EW = BN * KR / NT, BLOCK = PARTS * BM * 4 + BN * 4, FP = PARTS * BM * 4 / NT;
-    static_assert(EW * (int)sizeof(T) == 32, "two chunks of W a thread");
+    constexpr int WC = EW * (int)sizeof(T) / 16;  // chunks of W a thread
+    static_assert(WC * 16 == EW * (int)sizeof(T) && (PL + PB) % MT == 0, "whole chunks, whole rows of tiles");
     const int wi = tid % BN, we = __builtin_amdgcn_readfirstlane(tid / BN * EW);
     T wx[EW];
     auto F = [](int r) { return (4 - ((r >> 2) & 3)) & 3; };  // chunk c of a row r of 64 bytes lies at r * 4 + (c ^ F(r)): all banks
@@ -829,7 +830,7 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& a, const Groups& o, un
     auto place = [&](int r0, int buf) {
         uint4* sw = lds + buf * BLOCK + PARTS * BM * 4;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
+        for (int k = 0; k < WC; ++k) {
             constexpr int E = 16 / (int)sizeof(T);
             T y[E];
 #pragma unroll
@@ -842,18 +843,18 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& a, const Groups& o, un
 #pragma unroll
     for (int i = 0; i < PL; ++i) load_a(0, i, 0);
 #pragma unroll
-    for (int i = 0; i < PL; ++i) load_b(0, i, 1);
+    for (int i = 0; i < PB; ++i) load_b(0, i, 1);
     if (steps > 1) {
 #pragma unroll
         for (int i = 0; i < PL; ++i) load_a(1, i, 2);
 #pragma unroll
-        for (int i = 0; i < PL; ++i) load_b(1, i, 3);
+        for (int i = 0; i < PB; ++i) load_b(1, i, 3);
     }
     if (steps > 2)
 #pragma unroll
         for (int i = 0; i < PL; ++i) load_a(2, i, 4);
-    if (steps > 2) asm volatile("s_waitcnt vmcnt(12)" ::: "memory");  // the first stage
-    else if (steps > 1) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+    if (steps > 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * PL + PB) : "memory");  // the first stage
+    else if (steps > 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PL + PB) : "memory");
     else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
@@ -966,10 +967,10 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& a, const Groups& o, un
     else store(a.part + (int64_t)split * a.M * a.ldp, a.ldp, true);
 }
 
-template <typename T, typename O, int BM, int WM, int WN>
+template <typename T, typename O, int BM, int BN, int WM, int WN>
 __global__ void __launch_bounds__(64 * WM * WN, 2) gemm_kernel(GemmArgs a, Groups o) {
     __shared__ uint4 lds[5 * BM * 8];
-    gemm_tile<T, O, BM, WM, WN, true>(a, o, blockIdx.x, lds);
+    gemm_tile<T, O, BM, BN, WM, WN, true>(a, o, blockIdx.x, lds);
 }
 
 
@@ -1164,12 +1165,12 @@ few_join_kernel(FewArgs a, const T* __restrict__ up, int64_t wp, const float* __
 // ------------------------------------------------------------------------------------------
 // Some rows (over 64, but too few tiles for the chip): the product over splits of the contraction and, in blocks of the same launch, the
 // shrink over ranges of it, since neither needs the other; few_join_kernel adds both up and expands.
-template <typename T, int KT>
+template <typename T, int KT, int BN>
 __global__ void __launch_bounds__(256, 2) some_sums_kernel(GemmArgs g, ShrinkArgs s, Groups o, float* part_h, int r_blocks, int r_splits, int64_t n) {
     __shared__ uint4 lds[5 * 128 * 8];
     const unsigned products = g.per_xcd * 8;
     if (blockIdx.x < products) {
-        gemm_tile<T, float, 128, 2, 2, false>(g, o, blockIdx.x, lds);
+        gemm_tile<T, float, 128, BN, BN == 128 ? 2 : 4, BN == 128 ? 2 : 1, false>(g, o, blockIdx.x, lds);
         return;
     }
     const int id = (int)(blockIdx.x - products), split = id % r_splits, k = id / r_splits, r0 = k % r_blocks * 16 * KT;
@@ -1317,13 +1318,14 @@ struct Plan {
 // time beside another: 40 for two small tiles a unit, 25 for one (20 in f32, where the matrix instructions alone bind), 60 for a large
 // one (76). The cheaper kind is taken. Whole calls in us, small and large: bf16, rank 64, from 4096 to 4096: 103 and 129 at 1777 rows, 141
 // and 132 at 2304, 220 and 242 at 5000; f32, rank 8 and 16: 415 and 520 at 3000 x 2000 -> 2900, 2098 and 2010 at 8192 x 4096 -> 4096.
+// Results of up to 64 columns take tiles of 128 x 64: 24203 x 2368 -> 21 in f32 131 us, 199 with 128 x 128; -> 64 in bf16 70 and 74.
 // Small tiles that leave much of the chip idle are split over the contraction (`few`), for up to 512 blocks of 8 stages and more (256 of
 // 2 in f32, where two on a unit take twice as long: 27 and 31 us of sums at 1003 x 4001 -> 200), and the adapters' part is left to the
 // join: where the part of the time that is idle (0.6 us a stage for a block alone, 1.75 in f32) is more than the partial sums take.
 // Whole and split: 61 and 45 us at 2100 x 4096 -> 1024, 66 and 69 at 3900 rows, 29 and 37 at 3900 x 512, 38 and 28 at 300 x 2000 -> 2900;
 // f32 279 and 40 at 1003 x 4001 -> 200, 94 and 100 at 3900 x 1024 -> 1024.
 struct Tiling {
-    bool big, few;
+    bool big, narrow, few;
     unsigned m_tiles, n_tiles, splits;
 };
 Tiling tiling(int64_t M, int64_t N, int64_t row_bytes, int es) {
@@ -1331,12 +1333,13 @@ Tiling tiling(int64_t M, int64_t N, int64_t row_bytes, int es) {
     const auto tiles_of = [&](int64_t b) { return ((M + b - 1) / b) * ((N + b - 1) / b); };
     const int64_t left = tiles_of(128) % 512;
     const int64_t small = tiles_of(128) / 512 * 40 + (left > 256 ? 40 : left == 0 ? 0 : es == 2 ? 25 : 20);
-    t.big = (tiles_of(256) + 255) / 256 * (es == 2 ? 60 : 76) < small;
+    t.big = N > 64 && (tiles_of(256) + 255) / 256 * (es == 2 ? 60 : 76) < small;
     const int64_t b = t.big ? 256 : 128, tiles = std::max<int64_t>(1, tiles_of(b)), stages = row_bytes / 128;
+    t.narrow = !t.big && N <= 64;
     t.m_tiles = (unsigned)((M + b - 1) / b), t.n_tiles = (unsigned)((N + b - 1) / b);
     t.splits = (unsigned)std::max<int64_t>(1, es == 2 ? std::min<int64_t>({512 / tiles, stages / 8, 16}) : std::min<int64_t>({256 / tiles, stages / 2, 32}));
     const double idle = 1 - (double)tiles / (es == 2 ? 320 : 256);  // in bf16 two blocks on a unit have 1.25 times the rate of one
-    t.few = !t.big && (double)stages * (es == 2 ? 0.6 : 1.75) * idle > 0.028 * (double)(tiles * t.splits);
+    t.few = !t.big && (double)stages * (es == 2 ? 0.6 : 1.75) * (t.narrow ? 0.5 : 1) * idle > 0.028 * (double)(tiles * t.splits);
     if (!t.few) t.splits = 1;
     return t;
 }
@@ -1528,8 +1531,9 @@ template <typename T, typename O>
 int launch_gemm(GemmArgs a, const Groups& o, hipStream_t st) {
     const Tiling t = tiling(a.M, a.N, (int64_t)a.steps * 128, sizeof(T));
     if (const int rc = place_tiles(a, t)) return rc;
-    if (t.big) hipLaunchKernelGGL((gemm_kernel<T, O, 256, 2, 4>), dim3(a.per_xcd * 8), dim3(512), 0, st, a, o);
-    else hipLaunchKernelGGL((gemm_kernel<T, O, 128, 2, 2>), dim3(a.per_xcd * 8), dim3(256), 0, st, a, o);
+    if (t.big) hipLaunchKernelGGL((gemm_kernel<T, O, 256, 256, 2, 4>), dim3(a.per_xcd * 8), dim3(512), 0, st, a, o);
+    else if (t.narrow) hipLaunchKernelGGL((gemm_kernel<T, O, 128, 64, 4, 1>), dim3(a.per_xcd * 8), dim3(256), 0, st, a, o);
+    else hipLaunchKernelGGL((gemm_kernel<T, O, 128, 128, 2, 2>), dim3(a.per_xcd * 8), dim3(256), 0, st, a, o);
     HIP_TRY(hipGetLastError());
     return RP_OK;
 }
@@ -1560,8 +1564,10 @@ int launch_some(const Plan& l, const T* X, int64_t ldx, const T* C, int64_t kp, 
     float* part_h = g.part + t.splits * n * g.ldp;
     const ShrinkArgs s{X, ldx, kp, W, G, R, nullptr, nullptr, 0, nullptr, nullptr};
     const dim3 grid(g.per_xcd * 8 + (unsigned)(l.max_tiles * c.r_blocks * c.r_splits)), block(256);
-    if (R <= 16) hipLaunchKernelGGL((some_sums_kernel<T, 1>), grid, block, 0, st, g, s, o, part_h, c.r_blocks, c.r_splits, n);
-    else hipLaunchKernelGGL((some_sums_kernel<T, 2>), grid, block, 0, st, g, s, o, part_h, c.r_blocks, c.r_splits, n);
+    if (R <= 16 && t.narrow) hipLaunchKernelGGL((some_sums_kernel<T, 1, 64>), grid, block, 0, st, g, s, o, part_h, c.r_blocks, c.r_splits, n);
+    else if (R <= 16) hipLaunchKernelGGL((some_sums_kernel<T, 1, 128>), grid, block, 0, st, g, s, o, part_h, c.r_blocks, c.r_splits, n);
+    else if (t.narrow) hipLaunchKernelGGL((some_sums_kernel<T, 2, 64>), grid, block, 0, st, g, s, o, part_h, c.r_blocks, c.r_splits, n);
+    else hipLaunchKernelGGL((some_sums_kernel<T, 2, 128>), grid, block, 0, st, g, s, o, part_h, c.r_blocks, c.r_splits, n);
     HIP_TRY(hipGetLastError());
     FewArgs a{};
     a.n = (int)n, a.p = (int)p, a.pp = (int)g.ldp, a.G = G, a.R = R, a.ids = ids;

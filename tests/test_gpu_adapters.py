@@ -464,3 +464,12 @@ def test_few_odd_rows(n, m, p, R, G, compute):
     rest = torch.ones(G, dtype=torch.bool, device="cuda")
     rest[used] = False
     assert not dd2[rest].any() and not du2[rest].any()
+
+
+@pytest.mark.parametrize("compute", ["bf16", "fp32"])
+@pytest.mark.parametrize("shape", [(9000, 64, 50, 4, 40), (3000, 700, 64, 3, 128), (40000, 60, 33, 5, 9), (50000, 1000, 64, 6, 16), (700, 5000, 3, 9, 7), (45000, 63, 1, 2, 1)])
+def test_narrow_results(shape, compute):
+    """Up to 64 columns of Y or of dX."""
+    g = torch.Generator().manual_seed(shape[0])
+    ids = torch.repeat_interleave(torch.randint(-1, shape[3], (shape[0] // 50 + 1,), generator=g), 50)[:shape[0]]
+    check(make(*shape, compute, seed=shape[1], ids=ids), compute)

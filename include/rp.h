@@ -336,8 +336,8 @@ int rp_dense_project_device(int device, const void* X, int32_t dtype, int64_t n,
  * and hidden are f32. With s = 64 (bf16) or 32 (f32), mk and pk are m and p rounded up to a multiple
  * of s: C is p x mk, down adapters x rank x mk, up adapters x rank x pk, zeros in the columns past m or p,
  * 16-byte aligned. X is n x m with row stride ldx; its rows are 16-byte aligned where m is a multiple of s, and
- * are copied to padded ones in the workspace where it is not. rank <= 128 (an adapter of
- * a smaller rank is padded with zero rows), adapters <= 16383. scale: device f32, one for each
+ * begin at any element where it is not. rank <= 128 (an adapter of a smaller rank is padded with zero
+ * rows), adapters <= 16383. scale: device f32, one for each
  * adapter, or NULL (1). Y: n x p, row stride ldy. hidden: n x rank (contiguous, zeros for rows without
  * an adapter) or NULL when the backward pass is not wanted. workspace: rp_adapt_workspace_bytes bytes,
  * 256-byte aligned, in use until the call's work on `stream` is done. Asynchronous on `stream`; does

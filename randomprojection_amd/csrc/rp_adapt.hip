@@ -1000,7 +1000,8 @@ struct FewArgs {
 // groups the rows where the gradients of the banks are to come.
 template <typename T, int NT, int KT, bool ODD>
 __global__ void __launch_bounds__(64 * kFewWaves, 4) few_sums_kernel(FewArgs a, Groups o) {
-    constexpr int XL = 16 * NT * 8, E = 16 / (int)sizeof(T), LE = 128 / (int)sizeof(T);  // chunks of a line of all rows; elements of a chunk, of a line
+    constexpr int XL = 16 * NT * 8;  // chunks of a line of all rows
+    constexpr int E = 16 / (int)sizeof(T), LE = 128 / (int)sizeof(T);  // elements of a chunk, of a line
     __shared__ uint4 lds[kFewLines * (XL > KT * 64 ? XL : KT * 64)];
     __shared__ int members[17];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, c = lane & 15, q = lane >> 4;
@@ -1297,8 +1298,8 @@ int launch_few(const T* X, int64_t ldx, int64_t width, const T* C, int64_t kp, i
     if (R <= 16) kp == width ? launch(integral_constant<int, 1>{}, false_type{}) : launch(integral_constant<int, 1>{}, true_type{});
     else kp == width ? launch(integral_constant<int, 2>{}, false_type{}) : launch(integral_constant<int, 2>{}, true_type{});
     HIP_TRY(hipGetLastError());
-    hipLaunchKernelGGL((few_join_kernel<T, O>), dim3((unsigned)n, (unsigned)std::max<int64_t>(1, (p + 255) / 256)), dim3(64), 0, st, a, U, wp, scale, out, ldo,
-                       hidden);
+    hipLaunchKernelGGL((few_join_kernel<T, O>), dim3((unsigned)n, (unsigned)std::max<int64_t>(1, (p + 255) / 256)), dim3(64), 0, st, a, U, wp,
+                       scale, out, ldo, hidden);
     HIP_TRY(hipGetLastError());
     return RP_OK;
 }
@@ -1337,7 +1338,8 @@ Tiling tiling(int64_t M, int64_t N, int64_t row_bytes, int es) {
     const int64_t b = t.big ? 256 : 128, tiles = std::max<int64_t>(1, tiles_of(b)), stages = row_bytes / 128;
     t.narrow = !t.big && N <= 64;
     t.m_tiles = (unsigned)((M + b - 1) / b), t.n_tiles = (unsigned)((N + b - 1) / b);
-    t.splits = (unsigned)std::max<int64_t>(1, es == 2 ? std::min<int64_t>({512 / tiles, stages / 8, 16}) : std::min<int64_t>({256 / tiles, stages / 2, 32}));
+    const int64_t splits = es == 2 ? std::min<int64_t>({512 / tiles, stages / 8, 16}) : std::min<int64_t>({256 / tiles, stages / 2, 32});
+    t.splits = (unsigned)std::max<int64_t>(1, splits);
     const double idle = 1 - (double)tiles / (es == 2 ? 320 : 256);  // in bf16 two blocks on a unit have 1.25 times the rate of one
     t.few = !t.big && (double)stages * (es == 2 ? 0.6 : 1.75) * (t.narrow ? 0.5 : 1) * idle > 0.028 * (double)(tiles * t.splits);
     if (!t.few) t.splits = 1;
@@ -1453,7 +1455,8 @@ unsigned pad_blocks(const Pad& p, const Pad& q, int threads) {
 int launch_groups(const Plan& l, const Groups& o, const int32_t* ids, int64_t n, int G, const Pad& p, const Pad& q, hipStream_t st) {
     if (l.small) {
         const unsigned waves = n <= 256 ? 4 : 16;
-        hipLaunchKernelGGL(group_small_kernel, dim3(1 + pad_blocks(p, q, (int)waves * 64)), dim3(64 * waves), 4 * ((waves + 4) * (G + 1) + 1), st, ids,
+        const size_t lds = 4 * ((waves + 4) * (G + 1) + 1);
+        hipLaunchKernelGGL(group_small_kernel, dim3(1 + pad_blocks(p, q, (int)waves * 64)), dim3(64 * waves), lds, st, ids,
                            (int)n, G, l.bits, l.tile_rows, l.chunk_rows, o, p, q);
     } else {
         if (const unsigned blocks = pad_blocks(p, q, 256)) {

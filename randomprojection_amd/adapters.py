@@ -20,7 +20,7 @@ import functools
 import torch
 
 from . import _native as nat
-from .gaussian import _STEP
+from .gaussian import _STEP, stream_of
 
 __all__ = ["adapted_project_device", "adapted_project_backward_device", "prepare_bank", "MAX_RANK", "MAX_ADAPTERS"]
 
@@ -122,7 +122,7 @@ def _on_stream(stream, dev, tensors):
     if stream is None or stream == now:
         return now
     cur = torch.cuda.current_stream(dev)
-    ext = torch.cuda.ExternalStream(stream, device=cur.device)
+    ext = stream_of(stream, dev)
     ext.wait_stream(cur)
     for t in tensors:
         if t is not None:

@@ -49,6 +49,13 @@ def _dtype(torch, compute):
         raise ValueError("compute must be 'fp32', 'fp64' or 'bf16'") from None
 
 
+def stream_of(handle, device):
+    """The stream of a raw handle. 0 is the default stream's: an ExternalStream of 0 would be a new stream."""
+    import torch
+
+    return torch.cuda.ExternalStream(handle, device=device) if handle else torch.cuda.default_stream(device)
+
+
 def prepare_operand(A, compute: str):
     """A (rows x m) cast to the compute dtype, contiguous, the contraction padded with zeros to the
     kernel's K multiple (zeros add nothing). Done once for the components in ``transform``."""
@@ -91,7 +98,7 @@ def dense_project_device(X, C, out=None, compute: str = "fp32", stream=None, pre
     elif stream != cur.cuda_stream:
         # the GEMM reads Xc / Cc on another stream: order it after the casts / pads queued on the
         # current stream (an event wait on the device, no host sync), and keep them alive for it
-        ext = torch.cuda.ExternalStream(stream, device=X.device)
+        ext = stream_of(stream, X.device)
         ext.wait_stream(cur)
         for t in (Xc, Cc):
             t.record_stream(ext)

@@ -13,6 +13,7 @@ import torch
 
 from . import _native as nat
 from .adapters import raw_stream
+from .gaussian import stream_of
 
 __all__ = ["AdamW", "BLOCK"]
 
@@ -106,7 +107,7 @@ class AdamW:
         if stream is None or stream == now:
             return now
         cur = torch.cuda.current_stream(self.device)
-        ext = torch.cuda.ExternalStream(stream, device=self.device)
+        ext = stream_of(stream, self.device)
         ext.wait_stream(cur)
         for t in tensors:
             if t is not None:

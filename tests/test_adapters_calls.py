@@ -1,0 +1,53 @@
+"""Adapters beside the dense projection and AdamW: which stream a call takes, sizes at the limits, checked without a GPU."""
+import contextlib
+
+import pytest
+import torch
+
+from randomprojection_amd import adapters, optim
+
+
+class _Stream:
+    def __init__(self, handle):
+        self.cuda_stream, self.device, self.waited = handle, torch.device("cuda", 0), []
+
+    def wait_stream(self, other):
+        self.waited.append(other)
+
+
+@pytest.fixture
+def streams(monkeypatch):
+    """torch's streams as they are where the current one is a side stream: handle 0 is the default stream, and an
+    ExternalStream of 0 would be a stream of its own."""
+    made = {0: _Stream(0), 111: _Stream(111)}
+    external = lambda handle, device=None: made.setdefault(handle or 999, _Stream(handle or 999))  # noqa: E731
+    monkeypatch.setattr(torch.cuda, "default_stream", lambda device=None: made[0])
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: made[111])
+    monkeypatch.setattr(torch.cuda, "ExternalStream", external)
+    monkeypatch.setattr(torch.cuda, "stream", lambda s: contextlib.nullcontext(s))
+    for module in (adapters, optim):
+        monkeypatch.setattr(module, "raw_stream", lambda device: 111)
+    return made
+
+
+@pytest.mark.parametrize("handle", [0, 222, 111, None])
+def test_the_stream_that_is_named_waits_for_the_current_one(streams, handle):
+    """The default stream's handle is 0: it is that stream that has to wait for the casts queued on the current one."""
+    class Temporary:
+        kept = []
+
+        def record_stream(self, s):
+            self.kept.append(s)
+
+    dev = torch.device("cuda", 0)
+    opt = optim.AdamW.__new__(optim.AdamW)
+    opt.device = dev
+    for call in (lambda t: adapters._on_stream(handle, dev, (t, None)), lambda t: opt._stream(handle, t, None)):
+        temporary = Temporary()
+        temporary.kept = []
+        for s in streams.values():
+            s.waited.clear()
+        assert call(temporary) == (111 if handle is None else handle)
+        other = handle not in (None, 111)
+        assert temporary.kept == ([streams[handle]] if other else [])
+        assert {k: v.waited for k, v in streams.items() if v.waited} == ({handle: [streams[111]]} if other else {})

@@ -1,0 +1,38 @@
+"""Adapters and AdamW in calls that the documentation allows: streams of any handle, empty batches, the largest sizes, values
+that are not finite, every form of the shrink. Bounds as in test_gpu_adapters.py."""
+import pytest
+import torch
+
+from test_gpu_adapters import TYPE, check, make
+
+pytestmark = pytest.mark.gpu
+
+
+def test_default_stream_waits_for_the_current_one():
+    """Called under a side stream that still makes the operands, the default stream (handle 0) waits for it."""
+    from randomprojection_amd.adapters import adapted_project_backward_device, adapted_project_device
+    from randomprojection_amd.gaussian import dense_project_device
+    from randomprojection_amd.optim import AdamW
+
+    t = make(700, 333, 100, 6, 8, "bf16", seed=2)
+    kw = dict(scale=t["scale"], compute="bf16")
+
+    def run(X, **on):
+        Y, h = adapted_project_device(X, t["C"], t["down"], t["up"], t["ids"], return_hidden=True, **kw, **on)
+        got = adapted_project_backward_device(t["dY"], X, t["C"].T, t["down"], t["up"], t["ids"], h, **kw, **on)
+        w, g = torch.ones(5000, device="cuda"), X.float().view(-1)[:5000]
+        opt = AdamW([w], [g], state_bits=8)
+        opt.step(**on)
+        return [Y, h, *got, w, *opt.state_values(**on), dense_project_device(X, t["C"], compute="bf16", **on)]
+
+    wide = t["X"].double()
+    want = run(wide.to(TYPE["bf16"]))
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        late = torch.zeros_like(wide)
+        torch.cuda._sleep(100_000_000)  # cycles: the copy below comes tens of milliseconds later
+        late.copy_(wide)
+        got = run(late.to(TYPE["bf16"]), stream=torch.cuda.default_stream().cuda_stream)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

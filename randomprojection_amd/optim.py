@@ -130,10 +130,14 @@ class AdamW:
 
     def state_values(self, *, stream=None):
         """(m, sqrt(v)) of all blocks in float32: 256 elements a block, the last block of a tensor padded with zeros."""
-        if self.state_bits == 32:
-            return self.state["exp_avg"].clone(), self.state["exp_avg_sq"].sqrt()
         m, root = (torch.empty(self.state["exp_avg"].numel(), dtype=torch.float32, device=self.device) for _ in range(2))
-        nat.check(nat.load().rp_adamw_values(self._h, m.data_ptr(), root.data_ptr(), self._stream(stream, m, root)))
+        now, on = raw_stream(self.device.index), self._stream(stream, m, root)
+        if self.state_bits == 8:
+            nat.check(nat.load().rp_adamw_values(self._h, m.data_ptr(), root.data_ptr(), on))
+            return m, root
+        with torch.cuda.stream(None if on == now else stream_of(on, self.device)):  # None: the current one stays
+            m.copy_(self.state["exp_avg"])
+            torch.sqrt(self.state["exp_avg_sq"], out=root)
         return m, root
 
     def state_dict(self):

@@ -51,3 +51,25 @@ def test_the_stream_that_is_named_waits_for_the_current_one(streams, handle):
         other = handle not in (None, 111)
         assert temporary.kept == ([streams[handle]] if other else [])
         assert {k: v.waited for k, v in streams.items() if v.waited} == ({handle: [streams[111]]} if other else {})
+
+
+def test_state_values_take_the_stream_in_both_widths(streams):
+    """States in 32 bits are read out on the stream that is named too, behind the steps queued there."""
+    opt = optim.AdamW.__new__(optim.AdamW)
+    opt.device, opt.state_bits = torch.device("cpu"), 32
+    opt.state = {"exp_avg": torch.tensor([1.0, -2.0]), "exp_avg_sq": torch.tensor([9.0, 0.25])}
+    entered, current = [], torch.cuda.stream
+    torch.cuda.stream = lambda s: entered.append(s) or current(s)  # the fixture puts torch's own back
+    torch.Tensor.record_stream, record = lambda t, s: None, torch.Tensor.record_stream
+    try:
+        for handle, waits in ((None, []), (111, []), (0, [streams[111]]), (222, [streams[111]])):
+            entered.clear()
+            m, root = opt.state_values(stream=handle)
+            assert torch.equal(m, opt.state["exp_avg"]) and torch.equal(root, torch.tensor([3.0, 0.5]))
+            assert m.data_ptr() != opt.state["exp_avg"].data_ptr()
+            if waits:
+                assert entered == [streams[handle]] and streams[handle].waited == waits
+            else:
+                assert entered in ([], [None])
+    finally:
+        torch.Tensor.record_stream = record

@@ -36,3 +36,25 @@ def test_default_stream_waits_for_the_current_one():
         got = run(late.to(TYPE["bf16"]), stream=torch.cuda.default_stream().cuda_stream)
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_state_values_behind_a_step_on_another_stream(bits):
+    """The states are read out on the stream whose step makes them."""
+    from randomprojection_amd.optim import AdamW
+
+    def run(**on):
+        g = torch.Generator().manual_seed(1)
+        opt = AdamW([torch.zeros(70000, device="cuda")], [torch.randn(70000, generator=g).cuda()], state_bits=bits)
+        torch.cuda.synchronize()
+        if on:
+            with torch.cuda.stream(side):
+                torch.cuda._sleep(100_000_000)  # cycles: the step comes tens of milliseconds later
+        opt.step(**on)
+        got = opt.state_values(**on)
+        torch.cuda.synchronize()
+        return got
+
+    side = torch.cuda.Stream()
+    for a, b in zip(run(stream=side.cuda_stream), run()):
+        assert b.any() and torch.equal(a, b)

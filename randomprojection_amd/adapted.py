@@ -37,7 +37,7 @@ class _Bank:
         self.scale = torch.ones(G, device=dev)
         each = lambda ts: [t[g] for t in ts for g in range(G)]  # noqa: E731
         self.opt = AdamW(each(self.params), each(self.grads), lr=est.learning_rate, betas=est.betas, weight_decay=est.weight_decay,
-                         state_bits=est.state_bits, copies=each(self.low) if mode == "bf16" else None, seed=int(est.seed))
+                         state_bits=est.state_bits, copies=each(self.low) if mode == "bf16" else None, seed=est._seed)
         if state is not None:
             self.opt.load_state_dict({k: torch.as_tensor(v).view(self.opt.state[k].dtype) for k, v in state.items()})
 
@@ -103,6 +103,7 @@ class AdaptedGaussianProjection(GaussianRandomProjection):
             self.random_state).randint(2 ** 31 - 1)))
         self._down = rng.normal(0, m ** -0.5, (self.n_adapters, self.rank, m)).astype(np.float32)
         self._up = np.zeros((self.n_adapters, self.rank, p), np.float32)
+        self._seed = int(self.seed)
         self._bank, self._state, self._state_of = None, None, None
         return self
 

@@ -73,3 +73,30 @@ def test_state_values_take_the_stream_in_both_widths(streams):
                 assert entered in ([], [None])
     finally:
         torch.Tensor.record_stream = record
+
+
+def test_seed_is_as_fitted(monkeypatch):
+    """What the optimizer rounds by is the seed of the last fit, whenever it is made and whatever was set since; it travels in a pickle."""
+    import pickle
+
+    import numpy as np
+
+    from randomprojection_amd import AdaptedGaussianProjection, gaussian
+
+    made = []
+
+    class Optimizer:
+        def __init__(self, params, grads, *, seed, **kw):
+            made.append(seed)
+
+    device = torch.device
+    monkeypatch.setattr(torch, "device", lambda *a: device("cpu"))
+    monkeypatch.setattr(optim, "AdamW", Optimizer)
+    monkeypatch.setattr(gaussian, "_torch", lambda: torch)
+    X = np.random.default_rng(0).standard_normal((20, 33))
+    est = AdaptedGaussianProjection(n_components=7, n_adapters=3, rank=2, random_state=5, seed=4).fit(X)
+    est.set_params(seed=9)
+    pickle.loads(pickle.dumps(est))._on_device()
+    est._on_device()
+    est.set_params(seed=9).fit(X)._on_device()
+    assert made == [4, 4, 9]

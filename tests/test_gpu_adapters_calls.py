@@ -58,3 +58,18 @@ def test_state_values_behind_a_step_on_another_stream(bits):
     side = torch.cuda.Stream()
     for a, b in zip(run(stream=side.cuda_stream), run()):
         assert b.any() and torch.equal(a, b)
+
+
+def test_seed_set_after_fit_waits_for_the_next_fit():
+    """Rounding to 8 bits goes by the seed as fitted: two estimators of one history agree bit for bit."""
+    from randomprojection_amd import AdaptedGaussianProjection
+
+    g = torch.Generator().manual_seed(1)
+    X, T, ids = torch.randn(300, 70, generator=g).numpy(), torch.randn(300, 20, generator=g).numpy(), (torch.arange(300) % 3).numpy()
+    kept, changed, other = (AdaptedGaussianProjection(n_components=20, n_adapters=3, rank=4, random_state=3, state_bits=8, seed=s).fit(X)
+                            for s in (5, 5, 6))
+    changed.set_params(seed=6)
+    for _ in range(3):
+        for est in (kept, changed, other):
+            est.partial_fit(X, T, ids)
+    assert (kept.down_ == changed.down_).all() and (kept.up_ == changed.up_).all() and (kept.up_ != other.up_).any()

@@ -73,3 +73,21 @@ def test_seed_set_after_fit_waits_for_the_next_fit():
         for est in (kept, changed, other):
             est.partial_fit(X, T, ids)
     assert (kept.down_ == changed.down_).all() and (kept.up_ == changed.up_).all() and (kept.up_ != other.up_).any()
+
+
+# Shapes on both sides of the branches that pick a shrink for the forward pass: 16 rows a tile under 512 tiles of 64 rows (32 over rank
+# 64), else 64 (32); and 16 again, beside a split product, where there are few tiles of it. The backward pass takes the same branches with
+# m and p exchanged. The rank pads to 16, 32, 64 or 128 (f32: its pieces to a multiple of 16).
+FORMS = [(32768, 70, 200, 3, 17), (33001, 100, 90, 5, 20), (32768, 65, 66, 3, 32), (33100, 130, 70, 4, 33), (40000, 64, 129, 7, 64), (32799, 200, 65, 2, 48),
+         (32767, 70, 200, 3, 20), (32767, 129, 90, 4, 50), (16384, 70, 90, 3, 65), (16383, 100, 70, 2, 128), (35000, 65, 77, 900, 24)]
+
+
+@pytest.mark.parametrize("compute", ["bf16", "fp32"])
+@pytest.mark.parametrize("shape", FORMS)
+def test_every_form_of_the_shrink(shape, compute):
+    """Runs of rows of every length, so that tiles end inside, at and behind a multiple of 16, 32 and 64 rows."""
+    n, _, _, G, _ = shape
+    g = torch.Generator().manual_seed(sum(shape))
+    lengths = torch.randint(1, 300, (n,), generator=g)
+    ids = torch.repeat_interleave(torch.randint(-1, G, (n,), generator=g), lengths)[:n]
+    check(make(*shape, compute, seed=G, ids=ids), compute, prepared=True)

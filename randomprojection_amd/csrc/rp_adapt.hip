@@ -1388,7 +1388,7 @@ Plan plan_for(int32_t dtype, int64_t n, int64_t m, int64_t p, int64_t G, int R, 
     // adapters: 0.10 ms, 0.70 with 128 waves)
     l.each = std::min<int64_t>(2048, std::max<int64_t>(256, (n / 128 + 63) / 64 * 64));
     while ((n + l.each - 1) / l.each * (G + 1) > (1 << 20)) l.each *= 2;
-    l.n_chunks = l.small ? 0 : (int)((n + l.each - 1) / l.each);
+    l.n_chunks = l.small ? 0 : (int)std::max<int64_t>(1, (n + l.each - 1) / l.each);  // one without rows too: the lists come from its counts
     l.max_tiles = n / l.tile_rows + std::min(n, G + 1);
     l.max_chunks = n / l.chunk_rows + G;
     l.max_parts = 2 * (n / l.chunk_rows);

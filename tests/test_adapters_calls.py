@@ -4,6 +4,7 @@ import contextlib
 import pytest
 import torch
 
+from randomprojection_amd import _native as nat
 from randomprojection_amd import adapters, optim
 
 
@@ -100,3 +101,12 @@ def test_seed_is_as_fitted(monkeypatch):
     est._on_device()
     est.set_params(seed=9).fit(X)._on_device()
     assert made == [4, 4, 9]
+
+
+@pytest.mark.parametrize("dtype", [nat.RP_F32, nat.RP_BF16])
+def test_workspace_without_rows_holds_the_counts(dtype):
+    """Over 700 adapters the gradients of an empty batch count its rows as those of a longer one do: five lists of an entry an adapter and 16
+    bytes of each one's chunk."""
+    for G in (701, 4000, 16383):
+        for what in (nat.RP_ADAPT_GRADIENTS, nat.RP_ADAPT_GRADIENTS_DX):
+            assert nat.load().rp_adapt_workspace_bytes(dtype, 0, 70, 20, G, 1, what) >= (5 * 4 + 16) * G

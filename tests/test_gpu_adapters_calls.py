@@ -91,3 +91,21 @@ def test_every_form_of_the_shrink(shape, compute):
     lengths = torch.randint(1, 300, (n,), generator=g)
     ids = torch.repeat_interleave(torch.randint(-1, G, (n,), generator=g), lengths)[:n]
     check(make(*shape, compute, seed=G, ids=ids), compute, prepared=True)
+
+
+@pytest.mark.parametrize("compute", ["bf16", "fp32"])
+@pytest.mark.parametrize("G", [3, 700, 701, 3999, 4000, 16383])
+def test_no_rows_whatever_the_number_of_adapters(G, compute):
+    """An empty batch: zeros for every adapter, written over what was there; what lies between stays."""
+    from randomprojection_amd.adapters import adapted_project_backward_device
+
+    m, p, R = 70, 20, 2
+    t = make(0, m, p, G, R, compute)
+    bd, bu = torch.full((G, R + 1, m + 3), 7.0, device="cuda"), torch.full((G, R, p + 1), 7.0, device="cuda")
+    for Ct in (None, t["C"].T):
+        hidden = torch.empty(0, R, device="cuda")
+        dX, dd, du = adapted_project_backward_device(t["dY"], t["X"], Ct, t["down"], t["up"], t["ids"], hidden, scale=t["scale"], compute=compute,
+                                                     out=(bd[:, :R, :m], bu[..., :p]))
+        assert not dd.any() and not du.any() and (Ct is None or dX.shape == (0, m))
+        assert bool((bd[:, R] == 7).all()) and bool((bd[..., m:] == 7).all()) and bool((bu[..., p:] == 7).all())
+        bd[:, :R, :m], bu[..., :p] = 7.0, 7.0

@@ -23,6 +23,11 @@ namespace {
 // rows that one block groups (up to 700 adapters, whose counts by 16 waves fit its LDS), else three launches: a call of 6225 rows 60 us, 70
 // with three; 16384 rows grouped in 22 us and in 17.5
 constexpr int kSmallRows = 8192;
+// An axis of a grid has fewer than 2^32 threads: blocks of the largest grids fill rows of 2^20 (up to 512 threads a block; a multiple of 8,
+// so block i runs on XCD i % 8 in every row)
+constexpr int64_t kGridRow = 1 << 20;
+dim3 grid_of(int64_t blocks, unsigned z = 1) { return dim3((unsigned)std::min(blocks, kGridRow), (unsigned)((blocks + kGridRow - 1) / kGridRow), z); }
+__device__ __forceinline__ unsigned block_of_grid() { return blockIdx.y * gridDim.x + blockIdx.x; }
 constexpr int kMaxRank = 128, kMaxAdapters = 16383;  // a wave's counts of all groups fit 64 KB of LDS
 
 // rounded to nearest even, two at a time (one instruction); a NaN stays one
@@ -560,7 +565,8 @@ __global__ void __launch_bounds__(256, KT == 1 ? 4 : 2) outer_kernel(OuterArgs a
     constexpr int RS = sizeof(T) == 2 ? 8 : 4;  // rows of a lane in a step of 4 RS rows
     __shared__ int32_t list[kMaxChunk];
     __shared__ float red[4][NC][64][4];
-    const int which = blockIdx.x / blocks, block = blockIdx.x % blocks;
+    const unsigned id = block_of_grid();
+    const int which = (int)(id / (unsigned)blocks), block = (int)(id % (unsigned)blocks);
     if (which >= o.number[1]) return;
     const bool second = block >= blocks0;  // both banks' gradients in one launch
     const OuterArgs& a = second ? a1 : a0;
@@ -746,7 +752,7 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& a, const Groups& o, un
     // XCD x (block i runs on XCD i % 8) takes a run of tiles; tiles go down 8 row tiles, then along the columns, so the
     // tiles that run at the same time on an XCD share their rows of A and of B in its L2
     const unsigned tiles = a.m_tiles * a.n_tiles, id = (block & 7u) * a.per_xcd + (block >> 3);
-    if (id >= tiles * a.splits) return;
+    if ((block >> 3) >= a.per_xcd || id >= tiles * a.splits) return;
     const unsigned split = id / tiles, t = id % tiles, band = t / (8u * a.n_tiles), in = t % (8u * a.n_tiles);
     const unsigned high = min(8u, a.m_tiles - band * 8u), mt = band * 8u + in % high, nt = in / high;
     const int64_t m0 = (int64_t)mt * BM;
@@ -970,7 +976,7 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& a, const Groups& o, un
 template <typename T, typename O, int BM, int BN, int WM, int WN>
 __global__ void __launch_bounds__(64 * WM * WN, 2) gemm_kernel(GemmArgs a, Groups o) {
     __shared__ uint4 lds[5 * BM * 8];
-    gemm_tile<T, O, BM, BN, WM, WN, true>(a, o, blockIdx.x, lds);
+    gemm_tile<T, O, BM, BN, WM, WN, true>(a, o, block_of_grid(), lds);
 }
 
 
@@ -1263,14 +1269,15 @@ FewCut few_cut(int64_t n, int64_t p, int R, int64_t line_bytes) {
     f.c_blocks = (int)((p + 127) / 128), f.r_blocks = (R + (R <= 16 ? 15 : 31)) / (R <= 16 ? 16 : 32);
     // 8 lines a block, fewer where that leaves under 256 blocks; an adapter's lines over about 512 blocks, none with less than two a wave
     f.c_lines = (int)std::max<int64_t>(2, std::min<int64_t>(kFewLines, lines * f.c_blocks / 256));
-    f.c_splits = (int)((lines + f.c_lines - 1) / f.c_lines);
+    f.c_splits = p ? (int)((lines + f.c_lines - 1) / f.c_lines) : 0;
     f.r_splits = (int)std::max<int64_t>(1, std::min<int64_t>({512 / std::max<int64_t>(1, n * f.r_blocks), lines / (2 * kFewWaves), 16}));
     return f;
 }
 size_t few_bytes(int64_t n, int64_t p, int R, int64_t line_bytes) {
     const FewCut f = few_cut(n, p, R, line_bytes);
-    return ((size_t)4 * n * ((size_t)(p ? f.c_splits : 0) * ((p + 3) / 4 * 4) + (size_t)f.r_splits * R) + 255) & ~(size_t)255;
+    return ((size_t)4 * n * ((size_t)f.c_splits * ((p + 3) / 4 * 4) + (size_t)f.r_splits * R) + 255) & ~(size_t)255;
 }
+int64_t few_blocks(const FewCut& f, int64_t n) { return (int64_t)f.c_blocks * f.c_splits + n * f.r_blocks * f.r_splits; }
 
 template <typename T, typename O>
 int launch_few(const T* X, int64_t ldx, int64_t width, const T* C, int64_t kp, int64_t n, int64_t p, const T* W, const T* U, int64_t wp, int G, int R,
@@ -1280,12 +1287,10 @@ int launch_few(const T* X, int64_t ldx, int64_t width, const T* C, int64_t kp, i
     a.X = (const char*)X, a.C = (const char*)C, a.W = (const char*)W, a.ldx = ldx * es, a.kp = kp * es, a.width = (int)width;
     a.n = (int)n, a.p = (int)p, a.pp = (int)((p + 3) / 4 * 4), a.G = G, a.R = R, a.ids = ids;
     const FewCut f = few_cut(n, p, R, a.kp);
-    a.c_blocks = f.c_blocks, a.c_lines = f.c_lines, a.c_splits = p ? f.c_splits : 0, a.r_blocks = f.r_blocks, a.r_splits = f.r_splits;
+    a.c_blocks = f.c_blocks, a.c_lines = f.c_lines, a.c_splits = f.c_splits, a.r_blocks = f.r_blocks, a.r_splits = f.r_splits;
     a.part = (float*)ws, a.part_h = a.part + (int64_t)a.c_splits * n * a.pp;
-    const int64_t blocks = (int64_t)a.c_blocks * a.c_splits + n * a.r_blocks * a.r_splits + (groups ? 1 : 0);
     const Groups o = groups ? *groups : Groups{};
-    if (blocks >= ((int64_t)1 << 31)) return fail(RP_ERR_UNSUPPORTED, "m or p too large");
-    const dim3 grid((unsigned)blocks), block(64 * kFewWaves);
+    const dim3 grid((unsigned)(few_blocks(f, n) + (groups ? 1 : 0))), block(64 * kFewWaves);
     const int nt = n <= 16 ? 1 : n <= 32 ? 2 : 4;
     const auto launch = [&](auto k_tiles, auto odd) {
         constexpr int KT = decltype(k_tiles)::value;
@@ -1503,13 +1508,13 @@ int launch_shrink(const Plan& l, const ShrinkArgs& a, const Groups& o, hipStream
     return RP_OK;
 }
 
+int64_t outer_columns(int64_t q, int es) { return (q + 256 / es - 1) / (256 / es); }  // blocks of 128 (bf16) or 64 columns
+
 template <typename T>
 int launch_outer(const Plan& l, const OuterArgs& a, const OuterArgs& b, const Groups& o, int64_t n, int G, hipStream_t st) {
-    const int64_t wide = 16 * (sizeof(T) == 2 ? 8 : 4);
-    const int64_t qa = (a.q + wide - 1) / wide, qb = (b.q + wide - 1) / wide;
-    if ((qa + qb) * l.max_chunks >= ((int64_t)1 << 31)) return fail(RP_ERR_UNSUPPORTED, "too many adapters and columns for one launch");
+    const int64_t qa = outer_columns(a.q, sizeof(T)), qb = outer_columns(b.q, sizeof(T)), blocks = (qa + qb) * l.max_chunks;
     const int kt = a.R <= 16 ? 1 : a.R <= 32 ? 2 : 4;
-    const dim3 grid((unsigned)((qa + qb) * l.max_chunks), 1, (unsigned)((a.R + 16 * kt - 1) / (16 * kt))), block(256);
+    const dim3 grid = grid_of(blocks, (unsigned)((a.R + 16 * kt - 1) / (16 * kt))), block(256);
     if (kt == 1) hipLaunchKernelGGL((outer_kernel<T, 1>), grid, block, 0, st, a, b, (int)qa, (int)(qa + qb), o);
     else if (kt == 2) hipLaunchKernelGGL((outer_kernel<T, 2>), grid, block, 0, st, a, b, (int)qa, (int)(qa + qb), o);
     else hipLaunchKernelGGL((outer_kernel<T, 4>), grid, block, 0, st, a, b, (int)qa, (int)(qa + qb), o);
@@ -1522,21 +1527,19 @@ int launch_outer(const Plan& l, const OuterArgs& a, const OuterArgs& b, const Gr
     return RP_OK;
 }
 
-int place_tiles(GemmArgs& a, const Tiling& t) {
-    a.m_tiles = t.m_tiles, a.n_tiles = t.n_tiles, a.splits = t.splits;
-    const uint64_t per = ((uint64_t)t.m_tiles * t.n_tiles * t.splits + 7) / 8;
-    if (per * 8 >= (1ull << 30)) return fail(RP_ERR_UNSUPPORTED, "too many rows for one launch");
-    a.per_xcd = (unsigned)per;
-    return RP_OK;
+int64_t tiles_per_xcd(const Tiling& t) { return ((int64_t)t.m_tiles * t.n_tiles * t.splits + 7) / 8; }
+void place_tiles(GemmArgs& a, const Tiling& t) {
+    a.m_tiles = t.m_tiles, a.n_tiles = t.n_tiles, a.splits = t.splits, a.per_xcd = (unsigned)tiles_per_xcd(t);
 }
 
 template <typename T, typename O>
 int launch_gemm(GemmArgs a, const Groups& o, hipStream_t st) {
     const Tiling t = tiling(a.M, a.N, (int64_t)a.steps * 128, sizeof(T));
-    if (const int rc = place_tiles(a, t)) return rc;
-    if (t.big) hipLaunchKernelGGL((gemm_kernel<T, O, 256, 256, 2, 4>), dim3(a.per_xcd * 8), dim3(512), 0, st, a, o);
-    else if (t.narrow) hipLaunchKernelGGL((gemm_kernel<T, O, 128, 64, 4, 1>), dim3(a.per_xcd * 8), dim3(256), 0, st, a, o);
-    else hipLaunchKernelGGL((gemm_kernel<T, O, 128, 128, 2, 2>), dim3(a.per_xcd * 8), dim3(256), 0, st, a, o);
+    place_tiles(a, t);
+    const dim3 grid = grid_of((int64_t)a.per_xcd * 8);
+    if (t.big) hipLaunchKernelGGL((gemm_kernel<T, O, 256, 256, 2, 4>), grid, dim3(512), 0, st, a, o);
+    else if (t.narrow) hipLaunchKernelGGL((gemm_kernel<T, O, 128, 64, 4, 1>), grid, dim3(256), 0, st, a, o);
+    else hipLaunchKernelGGL((gemm_kernel<T, O, 128, 128, 2, 2>), grid, dim3(256), 0, st, a, o);
     HIP_TRY(hipGetLastError());
     return RP_OK;
 }
@@ -1561,7 +1564,7 @@ int launch_some(const Plan& l, const T* X, int64_t ldx, const T* C, int64_t kp, 
     GemmArgs g = gemm_args<T, float>(X, ldx, C, kp, n, p, (float*)nullptr, 0, nullptr, U, wp, G, R, ws);
     Tiling t = tiling(n, p, kp * (int64_t)sizeof(T), sizeof(T));
     if (!p) t.splits = 0;
-    if (const int rc = place_tiles(g, t)) return rc;
+    place_tiles(g, t);
     const SomeCut c = some_cut(l.max_tiles, R, kp * (int64_t)sizeof(T));
     g.ldp = (p + 3) / 4 * 4;
     float* part_h = g.part + t.splits * n * g.ldp;
@@ -1579,6 +1582,35 @@ int launch_some(const Plan& l, const T* X, int64_t ldx, const T* C, int64_t kp, 
                        scale, out, ldo, H);
     HIP_TRY(hipGetLastError());
     return RP_OK;
+}
+
+// The arguments both directions share, and that each launch of the call fits: fewer than 2^31 blocks of the product and of the outer
+// products, and of the others fewer than 2^32 threads.
+int check_call(int32_t dtype, int64_t n, int64_t m, int64_t p, int64_t G, int32_t R, int what) {
+    if (const int rc = check_shared(dtype, n, m, p, G, R)) return rc;
+    const int es = dtype == RP_BF16 ? 2 : 4;
+    const bool forward = what == RP_ADAPT_PROJECT;
+    const int64_t width = forward ? p : m, made = what == RP_ADAPT_GRADIENTS ? 0 : width, row_bytes = padded(forward ? m : p, dtype) * es;
+    const bool few = few_rows(n, width);
+    int64_t outer = 0, product = 0, threads = 0;
+    if (few) threads = (few_blocks(few_cut(n, made, R, row_bytes), n) + 1) * 64 * kFewWaves;
+    if (!few || !forward) {
+        const Plan l = plan_for(dtype, n, m, p, G, R, what);
+        if (!forward) outer = (outer_columns(m, es) + outer_columns(p, es)) * l.max_chunks;
+        if (!few) {
+            const SomeCut c = some_cut(l.max_tiles, R, row_bytes);
+            if (made) product = tiles_per_xcd(tiling(n, width, row_bytes, es)) * 8;
+            threads = (l.some ? product + l.max_tiles * c.r_blocks * c.r_splits : l.max_tiles) * 256;
+        }
+    }
+    if (std::max(outer, product) >= (int64_t)1 << 31 || threads >= (int64_t)1 << 32)
+        return fail(RP_ERR_UNSUPPORTED, "too many rows, columns or adapters for one launch");
+    return RP_OK;
+}
+
+int64_t workspace_of(int32_t dtype, int64_t n, int64_t m, int64_t p, int64_t G, int32_t R, int what) {
+    if (what == RP_ADAPT_PROJECT && few_rows(n, p)) return (int64_t)few_bytes(n, p, R, padded(m, dtype) * (dtype == RP_BF16 ? 2 : 4));
+    return (int64_t)plan_for(dtype, n, m, p, G, R, what).bytes;
 }
 
 template <typename T>
@@ -1654,16 +1686,15 @@ extern "C" {
 
 int64_t rp_adapt_workspace_bytes(int32_t dtype, int64_t n, int64_t m, int64_t p, int64_t adapters, int32_t rank,
                                  int32_t what) {
-    if (check_shared(dtype, n, m, p, adapters, rank)) return -1;
-    if (what == RP_ADAPT_PROJECT && few_rows(n, p)) return (int64_t)few_bytes(n, p, rank, padded(m, dtype) * (dtype == RP_BF16 ? 2 : 4));
-    return (int64_t)plan_for(dtype, n, m, p, adapters, rank, what).bytes;
+    if (check_call(dtype, n, m, p, adapters, rank, what)) return -1;
+    return workspace_of(dtype, n, m, p, adapters, rank, what);
 }
 
 int rp_adapt_project_device(int device, const void* X, int64_t ldx, int32_t dtype, int64_t n, int64_t m, const void* C,
                             int64_t p, const void* down, const void* up, int64_t adapters, int32_t rank, const float* scale,
                             const int32_t* ids, float* Y, int64_t ldy, float* hidden, void* workspace,
                             int64_t workspace_bytes, void* stream) {
-    int rc = check_shared(dtype, n, m, p, adapters, rank);
+    int rc = check_call(dtype, n, m, p, adapters, rank, RP_ADAPT_PROJECT);
     if (rc) return rc;
     const int64_t mk = padded(m, dtype), pk = padded(p, dtype);
     if ((rc = check_rows("X", X, ldx, m, dtype)) || (rc = check_operand("C", C, mk, mk, dtype)) ||
@@ -1672,7 +1703,7 @@ int rp_adapt_project_device(int device, const void* X, int64_t ldx, int32_t dtyp
     if (!ids || !Y) return fail(RP_ERR_INVALID, "NULL ids or Y");
     if (ldy < p) return fail(RP_ERR_INVALID, "Y: row stride %lld is under p=%lld", (long long)ldy, (long long)p);
     if (n == 0) return RP_OK;
-    const int64_t need = rp_adapt_workspace_bytes(dtype, n, m, p, adapters, rank, RP_ADAPT_PROJECT);
+    const int64_t need = workspace_of(dtype, n, m, p, adapters, rank, RP_ADAPT_PROJECT);
     if (!workspace || ((uintptr_t)workspace & 255) || workspace_bytes < need)
         return fail(RP_ERR_INVALID, "workspace must be 256-byte aligned and hold %lld bytes", (long long)need);
     DeviceGuard guard;
@@ -1693,7 +1724,7 @@ int rp_adapt_gradients_device(int device, const void* dY, int64_t lddy, const vo
                               int64_t lddx, float* d_down, int64_t d_down_row, int64_t d_down_adapter, float* d_up,
                               int64_t d_up_row, int64_t d_up_adapter, void* workspace, int64_t workspace_bytes,
                               void* stream) {
-    int rc = check_shared(dtype, n, m, p, adapters, rank);
+    int rc = check_call(dtype, n, m, p, adapters, rank, dX ? RP_ADAPT_GRADIENTS_DX : RP_ADAPT_GRADIENTS);
     if (rc) return rc;
     const int64_t mk = padded(m, dtype), pk = padded(p, dtype);
     if (n && ((rc = check_rows("dY", dY, lddy, p, dtype)) || (rc = check_rows("X", X, ldx, m, dtype)))) return rc;
@@ -1704,8 +1735,7 @@ int rp_adapt_gradients_device(int device, const void* dY, int64_t lddy, const vo
     if (!d_down || !d_up || (n && (!ids || !hidden))) return fail(RP_ERR_INVALID, "NULL ids, hidden, d_down or d_up");
     if (d_down_row < m || d_down_adapter < d_down_row * rank || d_up_row < p || d_up_adapter < d_up_row * rank)
         return fail(RP_ERR_INVALID, "d_down or d_up: strides under the shape");
-    const int64_t need = rp_adapt_workspace_bytes(dtype, n, m, p, adapters, rank,
-                                                  dX ? RP_ADAPT_GRADIENTS_DX : RP_ADAPT_GRADIENTS);
+    const int64_t need = workspace_of(dtype, n, m, p, adapters, rank, dX ? RP_ADAPT_GRADIENTS_DX : RP_ADAPT_GRADIENTS);
     if (need && (!workspace || ((uintptr_t)workspace & 255) || workspace_bytes < need))
         return fail(RP_ERR_INVALID, "workspace must be 256-byte aligned and hold %lld bytes", (long long)need);
     DeviceGuard guard;

@@ -40,6 +40,7 @@ constexpr int kBlock = 256;     // elements under one scale: 4 for each lane of 
 // blocks of one tensor that one wave takes: one while the chip holds a wave for each (8192), four beyond. A wave's blocks follow each
 // other, each with its loads' latency: 1 MB in tensors of 16 KB takes 5.0 us a step with one block, 6.8 with four
 constexpr int kWaves = 8192, kItemBlocks = 4;
+constexpr int64_t kMaxItems = (1 << 26) - 4;  // a wave each: a grid has fewer than 2^32 threads
 
 struct Tensor {
     float* w;
@@ -271,18 +272,20 @@ __global__ void __launch_bounds__(256) adamw_one_kernel(StepArgs a) {
     if (threadIdx.x == 0) *a.done = 0u;
 }
 
-// the states in 8 bits as the values they stand for: one wave a block
+// the states in 8 bits as the values they stand for: one wave a block, further ones beyond the 2^22 of the largest grid (an axis of a grid
+// has fewer than 2^32 threads)
+constexpr int64_t kValuesGrid = 1 << 20;
 __global__ void __launch_bounds__(256)
 adamw_values_kernel(const uint32_t* __restrict__ m, const uint32_t* __restrict__ v, const uint8_t* __restrict__ m_scale,
                     const uint8_t* __restrict__ v_scale, int64_t blocks, float4* __restrict__ out_m, float4* __restrict__ out_root) {
-    const int64_t b = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (b >= blocks) return;
-    const int64_t i = b * 64 + (threadIdx.x & 63);
-    const uint32_t cm = m[i], cv = v[i];
-    const int em = m_scale[b], ev = v_scale[b];
-    out_m[i] = make_float4(decode_m(cm & 255u, em), decode_m(cm >> 8 & 255u, em), decode_m(cm >> 16 & 255u, em), decode_m(cm >> 24, em));
-    out_root[i] = make_float4(decode_root(cv & 255u, ev), decode_root(cv >> 8 & 255u, ev), decode_root(cv >> 16 & 255u, ev),
-                              decode_root(cv >> 24, ev));
+    for (int64_t b = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); b < blocks; b += (int64_t)gridDim.x * 4) {
+        const int64_t i = b * 64 + (threadIdx.x & 63);
+        const uint32_t cm = m[i], cv = v[i];
+        const int em = m_scale[b], ev = v_scale[b];
+        out_m[i] = make_float4(decode_m(cm & 255u, em), decode_m(cm >> 8 & 255u, em), decode_m(cm >> 16 & 255u, em), decode_m(cm >> 24, em));
+        out_root[i] = make_float4(decode_root(cv & 255u, ev), decode_root(cv >> 8 & 255u, ev), decode_root(cv >> 16 & 255u, ev),
+                                  decode_root(cv >> 24, ev));
+    }
 }
 
 }  // namespace
@@ -319,10 +322,10 @@ int rp_adamw_create(int device, int32_t n_tensors, const int64_t* numels, float*
             x.w = params[t], x.g = grads[t], x.copy = copies ? copies[t] : nullptr, x.n = n, x.first_block = first, x.pad = 0;
             x.vec = !((uintptr_t)x.w & 15) && !((uintptr_t)x.g & (4 * gs - 1)) && !((uintptr_t)x.copy & 7);
             const int64_t nb = (n + kBlock - 1) / kBlock;
+            if ((int64_t)items.size() + (nb + each - 1) / each > kMaxItems) return fail(RP_ERR_UNSUPPORTED, "too many elements");
             for (int64_t b = 0; b < nb; b += each) items.push_back({(uint32_t)t, (uint32_t)b});
             first += nb;
         }
-        if ((int64_t)items.size() >= ((int64_t)1 << 33)) return fail(RP_ERR_UNSUPPORTED, "too many elements");
         h = new rp_adamw;
         h->device = device, h->tensors = n_tensors, h->bits = state_bits, h->grad_type = grad_type;
         h->items = (int64_t)items.size(), h->blocks = first, h->each = each;
@@ -396,7 +399,7 @@ int rp_adamw_values(rp_adamw* h, float* exp_avg, float* root, void* stream) {
     DeviceGuard guard;
     int rc = guard.enter(h->device);
     if (rc) return rc;
-    hipLaunchKernelGGL(adamw_values_kernel, dim3((unsigned)((h->blocks + 3) / 4)), dim3(256), 0, (hipStream_t)stream,
+    hipLaunchKernelGGL(adamw_values_kernel, dim3((unsigned)std::min(kValuesGrid, (h->blocks + 3) / 4)), dim3(256), 0, (hipStream_t)stream,
                        (const uint32_t*)h->m, (const uint32_t*)h->v, h->m_scale, h->v_scale, h->blocks, (float4*)exp_avg, (float4*)root);
     HIP_TRY(hipGetLastError());
     return RP_OK;

@@ -1,5 +1,6 @@
 """Adapters beside the dense projection and AdamW: which stream a call takes, sizes at the limits, checked without a GPU."""
 import contextlib
+import ctypes
 
 import pytest
 import torch
@@ -110,3 +111,35 @@ def test_workspace_without_rows_holds_the_counts(dtype):
     for G in (701, 4000, 16383):
         for what in (nat.RP_ADAPT_GRADIENTS, nat.RP_ADAPT_GRADIENTS_DX):
             assert nat.load().rp_adapt_workspace_bytes(dtype, 0, 70, 20, G, 1, what) >= (5 * 4 + 16) * G
+
+
+def test_calls_whose_grids_would_not_fit_are_refused():
+    """An axis of a grid has fewer than 2^32 threads: sizes past that are refused before anything is launched, those below are not."""
+    lib = nat.load()
+    size = lambda dtype, what, **kw: lib.rp_adapt_workspace_bytes(  # noqa: E731
+        dtype, *(({"n": 1, "m": 64, "p": 1, "G": 1, "R": 1} | kw).values()), what)
+    project, banks, both = nat.RP_ADAPT_PROJECT, nat.RP_ADAPT_GRADIENTS, nat.RP_ADAPT_GRADIENTS_DX
+    most = 2 ** 31 - 513
+    for dtype, what, over, under in (
+            (nat.RP_F32, project, {"m": most}, {"m": most - 8192}),  # few rows: 2^23 blocks of 512 threads, 8 lines of 32 columns each
+            (nat.RP_F32, both, {"p": most}, {"p": most - 8192}),
+            (nat.RP_BF16, project, {"n": 2 ** 31 - 1, "p": 64}, {"n": 2 ** 30 - 4096, "p": 64}),  # 64 rows a block of the shrink
+            (nat.RP_BF16, banks, {"n": 2 ** 31 - 1}, {"n": 2 ** 30 - 4096}),
+            (nat.RP_BF16, banks, {"G": 16383, "m": 2 ** 24 + 2048}, {"G": 16383, "m": 65536}),  # 2^31 blocks of outer products
+            (nat.RP_F32, both, {"G": 16383, "m": 2 ** 23 + 2048}, {"G": 16383, "m": 65536, "p": 64})):
+        assert size(dtype, what, **under) > 0 and size(dtype, what, **over) == -1, (what, over, under)
+        assert b"one launch" in lib.rp_last_error()
+    a = 1 << 20  # never read
+    assert lib.rp_adapt_project_device(0, a, most + 1, nat.RP_F32, 1, most, a, 1, a, a, 1, 1, None, a, a, 1, None, a, 1 << 40, None) == nat.RP_ERR_UNSUPPORTED
+    assert lib.rp_adapt_gradients_device(0, a, 64, a, 2 ** 25, nat.RP_BF16, 1, 2 ** 24 + 2048, 1, None, a, a, 16383, 1, None, a, a, None, 0, a, 2 ** 25, 2 ** 25,
+                                         a, 1, 1, a, 1 << 50, None) == nat.RP_ERR_UNSUPPORTED
+
+
+def test_adamw_refuses_lists_whose_grid_would_not_fit():
+    """2^26 waves of 64 threads, a wave for 1024 elements: refused from the sizes alone, before any table is made."""
+    lib, a, h = nat.load(), 1 << 20, ctypes.c_void_p()
+    for sizes in ([2 ** 36], [2 ** 38], [2 ** 35, 2 ** 35, 1]):
+        T = len(sizes)
+        many = (ctypes.c_void_p * T)(*[a] * T)
+        rc = lib.rp_adamw_create(0, T, (ctypes.c_int64 * T)(*sizes), many, many, nat.RP_F32, None, 32, a, a, None, None, a, ctypes.byref(h))
+        assert rc == nat.RP_ERR_UNSUPPORTED and b"too many elements" in lib.rp_last_error() and not h

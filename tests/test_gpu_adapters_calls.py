@@ -3,7 +3,7 @@ that are not finite, every form of the shrink. Bounds as in test_gpu_adapters.py
 import pytest
 import torch
 
-from test_gpu_adapters import TYPE, check, make
+from test_gpu_adapters import TYPE, check, make, near
 
 pytestmark = pytest.mark.gpu
 
@@ -109,3 +109,62 @@ def test_no_rows_whatever_the_number_of_adapters(G, compute):
         assert not dd.any() and not du.any() and (Ct is None or dX.shape == (0, m))
         assert bool((bd[:, R] == 7).all()) and bool((bd[..., m:] == 7).all()) and bool((bu[..., p:] == 7).all())
         bd[:, :R, :m], bu[..., :p] = 7.0, 7.0
+
+
+def test_gradients_of_many_adapters_and_columns():
+    """16.8 million blocks of outer products, more than a row of 2^32 threads holds: d_down of 4.3 GB, a few adapters of it with rows."""
+    from randomprojection_amd.adapters import adapted_project_backward_device
+
+    n, m, p, G, used = 600, 65536, 64, 16383, [0, 77, 8191, 16382]
+    g = torch.Generator(device="cuda").manual_seed(1)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    X, dY, down, up, hidden = r(n, m), r(n, p), r(G, 1, m), r(G, 1, p), r(n, 1)
+    ids = torch.tensor(used + [-1], device="cuda", dtype=torch.int32)[torch.arange(n, device="cuda") % 5]
+    _, dd, du = adapted_project_backward_device(dY, X, None, down, up, ids, hidden)
+    rest = torch.ones(G, dtype=torch.bool, device="cuda")
+    rest[used] = False
+    for part in torch.nonzero(rest)[:, 0].split(2048):
+        assert not dd[part].any() and not du[part].any()
+    for a in used:
+        at = ids == a
+        x, dy, h, u = X[at].double(), dY[at].double(), hidden[at].double(), up[a, 0].double()
+        near(dd[a, 0], (dy @ u) @ x, (dy.abs() @ u.abs()) @ x.abs(), n + p + 8)
+        near(du[a, 0], h[:, 0] @ dy, h[:, 0].abs() @ dy.abs(), n + 8)
+
+
+@pytest.mark.parametrize("compute", ["bf16", "fp32"])
+def test_product_of_more_tiles_than_a_row_of_the_grid(compute):
+    """Over 2^20 tiles: rows of the grid's blocks come after each other. X of 17 GB; rows drawn from all of it."""
+    from randomprojection_amd.adapters import adapted_project_device
+
+    n, m, p, G, R = 2 ** 27 + 77, 64 if compute == "bf16" else 32, 1, 3, 1
+    g = torch.Generator(device="cuda").manual_seed(1)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda", dtype=TYPE[compute])  # noqa: E731
+    X, C, down, up = r(n, m), r(p, m), r(G, R, m), r(G, R, p)
+    ids = (torch.arange(n, device="cuda") * 4 // n - 1).int()
+    Y, h = adapted_project_device(X, C, down, up, ids, compute=compute, return_hidden=True)
+    rows = torch.cat([torch.randint(0, n, (5000,), generator=g, device="cuda"), torch.arange(n - 200, n, device="cuda"), torch.arange(200, device="cuda")])
+    x, a = X[rows].double(), ids[rows].long()
+    d, u = (torch.where((a >= 0)[:, None], b[a, 0].double(), 0.0) for b in (down, up))
+    hid, size = (x * d).sum(1), (x * d).abs().sum(1)
+    near(h[rows, 0], hid, size, m + 8)
+    near(Y[rows, 0], x @ C[0].double() + hid * u[:, 0], x.abs() @ C[0].double().abs() + size * u[:, 0].abs(), m + R + 8)
+
+
+def test_values_of_more_blocks_than_the_grid():
+    """Over 2^22 blocks of states in 8 bits: 1.07 billion elements, their values as they are held by an optimizer of the last ones alone."""
+    from randomprojection_amd.optim import AdamW
+
+    n, tail = 2 ** 30 + 1000, 3 * 2 ** 18
+    g = torch.Generator(device="cuda").manual_seed(1)
+    w, grad = torch.zeros(n, device="cuda"), torch.randn(n, device="cuda", generator=g, dtype=torch.bfloat16)
+    opt = AdamW([w], [grad], state_bits=8)
+    opt.step()
+    first = n // 256 * 256 - tail
+    alone = AdamW([w[first:]], [grad[first:]], state_bits=8)
+    held, own = opt.state_dict(), alone.state_dict()
+    alone.load_state_dict({k: (v if k == "steps" else v.view(torch.uint8)[-own[k].numel():].view(v.dtype)) for k, v in held.items()})
+    for a, b in zip(opt.state_values(), alone.state_values()):
+        assert a.numel() == held["exp_avg"].numel() and b.any() and torch.equal(a[-b.numel():], b)
+        middle = a[2 ** 29:2 ** 29 + 10 ** 6].double()
+        assert bool(middle.any()) and bool(torch.isfinite(middle).all())

@@ -390,6 +390,15 @@ __device__ __forceinline__ void split3(float x, uint32_t& hi, uint32_t& mid, uin
     mid = __float_as_uint(y) & 0xffff0000u;
     low = __float_as_uint(y - __uint_as_float(mid)) & 0xffff0000u;
 }
+// What mid and low are multiplied by: bf16 values with the largest finite one for an infinity or a NaN. Against an infinity itself a mid or
+// low of 0 would make a NaN; hi, which has it, is 0 only where x is (or under 2^-133), and a mid or low that is not 0 has the sign of hi. Under
+// what one box varies by: gradients of 16384 x 16384 -> 1024 703 us, 707 without; 1777 x 4096 -> 4096 of rank 64 100 to 103, 101 to 103 without.
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t finite(uint32_t x) {
+    const u16x2 y = __builtin_elementwise_min(__builtin_bit_cast(u16x2, x & 0x7fff7fffu), u16x2{0x7f7f, 0x7f7f});
+    return (__builtin_bit_cast(uint32_t, y) & 0x7fff7fffu) | (x & 0x80008000u);
+}
+__device__ __forceinline__ uint4 finite(uint4 x) { return make_uint4(finite(x.x), finite(x.y), finite(x.z), finite(x.w)); }
 // the upper halves of a (low half of the result) and b
 __device__ __forceinline__ uint32_t pack_high(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
 __device__ __forceinline__ uint32_t pack_low(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
@@ -624,11 +633,11 @@ __global__ void __launch_bounds__(256, KT == 1 ? 4 : 2) outer_kernel(OuterArgs a
             for (int j = 0; j < 8; ++j) {
                 const auto word = [&](int i) { return j / 2 == 0 ? z[i].x : j / 2 == 1 ? z[i].y : j / 2 == 2 ? z[i].z : z[i].w; };
                 const auto pair = [&](int i) { return j & 1 ? pack_high(word(i), word(i + 1)) : pack_low(word(i), word(i + 1)); };
-                const uint4 zc = make_uint4(pair(0), pair(2), pair(4), pair(6));
+                const uint4 zc = make_uint4(pair(0), pair(2), pair(4), pair(6)), zf = finite(zc);
 #pragma unroll
                 for (int k = 0; k < KT; ++k)
 #pragma unroll
-                    for (int s = 0; s < 3; ++s) acc[k][j] = mma<T>(hp[k][s], zc, acc[k][j]);
+                    for (int s = 0; s < 3; ++s) acc[k][j] = mma<T>(hp[k][s], s ? zf : zc, acc[k][j]);
             }
         } else {
 #pragma unroll
@@ -946,7 +955,10 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& a, const Groups& o, un
             const uint4* st = lds + buf * BLOCK;
             const uint4* sw = st + PARTS * BM * 4;
 #pragma unroll
-            for (int ni = 0; ni < NN; ++ni) fb[0][ni] = sw[(rb + ni * 16) * 4 + (fq ^ F(rb + ni * 16))];
+            for (int ni = 0; ni < NN; ++ni) {
+                fb[0][ni] = sw[(rb + ni * 16) * 4 + (fq ^ F(rb + ni * 16))];
+                if constexpr (PARTS > 1) fb[1][ni] = finite(fb[0][ni]);  // here: between the products it spills 9 to 11 registers
+            }
 #pragma unroll
             for (int mi = 0; mi < MT; ++mi) {
                 const int r = ra + mi * 16;
@@ -958,7 +970,7 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& a, const Groups& o, un
                 for (int u = 0; u < PARTS; ++u) {
                     const uint4 h = st[(u * BM + r) * 4 + (fq ^ F(r))];
 #pragma unroll
-                    for (int ni = 0; ni < NN; ++ni) x[ni] = mma<T>(fb[0][ni], h, x[ni]);
+                    for (int ni = 0; ni < NN; ++ni) x[ni] = mma<T>(fb[u ? 1 : 0][ni], h, x[ni]);
                 }
                 if (r >= p0 && r < p1)
 #pragma unroll

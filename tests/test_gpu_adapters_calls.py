@@ -3,7 +3,7 @@ that are not finite, every form of the shrink. Bounds as in test_gpu_adapters.py
 import pytest
 import torch
 
-from test_gpu_adapters import TYPE, check, make, near
+from test_gpu_adapters import TYPE, check, formulas, make, near
 
 pytestmark = pytest.mark.gpu
 
@@ -168,3 +168,32 @@ def test_values_of_more_blocks_than_the_grid():
         assert a.numel() == held["exp_avg"].numel() and b.any() and torch.equal(a[-b.numel():], b)
         middle = a[2 ** 29:2 ** 29 + 10 ** 6].double()
         assert bool(middle.any()) and bool(torch.isfinite(middle).all())
+
+
+@pytest.mark.parametrize("compute", ["bf16", "fp32"])
+@pytest.mark.parametrize("n,m,p,R", [(40, 70, 90, 6), (700, 70, 90, 6), (20000, 70, 90, 6), (20000, 130, 150, 40), (35000, 64, 50, 20)])
+def test_infinities_are_those_of_the_formulas(n, m, p, R, compute):
+    """An infinity in an operand gives what the formulas give, an infinity or a NaN, whatever the number of rows. All values are small
+    whole numbers and halves, whose products and sums are exact in f32, and whose pieces of fewer bits are zeros mostly."""
+    from randomprojection_amd.adapters import adapted_project_backward_device, adapted_project_device
+
+    G, inf = 6, float("inf")
+    g = torch.Generator().manual_seed(n)
+    pick = lambda *s: torch.randint(1, 3, s, generator=g).float() * (torch.randint(0, 2, s, generator=g) * 2 - 1)  # noqa: E731
+    t = {"X": pick(n, m), "C": pick(p, m), "down": pick(G, R, m), "up": pick(G, R, p), "dY": pick(n, p)}
+    t["up"][2, 1, 5], t["up"][3, R - 1, 7], t["up"][4, 0, p - 1], t["down"][1, 2, 9], t["down"][2, 0, m - 1] = inf, -inf, inf, inf, -inf
+    t["X"][8, 33], t["X"][13, 0], t["X"][n - 1, 1], t["dY"][22, 5], t["dY"][n - 3, p - 1] = inf, -inf, inf, -inf, inf  # of adapters 0 and 5, ..
+    t = {k: v.to(TYPE[compute]) for k, v in t.items()}
+    t["scale"] = torch.tensor([1.0, 0.5, 2.0, -1.0, 0.0, 1.5])
+    t["ids"] = (torch.arange(n) % (G + 1) - 1).int()
+    u = {k: v.cuda() for k, v in t.items()}
+    kw = dict(scale=u["scale"], compute=compute)
+    Y, h = adapted_project_device(u["X"], u["C"], u["down"], u["up"], u["ids"], return_hidden=True, **kw)
+    got = dict(zip(("dX", "d_down", "d_up"), adapted_project_backward_device(u["dY"], u["X"], u["C"].T, u["down"], u["up"], u["ids"], h, **kw)))
+    got |= {"Y": Y, "hidden": h}
+    want, _ = formulas(t, h.cpu())
+    for k, x in got.items():
+        a, b = x.cpu(), want[k].to(x.dtype)
+        same = (a == b) | (a.isnan() & b.isnan())
+        assert same.all(), (k, torch.nonzero(~same)[:4].tolist(), a[~same][:4], b[~same][:4])
+        assert b.isinf().any() and b.isfinite().any(), k

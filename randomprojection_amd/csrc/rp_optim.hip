@@ -14,8 +14,17 @@
 // Rounding to a code is stochastic: the 20 mantissa bits that are dropped are first added to 16 random
 // bits (a hash of seed, step, tensor and element). With b2 = 0.999 a step changes v by 0.1 % while two
 // codes lie 6 to 12 % apart: rounding to the nearest would keep every v where its largest gradient
-// put it; rounded at random the expected value is the exact one.
+// put it; rounded at random the expected root is the exact one (and v, its square, larger by the rounding's variance: under 0.0125 %
+// of v a step).
+// One m is not rounded at random. The least code of m stands for 2^-17 to 2^-16 of the block's largest, far over the
+// least root's 2^-33: an m below it would now and then become one that its root, held well, turns into a step of
+// many lr. But whatever the gradients are they leave |m| <= B sqrt(v) (Cauchy and Schwarz on the two sums), with
+// B^2 = (1 - b1)^2 / ((1 - b2) (1 - b1^2 / b2)), B = 7.3 with the usual betas. Where the least code is more than B root it is
+// not taken and m becomes 0. Such an element, its root under 2^-19 or so of the block's largest m, then moves by its
+// current gradient's share of m alone, at (1 - b1) of its pace. Without the rule a steady gradient of 1e-7 beside one of 1
+// made steps of 190 lr, one of 1e-9 steps of 12000 lr (eps = 0).
 // A block that holds a NaN or an infinity gets e = 255 and stands for NaN from then on.
+#include <cmath>
 #include <new>
 #include <vector>
 
@@ -100,10 +109,12 @@ __device__ __forceinline__ float decode_root(uint32_t c, int e) {
     const float x = __uint_as_float(c << 20) * 0x1p96f * power(e - 126);
     return e == 255 ? __uint_as_float(0x7fc00000u) : x;
 }
-__device__ __forceinline__ uint32_t encode_m(float m, int e, uint32_t rnd) {
+// most: B root
+__device__ __forceinline__ uint32_t encode_m(float m, int e, uint32_t rnd, float most) {
     if (e == 255) return 0u;
-    const uint32_t t = __float_as_uint(fabsf(m) * power(134 - e) * 0x1p-120f);
-    return ((t + rnd) >> 20) | (__float_as_uint(m) >> 31 << 7);
+    const float by = power(134 - e);
+    const uint32_t t = __float_as_uint(fabsf(m) * by * 0x1p-120f), limit = __float_as_uint(most * by * 0x1p-120f), sign = __float_as_uint(m) >> 31 << 7;
+    return max(t, limit) < 1u << 20 ? sign : ((t + rnd) >> 20) | sign;
 }
 __device__ __forceinline__ uint32_t encode_root(float r, int e, uint32_t rnd) {
     if (e == 255) return 0u;
@@ -130,7 +141,7 @@ struct StepArgs {
     int32_t each;  // blocks of an item
     void *m, *v;
     uint8_t *m_scale, *v_scale;
-    float b1, c1, b2, c2, eps, keep;  // c = 1 - b, keep = 1 - lr decay
+    float b1, c1, b2, c2, eps, keep, bound;  // c = 1 - b, keep = 1 - lr decay, bound: B above
     // for one launch
     Numbers x;
     int32_t* steps;
@@ -216,7 +227,7 @@ __device__ __forceinline__ void step_item(const StepArgs& a, const Item& it, con
             uint32_t cm = 0u, cv = 0u;
             for (int k = 0; k < 4; ++k) {
                 const uint32_t rnd = mix((uint32_t)(at + k) ^ key);
-                cm |= encode_m(m[k], em, (rnd >> 16 << 4) + 8u) << (8 * k);
+                cm |= encode_m(m[k], em, (rnd >> 16 << 4) + 8u, root[k] * a.bound) << (8 * k);
                 cv |= encode_root(root[k], ev, ((rnd & 0xffffu) << 4) + 8u) << (8 * k);
             }
             *reinterpret_cast<uint32_t*>((uint8_t*)a.m + state) = cm;
@@ -365,10 +376,12 @@ int rp_adamw_step(rp_adamw* h, double lr, double beta1, double beta2, double eps
     int rc = guard.enter(h->device);
     if (rc) return rc;
     hipStream_t st = (hipStream_t)stream;
+    // no bound where b1^2 >= b2: gradients can leave any m then
+    const double bound = beta1 * beta1 < beta2 ? (1.0 - beta1) / sqrt((1.0 - beta2) * (1.0 - beta1 * beta1 / beta2)) : INFINITY;
     const Numbers x{lr, beta1, beta2, (uint32_t)seed, (uint32_t)(seed >> 32)};
     const StepArgs a{(const Tensor*)h->table.p, (const Item*)h->list.p, (const Scalars*)h->scalars.p, h->items, h->each, h->m, h->v, h->m_scale,
                      h->v_scale, (float)beta1, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps,
-                     (float)(1.0 - lr * weight_decay), x, h->steps, active, h->tensors, (uint32_t*)h->done.p};
+                     (float)(1.0 - lr * weight_decay), (float)bound, x, h->steps, active, h->tensors, (uint32_t*)h->done.p};
     const dim3 grid((unsigned)((h->items + 3) / 4)), block(256);
     const bool g16 = h->grad_type == RP_BF16;
     if (h->items && h->items <= kOneLaunch && h->tensors <= kOneTensors) {

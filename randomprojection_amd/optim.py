@@ -47,7 +47,9 @@ class AdamW:
 
     state_bits 32 holds m and v in float32; state_bits 8 holds m and sqrt(v) in a byte each, in blocks of 256 elements
     with one power-of-two scale, rounded at random by ``seed`` (hashed with the step, the tensor and the element: the same
-    seed gives the same bits). A gradient that is not finite makes its element's state NaN, with 8 bits its block's."""
+    seed gives the same bits). An m under the least of its block's codes, 2^-17 to 2^-16 of the largest m, is held as 0 where that code is
+    more than its root allows: elements whose gradients are under some 2^-19 of their block's largest move by their current
+    gradient alone, slower by 1 - b1. A gradient that is not finite makes its element's state NaN, with 8 bits its block's."""
 
     def __init__(self, params, grads, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, *, state_bits=32,
                  copies=None, seed=0):

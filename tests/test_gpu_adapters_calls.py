@@ -197,3 +197,55 @@ def test_infinities_are_those_of_the_formulas(n, m, p, R, compute):
         same = (a == b) | (a.isnan() & b.isnan())
         assert same.all(), (k, torch.nonzero(~same)[:4].tolist(), a[~same][:4], b[~same][:4])
         assert b.isinf().any() and b.isfinite().any(), k
+
+
+@pytest.mark.parametrize("kind", ["steady", "random", "one burst"])
+@pytest.mark.parametrize("betas", [(0.9, 0.999), (0.0, 0.99), (0.95, 0.95)])
+def test_small_gradients_beside_large_ones_in_8_bits(betas, kind):
+    """Elements whose gradients are far below their block's largest: the least code of m is taken only where B root covers it, and steps
+    stay near what AdamW can make.
+
+    Each step's codes are compared with m and the root in f32 from the values held before it: an m under the least code l is held as 0 where
+    l > B root, as 0 or l elsewhere; other m as one of the codes on its two sides (1e-5 aside, for the roundings in B root).
+    A steady gradient under l, which only grows while the block's largest m does, leaves m in {0, l}: b1 l + (1 - b1) |g| < l. l is held where it
+    is at most B root, a code of the root is at least 8/9 of it, and root' >= sqrt(b2) root_held, sqrt(1 - b2) |g|: so
+    |m'| / root' <= b1 B (9/8) / sqrt(b2) + (1 - b1) / sqrt(1 - b2). Roots too small for 8/9 (under 2^-30 of the largest) never hold l. The
+    step is lr sqrt(1 - b2^t) / (1 - b1^t) times that."""
+    from randomprojection_amd.optim import AdamW
+
+    (b1, b2), lr, steps, ratios = betas, 1e-3, 600, [1e-4, 1e-5, 1e-6, 1e-7, 1e-8, 1e-9, 1e-12]
+    B = (1 - b1) / ((1 - b2) * (1 - b1 ** 2 / b2)) ** 0.5
+    most = (b1 * B * 9 / 8 / b2 ** 0.5 + (1 - b1) / (1 - b2) ** 0.5) * max((1 - b2 ** t) ** 0.5 / (1 - b1 ** t) for t in range(1, steps + 1))
+    scale = torch.tensor(ratios, device="cuda")[:, None].expand(-1, 1024).clone()
+    scale[:, ::256] = 1.0  # one in each block of 256
+    grad, w = scale.clone(), torch.zeros_like(scale)
+    opt = AdamW(list(w), list(grad), lr=lr, betas=betas, eps=0.0, weight_decay=0.0, state_bits=8, seed=3)
+    rand = torch.Generator(device="cuda").manual_seed(2)
+    largest, before = torch.zeros_like(w), w.clone()
+    m0, r0 = opt.state_values()
+    refused = taken = 0
+    for t in range(steps):
+        if kind == "random":
+            grad.copy_(scale * torch.randn(scale.shape, device="cuda", generator=rand))
+        elif kind == "one burst" and t == 300:
+            grad.mul_(torch.where(scale < 1, 30.0, 1.0))
+        elif kind == "one burst" and t == 301:
+            grad.copy_(scale)
+        opt.step()
+        largest = torch.maximum(largest, (w - before).abs())
+        before.copy_(w)
+        g = grad.view(-1)
+        m, root = (m0 * b1 + g * (1 - b1)).abs(), (r0 * r0 * b2 + g * g * (1 - b2)).sqrt()
+        least = ((m.view(28, 256).amax(1).view(torch.int32) >> 23) - 16 << 23).view(torch.float32).repeat_interleave(256)  # 2^-16 of its binade
+        m0, r0 = opt.state_values()
+        held, under = m0.abs(), m < least * (1 - 1e-5)
+        refuse, take = under & (least > B * root * (1 + 1e-5)), under & (least < B * root * (1 - 1e-5))
+        assert not held[refuse].any() and ((held == 0) | (held == least))[under].all()
+        assert ((held - m).abs() <= torch.maximum(least, m / 8)).all()
+        refused, taken = refused + int((refuse & (m > 0)).sum()), taken + int((held[take] > 0).sum())
+    assert refused and taken and torch.isfinite(w).all()
+    if kind == "steady":
+        small = scale[:, 1] <= 1e-7
+        # 1e-5 for the roundings in the step, and half a step of w for its own
+        assert (largest.amax(1) <= lr * most * (1 + 1e-5) + w.abs().amax(1) * 2.0 ** -24)[small].all(), (largest.amax(1) / lr, most)
+        assert (w < 0).all()  # each moves against its gradient, the small ones too

@@ -209,3 +209,5 @@ class AdaptedGaussianProjection(GaussianRandomProjection):
 
     def __setstate__(self, state):
         self.__dict__.update(state)
+        if "_down" in state and "_seed" not in state:  # a pickle of an estimator that did not keep the seed of its fit
+            self._seed = int(self.seed)

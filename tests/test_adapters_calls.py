@@ -143,3 +143,18 @@ def test_adamw_refuses_lists_whose_grid_would_not_fit():
         many = (ctypes.c_void_p * T)(*[a] * T)
         rc = lib.rp_adamw_create(0, T, (ctypes.c_int64 * T)(*sizes), many, many, nat.RP_F32, None, 32, a, a, None, None, a, ctypes.byref(h))
         assert rc == nat.RP_ERR_UNSUPPORTED and b"too many elements" in lib.rp_last_error() and not h
+
+
+def test_a_state_without_the_seed_of_its_fit_takes_the_one_it_has():
+    import numpy as np
+
+    from randomprojection_amd import AdaptedGaussianProjection
+
+    est = AdaptedGaussianProjection(n_components=7, n_adapters=3, rank=2, random_state=5, seed=4)
+    again = AdaptedGaussianProjection()
+    again.__setstate__(est.__getstate__())  # not fitted
+    assert not hasattr(again, "_seed")
+    state = est.fit(np.random.default_rng(0).standard_normal((20, 33))).__getstate__()
+    for state, seed in ((state, 4), ({k: v for k, v in state.items() if k != "_seed"} | {"seed": 6}, 6)):
+        again.__setstate__(state)
+        assert again._seed == seed

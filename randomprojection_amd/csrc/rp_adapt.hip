@@ -1600,6 +1600,7 @@ int launch_some(const Plan& l, const T* X, int64_t ldx, const T* C, int64_t kp, 
 // products, and of the others fewer than 2^32 threads.
 int check_call(int32_t dtype, int64_t n, int64_t m, int64_t p, int64_t G, int32_t R, int what) {
     if (const int rc = check_shared(dtype, n, m, p, G, R)) return rc;
+    if (what < RP_ADAPT_PROJECT || what > RP_ADAPT_GRADIENTS_DX) return fail(RP_ERR_INVALID, "what must be one of RP_ADAPT_*");
     const int es = dtype == RP_BF16 ? 2 : 4;
     const bool forward = what == RP_ADAPT_PROJECT;
     const int64_t width = forward ? p : m, made = what == RP_ADAPT_GRADIENTS ? 0 : width, row_bytes = padded(forward ? m : p, dtype) * es;

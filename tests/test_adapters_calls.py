@@ -158,3 +158,10 @@ def test_a_state_without_the_seed_of_its_fit_takes_the_one_it_has():
     for state, seed in ((state, 4), ({k: v for k, v in state.items() if k != "_seed"} | {"seed": 6}, 6)):
         again.__setstate__(state)
         assert again._seed == seed
+
+
+def test_workspace_of_no_such_call_is_refused():
+    lib = nat.load()
+    for what in (-1, 3, 7):
+        for n in (0, 3, 1000):
+            assert lib.rp_adapt_workspace_bytes(nat.RP_BF16, n, 100, 50, 4, 8, what) == -1 and b"what" in lib.rp_last_error()

@@ -723,8 +723,8 @@ __global__ void __launch_bounds__(256) outer_join_kernel(OuterArgs a0, OuterArgs
 // at a time, and are multiplied into registers of their own, from where only the adapter's rows are added: a value that is
 // not finite in one adapter reaches no other's rows. The result goes through LDS so that rows are stored 128 bytes at a
 // time (16 rows a store otherwise: a tenth longer at 16384 x 1024 -> 16384 with bf16 out).
-// Measured: 65536 x 16384 -> 1024 1.61 ms with rank 16, 1.37 PFLOP/s, matrix units busy 0.71 of the time; 16384 x 1024 -> 16384 with bf16
-// out 0.60 ms, busy half of it: 16 stages a tile, and a unit holds one tile, whose first loads, adapters (0.05 ms in all) and stores (0.05
+// Measured: 65536 x 16384 -> 1024 1.61 to 1.68 ms with rank 16, 1.34 PFLOP/s, matrix units busy 0.72 of the time; 16384 x 1024 -> 16384 with bf16
+// out 0.60 to 0.62 ms, busy half of it: 16 stages a tile, and a unit holds one tile, whose first loads, adapters (0.05 ms in all) and stores (0.05
 // ms) nothing overlaps. Blocks that go from tile to tile and load the next one's first stage behind the stores need more than the 256
 // registers that a tile of 256 x 256 leaves nothing of: what is spilled made it 0.92 ms.
 struct GemmArgs {
@@ -998,7 +998,8 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm_kernel(GemmArgs a, Group
 //  * 128 rows of C by all rows over up to 8 lines (128 bytes) of the contraction: the rows' lines go to LDS directly, a line a wave,
 //    each wave loads its 16 rows of C into registers, all at once, and everyone waits once;
 //  * 16 KT ranks of one adapter by its rows (16 at a time) over a range of lines: the 8 waves take an eighth each and add up in LDS.
-// Bound by reading C and the used adapters' down (73 MB at 64 x 16384 -> 1024 with 64 adapters of rank 16: 18 us, 4.1 TB/s). A second launch adds the
+// Bound by reading C and the used adapters' down: 64 x 16384 -> 1024 with 38 of 64 adapters of rank 16 in use takes 18 us and reads 73 MB (4.1 TB/s),
+// 54 of them C and down, the rest X, which each XCD reads whole for its eighth of C (17), and once more for the adapters. A second launch adds the
 // ranges, in order, and expands: a lane four columns of one row. No sort: the rows of an adapter are found by comparing up to 64 ids, a
 // lane an id. Replayed in a graph, against the launches of more rows: 21 and 26 us there, 10 and 15 us at 16 x 4096 -> 1024.
 constexpr int kFewRows = 64, kFewWaves = 8, kFewLines = 8;
@@ -1401,8 +1402,8 @@ Plan plan_for(int32_t dtype, int64_t n, int64_t m, int64_t p, int64_t G, int R, 
     // joined in 11 us, 17 with 512 rows)
     l.chunk_rows = (int)std::max<int64_t>(512, std::min<int64_t>(kMaxChunk, n * ((m + 127) / 128) / 2048 / 64 * 64));
     l.small = n <= kSmallRows && G <= 700;
-    // rows of a wave: 128 waves and more, of up to 2048 rows, unless the counts to scan become more than a million (4 million rows, 32
-    // adapters: 0.10 ms, 0.70 with 128 waves)
+    // rows of a wave: 256 at least, which is fewer than 128 waves under 32768 rows, then 128 waves and more, of up to 2048 rows, unless the
+    // counts to scan become more than a million (4 million rows, 32 adapters: 0.10 ms, 0.70 with 128 waves)
     l.each = std::min<int64_t>(2048, std::max<int64_t>(256, (n / 128 + 63) / 64 * 64));
     while ((n + l.each - 1) / l.each * (G + 1) > (1 << 20)) l.each *= 2;
     l.n_chunks = l.small ? 0 : (int)std::max<int64_t>(1, (n + l.each - 1) / l.each);  // one without rows too: the lists come from its counts

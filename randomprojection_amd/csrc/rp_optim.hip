@@ -109,12 +109,12 @@ __device__ __forceinline__ float decode_root(uint32_t c, int e) {
     const float x = __uint_as_float(c << 20) * 0x1p96f * power(e - 126);
     return e == 255 ? __uint_as_float(0x7fc00000u) : x;
 }
-// most: B root
+// most: B root (a NaN, as of an infinite B and a root of 0, keeps nothing back)
 __device__ __forceinline__ uint32_t encode_m(float m, int e, uint32_t rnd, float most) {
     if (e == 255) return 0u;
-    const float by = power(134 - e);
-    const uint32_t t = __float_as_uint(fabsf(m) * by * 0x1p-120f), limit = __float_as_uint(most * by * 0x1p-120f), sign = __float_as_uint(m) >> 31 << 7;
-    return max(t, limit) < 1u << 20 ? sign : ((t + rnd) >> 20) | sign;
+    const float least = power(e - 143);  // what code 1 stands for
+    const uint32_t t = __float_as_uint(fabsf(m) * power(134 - e) * 0x1p-120f), sign = __float_as_uint(m) >> 31 << 7;
+    return fabsf(m) < least && most < least ? sign : ((t + rnd) >> 20) | sign;
 }
 __device__ __forceinline__ uint32_t encode_root(float r, int e, uint32_t rnd) {
     if (e == 255) return 0u;

@@ -266,8 +266,9 @@ def test_many_adapters_and_wide_rows():
     check(t, "bf16")
 
 
-# with 128 tiles and more the product is one launch of whole contractions, with 192 larger ones of the larger tile; over 8192 rows or 700
-# adapters are grouped by several blocks; from 32768 rows on (16384 over rank 64) the shrink takes more rows at a time
+# products of few tiles are split over the contraction where that takes less time than the tiles leave idle, others whole, in tiles of 128 or of
+# 256 rows and columns, whichever takes less time; over 8192 rows or 700 adapters are grouped by several blocks; from 32768 rows on (16384 over
+# rank 64) the shrink takes more rows at a time
 LARGE = [(2049, 1100, 1150, 7, 40), (3001, 1030, 700, 3, 128), (2050, 4100, 1090, 700, 1), (4100, 2950, 3000, 11, 17), (9001, 200, 2000, 5, 64),
          (8193, 64, 64, 701, 4), (8192, 100, 130, 700, 2), (33000, 96, 1040, 3, 9), (17000, 72, 1101, 2, 100), (20000, 128, 300, 5000, 2),
          (300, 70, 65, 16383, 1)]

@@ -249,3 +249,19 @@ def test_small_gradients_beside_large_ones_in_8_bits(betas, kind):
         # 1e-5 for the roundings in the step, and half a step of w for its own
         assert (largest.amax(1) <= lr * most * (1 + 1e-5) + w.abs().amax(1) * 2.0 ** -24)[small].all(), (largest.amax(1) / lr, most)
         assert (w < 0).all()  # each moves against its gradient, the small ones too
+
+
+def test_least_code_where_gradients_bound_nothing():
+    """b1^2 >= b2: any m can lie beside any root, so every m under the least code is rounded at random."""
+    from randomprojection_amd.optim import AdamW
+
+    g = torch.full((4096,), 1e-6, device="cuda")
+    g[::256] = 1.0
+    opt = AdamW([torch.zeros(4096, device="cuda")], [g], betas=(0.95, 0.9), state_bits=8, lr=1e-3)
+    opt.step()
+    held = opt.state_values()[0]
+    small = g < 1
+    # m = 5e-8, the least code 2^-16 of the binade of 0.05, 4.8e-7: about a tenth of 4080 are held as it (standard deviation 19)
+    least = 2.0 ** -5 * 2.0 ** -16
+    assert ((held == 0) | (held == least))[small].all() and 300 < int((held[small] > 0).sum()) < 560
+    assert torch.isfinite(opt.params[0]).all()

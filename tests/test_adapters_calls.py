@@ -165,3 +165,23 @@ def test_workspace_of_no_such_call_is_refused():
     for what in (-1, 3, 7):
         for n in (0, 3, 1000):
             assert lib.rp_adapt_workspace_bytes(nat.RP_BF16, n, 100, 50, 4, 8, what) == -1 and b"what" in lib.rp_last_error()
+
+
+def test_loads_to_lds_wait_for_their_destination():
+    """A load to LDS takes its destination from M0 and needs one instruction between it and the write of M0; the compiler puts it there, inline
+    asm has to."""
+    import pathlib
+    import re
+
+    import randomprojection_amd
+
+    found = 0
+    for source in sorted((pathlib.Path(randomprojection_amd.__file__).parent / "csrc").glob("*.hip")):
+        for text in re.findall(r'asm volatile\(((?:\s*"(?:[^"\\]|\\.)*")+)', source.read_text()):
+            steps = [s.strip() for s in re.sub(r'"\s*"', "", text).strip().strip('"').replace("\\t", "").split("\\n")]
+            for i, s in enumerate(steps):
+                if "load_lds" in s or ("buffer_load" in s and s.endswith("lds")):
+                    found += 1
+                    writes = [k for k in range(i) if " m0," in steps[k]]
+                    assert writes and i - writes[-1] >= 2, (source.name, steps)
+    assert found
